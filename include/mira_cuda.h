@@ -443,6 +443,135 @@ int mira_cuda_dynamic_slice(const mira_view4* x, const int64_t* x_dims, const in
 int mira_cuda_dynamic_update_slice(const mira_view4* x, const int64_t* x_dims, const mira_view4* upd,
                                    const int64_t* upd_dims, const int32_t* start, int64_t rank);
 
+/* ---------------------------------------------------------------- paged decoding
+ *
+ * Serving sequences of different lengths: keys and values live in fixed-size pages of a pool, a
+ * table lists each sequence's pages in order, and position t of sequence b is slot t % page_size of
+ * page table[b * table_ld + t / page_size].  The reference has no counterpart (its decode keeps one
+ * contiguous cache per layer, ops.py:533-576); the softmax and the products are those of
+ * ops.py:310-313 and ops.py:217-219.  Lengths and tables are device memory, read by the kernels, so
+ * a captured graph stays valid while they change.  A negative length or one beyond the table's
+ * max_pages * page_size, or a page id outside [0, num_pages), touches no memory outside the pool:
+ * the kernel leaves those tokens out and the next mira_cuda_sync fails with MIRA_CUDA_EKERNEL. */
+
+/* element types */
+#define MIRA_DT_F32 0
+#define MIRA_DT_F16 1
+#define MIRA_DT_BF16 2
+#define MIRA_DT_I8 3            /* pages only: value = code * the scale of its (page, head, slot) row */
+
+#define MIRA_PAGED_DH_MAX 256   /* head dimension */
+
+typedef struct mira_paged_kv {
+  int64_t num_pages, page_size, kv_heads, dh;
+  int64_t batch;              /* sequences */
+  int64_t max_pages;          /* pages a sequence may have: entries used of a table row */
+  int64_t table_ld;           /* entries between table rows, >= max_pages */
+  mira_view4 k, v;            /* element strides over (page, kv head, slot, element); stride[3] == 1 */
+  mira_view4 k_scale, v_scale;  /* MIRA_DT_I8: f32 scales over (page, kv head, slot); stride[3] unused */
+  const int32_t* table;       /* [batch][table_ld] page ids; entries past a sequence's last page unused */
+  const int32_t* lengths;     /* [batch] tokens of each sequence (0: an empty slot of the batch) */
+  int32_t dtype;              /* MIRA_DT_* of k and v */
+  int32_t reserved;           /* 0 */
+} mira_paged_kv;
+
+/* New rows into the pages: sequence b receives rows [row_start[b], row_start[b + 1]) (row_start NULL:
+ * one row per sequence, row b; rows == batch) as its LAST positions, i.e. lengths[b] already counts
+ * them and row row_start[b] + i goes to position lengths[b] - n_b + i.  A sequence of length 0 takes
+ * no row.  Values are rounded once to the pages' type (nearest even); MIRA_DT_I8 rows get
+ * scale = absmax / 127 (1 for a row of zeros) and codes clip(rint(x / scale), -127, 127).  Every
+ * position must be in a page that no other sequence holds; pages shared after a fork are only read. */
+typedef struct mira_kv_append {
+  mira_paged_kv kv;
+  int64_t rows;
+  mira_view4 k_new, v_new;    /* element strides over (-, kv head, row, element); stride[3] == 1 */
+  const int32_t* row_start;   /* [batch + 1] nondecreasing from 0 to rows, or NULL */
+  int32_t src_dtype;          /* MIRA_DT_F32, F16 or BF16 */
+  int32_t reserved;           /* 0 */
+} mira_kv_append;
+
+int mira_cuda_kv_append(const mira_kv_append* a);
+
+/* Attention of one new token per sequence over its pages (the token's own key and value are the last
+ * position: append first).  heads = kv_heads * group; query head h reads kv head h / group.
+ *   o[b, h] = sum_t p_t v_t,   p = softmax over the visible t of scale * q[b, h] . k_t
+ * Visible are t < lengths[b]; with window > 0 only t >= lengths[b] - window and the first `sinks`
+ * positions.  Slots that are not visible are never read into a result, whatever they hold.  A
+ * sequence of length 0 gives o = 0 and lse = -inf.  lse[b * heads + h] = log sum_t exp(scale q . k_t)
+ * (natural logarithm), which joins this result with another over other keys.
+ * Scores, softmax statistics and sums are f32; q, k and v enter the products exactly.  The visible
+ * tokens of all sequences are dealt out evenly over the GPU's SMs; the parts of one (sequence, head)
+ * are joined in a fixed order by whichever block finishes last, so equal inputs give equal bits.
+ * workspace: device memory of mira_cuda_paged_attention_workspace() bytes, 16-byte aligned, ZEROED
+ * ONCE by the caller before its first use; every call leaves it ready for the next.  Calls sharing a
+ * workspace must not overlap. */
+typedef struct mira_paged_attention {
+  mira_paged_kv kv;
+  int64_t heads;
+  mira_view4 q;               /* element strides over (batch, head, -, element) */
+  int32_t q_dtype;            /* MIRA_DT_F32, F16 or BF16; also of out */
+  float scale;
+  int64_t window;             /* 0: every earlier token */
+  int64_t sinks;              /* first positions that stay visible with a window */
+  mira_view4 out;             /* q_dtype, strides like q; ptr may be NULL */
+  mira_view4 out_i8;          /* int8 requantized with out_scale; ptr may be NULL */
+  float out_scale;
+  int32_t reserved;           /* 0 */
+  float* lse;                 /* [batch][heads], may be NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+} mira_paged_attention;
+
+int mira_cuda_paged_attention(const mira_paged_attention* a);
+/* 0 for bad sizes.  Depends on the current device's SM count. */
+int64_t mira_cuda_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh);
+
+/* Pages duplicated inside their pool(s): page dst[i] becomes a copy of page src[i], in every plane of
+ * every region (keys, values and scales of all layers), in one or a few launches.  src and dst are
+ * HOST arrays of n page ids in [0, num_pages), read before the call returns; a page may be a source
+ * several times, but no page is a destination twice, or a destination and a source (MIRA_CUDA_EINVAL). */
+typedef struct mira_page_region {
+  void* base;
+  int64_t planes, plane_stride;   /* bytes from one layer's pages to the next's */
+  int64_t page_stride;            /* bytes from one page to the next */
+  int64_t page_bytes;             /* bytes of a page, contiguous; <= page_stride */
+} mira_page_region;
+
+#define MIRA_PAGE_REGIONS 4
+
+int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* regions, int64_t num_pages, int64_t n,
+                        const int32_t* src, const int32_t* dst);
+
+/* Products with 4-bit weights, for the few rows of a decode step:
+ *   y[m, n] = steps(sum_g scales[n, g] * sum_{k in group g} x[m, k] * (w[n, k] - 8)),  g = k / group
+ * w: [n][ld_w] bytes, byte j of a row holds element 2 j in its low and 2 j + 1 in its high four bits
+ * (unsigned, 8 means 0); ld_w a multiple of 16 and at least ceil(k / 2); what the rows hold past
+ * element k is not used.  scales: [n][ld_scales] of scale_dtype, ceil(k / group) used; group a
+ * multiple of 32.  x, the weights and the scales enter the products exactly; sums are f32.  steps: the
+ * epilogue steps of mira_epilogue on the f32 result (CHANNEL operands need n entries here, FULL
+ * operands ptr[m * ld + n]); then one rounding to out_dtype.  Any m is taken; the weights are read
+ * once per 16 rows.  workspace: as for mira_cuda_paged_attention, of
+ * mira_cuda_w4_matvec_workspace() bytes (0: none needed, workspace may be NULL). */
+typedef struct mira_w4_matvec {
+  int64_t m, n, k, group;
+  const void* x;
+  int64_t ld_x;
+  const uint8_t* w;
+  int64_t ld_w;
+  const void* scales;
+  int64_t ld_scales;
+  int32_t x_dtype, scale_dtype, out_dtype;   /* MIRA_DT_F32, F16 or BF16 */
+  int32_t n_steps;
+  mira_epi_step steps[MIRA_EPI_MAX_STEPS];
+  void* out;
+  int64_t ld_out;
+  void* workspace;
+  int64_t workspace_bytes;
+} mira_w4_matvec;
+
+int mira_cuda_w4_matvec(const mira_w4_matvec* a);
+int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,9 @@ OPND_VIEW = 5
 LAYOUT_NHWC, LAYOUT_ROW4, LAYOUT_CP = 0, 1, 2
 EPI_MAX_STEPS = 8
 ROW_MAX = 8192
+DT_F32, DT_F16, DT_BF16, DT_I8 = 0, 1, 2, 3
+PAGED_DH_MAX = 256
+PAGE_REGIONS = 4
 
 UNARY_CODES = {"relu": EPI_RELU, "gelu": EPI_GELU, "sigmoid": EPI_SIGMOID, "tanh": EPI_TANH}
 BINARY_CODES = {"add": EPI_ADD, "sub": EPI_SUB, "mul": EPI_MUL, "div": EPI_DIV,
@@ -64,6 +67,38 @@ class Attention(C.Structure):
                 ("out_f32", View4),
                 ("out_i8", View4), ("out_scale", C.c_float), ("workspace", C.c_void_p),
                 ("workspace_bytes", C.c_int64)]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("num_pages", C.c_int64), ("page_size", C.c_int64), ("kv_heads", C.c_int64), ("dh", C.c_int64),
+                ("batch", C.c_int64), ("max_pages", C.c_int64), ("table_ld", C.c_int64), ("k", View4), ("v", View4),
+                ("k_scale", View4), ("v_scale", View4), ("table", C.c_void_p), ("lengths", C.c_void_p),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class KvAppend(C.Structure):
+    _fields_ = [("kv", PagedKV), ("rows", C.c_int64), ("k_new", View4), ("v_new", View4), ("row_start", C.c_void_p),
+                ("src_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [("kv", PagedKV), ("heads", C.c_int64), ("q", View4), ("q_dtype", C.c_int32), ("scale", C.c_float),
+                ("window", C.c_int64), ("sinks", C.c_int64), ("out", View4), ("out_i8", View4),
+                ("out_scale", C.c_float), ("reserved", C.c_int32), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class PageRegion(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("planes", C.c_int64), ("plane_stride", C.c_int64), ("page_stride", C.c_int64),
+                ("page_bytes", C.c_int64)]
+
+
+class W4Matvec(C.Structure):
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("group", C.c_int64), ("x", C.c_void_p),
+                ("ld_x", C.c_int64), ("w", C.c_void_p), ("ld_w", C.c_int64), ("scales", C.c_void_p),
+                ("ld_scales", C.c_int64), ("x_dtype", C.c_int32), ("scale_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("n_steps", C.c_int32), ("steps", EpiStep * EPI_MAX_STEPS), ("out", C.c_void_p), ("ld_out", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 _i64, _f32, _vp, _i32 = C.c_int64, C.c_float, C.c_void_p, C.c_int
@@ -145,6 +180,12 @@ SIGNATURES: dict[str, tuple] = {
     "mira_cuda_attention_f32": (_i32, [C.POINTER(Attention)]),
     "mira_cuda_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "mira_cuda_absmax_f32": (_i32, [_i64, _i64, _i64, _i64, C.POINTER(View4), _vp]),
+    "mira_cuda_kv_append": (_i32, [C.POINTER(KvAppend)]),
+    "mira_cuda_paged_attention": (_i32, [C.POINTER(PagedAttention)]),
+    "mira_cuda_paged_attention_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "mira_cuda_page_copy": (_i32, [_i64, C.POINTER(PageRegion), _i64, _i64, _vp, _vp]),
+    "mira_cuda_w4_matvec": (_i32, [C.POINTER(W4Matvec)]),
+    "mira_cuda_w4_matvec_workspace": (_i64, [_i64, _i64, _i64]),
 }
 
 

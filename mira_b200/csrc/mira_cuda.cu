@@ -11,6 +11,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "../../include/mira_cuda.h"
 #include "memory_bound.cuh"
@@ -21,6 +22,9 @@
 #include "runtime.h"
 #include "sequence_ops.cuh"
 #include "attention_tc.cuh"
+#include "paged_kv.cuh"
+#include "paged_attention.cuh"
+#include "w4_matvec.cuh"
 
 // Set by a kernel that gave up on a bounded wait or met an impossible index; read and cleared by
 // mira_cuda_sync.  One copy per device (module global).
@@ -634,6 +638,8 @@ extern "C" int mira_cuda_sync(void) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_mira_kernel_error, &zero, sizeof(int));
     if (flag == 3) return set_error(MIRA_CUDA_EKERNEL, "embedding row index out of range (error record 3)");
+    if (flag == PAGED_ERR)
+      return set_error(MIRA_CUDA_EKERNEL, "a page id, length or row range is outside its bounds (error record 4)");
     return set_error(MIRA_CUDA_EKERNEL, "a kernel gave up on a bounded wait (error record " + std::to_string(flag) + ")");
   }
   return MIRA_CUDA_OK;
@@ -1932,4 +1938,290 @@ extern "C" int mira_cuda_qgemm_splitk_static(int64_t M, int64_t N, int64_t K, co
   const int64_t num_kb = (K + QG_BK - 1) / QG_BK;
   MIRA_CHECK_ARG(splits <= 1 || int64_t(splits - 1) * kb_per < num_kb, "split-K plan with an empty K range");
   return qgemm_run(dev, M, N, K, A, lda, B, ldb, dq, epi, splits, kb_per, scratch);
+}
+
+// ---------------------------------------------------------------- paged decoding
+
+namespace mira {
+
+static int64_t dt_size(int dtype) {
+  switch (dtype) {
+    case MIRA_DT_F32: return 4;
+    case MIRA_DT_F16: case MIRA_DT_BF16: return 2;
+    case MIRA_DT_I8: return 1;
+    default: return 0;
+  }
+}
+
+static bool row_dtype(int dtype) { return dtype == MIRA_DT_F32 || dtype == MIRA_DT_F16 || dtype == MIRA_DT_BF16; }
+
+static bool aligned_to(const void* ptr, int64_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % uint64_t(bytes) == 0; }
+
+// Checks a mira_paged_kv and fills the kernels' form of it.
+static int paged_fill(const mira_paged_kv& a, PagedKv& p) {
+  MIRA_CHECK_ARG(dt_size(a.dtype) > 0 && a.reserved == 0, "unknown page type");
+  MIRA_CHECK_ARG(a.num_pages > 0 && a.num_pages <= INT32_MAX && a.page_size > 0 && a.kv_heads > 0 &&
+                     a.kv_heads <= 65535 && a.dh > 0 && a.dh <= MIRA_PAGED_DH_MAX,
+                 "bad page shape (1 <= dh <= 256)");
+  MIRA_CHECK_ARG(a.batch >= 0 && a.batch <= (1 << 24) && a.max_pages > 0 && a.table_ld >= a.max_pages, "bad page table");
+  // positions are 32-bit, with room for a tile past the last one
+  MIRA_CHECK_ARG(a.page_size <= (int64_t(1) << 30) && a.max_pages <= (int64_t(1) << 30) &&
+                     a.page_size * a.max_pages <= (int64_t(1) << 31) - 65536,
+                 "a sequence's pages hold too many positions");
+  MIRA_CHECK_ARG(a.k.ptr != nullptr && a.v.ptr != nullptr, "null pages");
+  MIRA_CHECK_ARG(a.k.stride[3] == 1 && a.v.stride[3] == 1, "elements of a key or value row must be contiguous");
+  MIRA_CHECK_ARG(aligned_to(a.k.ptr, dt_size(a.dtype)) && aligned_to(a.v.ptr, dt_size(a.dtype)), "misaligned pages");
+  const bool i8 = a.dtype == MIRA_DT_I8;
+  MIRA_CHECK_ARG(!i8 || (a.k_scale.ptr != nullptr && a.v_scale.ptr != nullptr && aligned_to(a.k_scale.ptr, 4) &&
+                         aligned_to(a.v_scale.ptr, 4)),
+                 "8-bit pages need key and value scales");
+  MIRA_CHECK_ARG(a.batch == 0 || (a.table != nullptr && a.lengths != nullptr), "null page table or lengths");
+  MIRA_CHECK_ARG(aligned_to(a.table, 4) && aligned_to(a.lengths, 4), "misaligned page table or lengths");
+  std::memset(&p, 0, sizeof(p));
+  p.k = a.k.ptr; p.v = a.v.ptr;
+  if (i8) {
+    p.ks = static_cast<float*>(a.k_scale.ptr);
+    p.vs = static_cast<float*>(a.v_scale.ptr);
+  }
+  for (int i = 0; i < 3; ++i) {
+    p.kst[i] = a.k.stride[i]; p.vst[i] = a.v.stride[i];
+    p.kss[i] = i8 ? a.k_scale.stride[i] : 0; p.vss[i] = i8 ? a.v_scale.stride[i] : 0;
+  }
+  p.table = a.table; p.table_ld = a.table_ld; p.lengths = a.lengths;
+  p.batch = int(a.batch); p.num_pages = int(a.num_pages); p.max_pages = int(a.max_pages);
+  p.page_size = int(a.page_size); p.kv_heads = int(a.kv_heads); p.dh = int(a.dh);
+  p.page_div = make_div(a.page_size);
+  p.err = device_err_ptr();
+  return MIRA_CUDA_OK;
+}
+
+// Whether every row of the pages starts on a multiple of `bytes` and ends on one.
+static bool paged_rows_aligned(const mira_paged_kv& a, int64_t bytes) {
+  const int64_t size = dt_size(a.dtype);
+  bool ok = a.dh * size % bytes == 0 && aligned_to(a.k.ptr, bytes) && aligned_to(a.v.ptr, bytes);
+  for (int i = 0; i < 3; ++i) ok = ok && a.k.stride[i] * size % bytes == 0 && a.v.stride[i] * size % bytes == 0;
+  return ok;
+}
+
+}  // namespace mira
+
+extern "C" int mira_cuda_kv_append(const mira_kv_append* a) {
+  MIRA_GET_DEVICE(dev);
+  MIRA_CHECK_ARG(a != nullptr, "null append descriptor");
+  AppendParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int rc = paged_fill(a->kv, p.kv);
+  if (rc != MIRA_CUDA_OK) return rc;
+  MIRA_CHECK_ARG(a->rows >= 0 && a->rows <= INT32_MAX, "bad row count");
+  MIRA_CHECK_ARG(row_dtype(a->src_dtype) && a->reserved == 0, "rows are f32, f16 or bf16");
+  MIRA_CHECK_ARG(a->row_start != nullptr || a->rows == a->kv.batch, "without row_start there is one row per sequence");
+  if (a->rows == 0) return MIRA_CUDA_OK;
+  MIRA_CHECK_ARG(a->kv.batch > 0, "rows without sequences");
+  MIRA_CHECK_ARG(a->k_new.ptr != nullptr && a->v_new.ptr != nullptr, "null rows");
+  MIRA_CHECK_ARG(a->k_new.stride[3] == 1 && a->v_new.stride[3] == 1, "elements of a row must be contiguous");
+  MIRA_CHECK_ARG(aligned_to(a->k_new.ptr, dt_size(a->src_dtype)) && aligned_to(a->v_new.ptr, dt_size(a->src_dtype)) &&
+                     aligned_to(a->row_start, 4),
+                 "misaligned rows");
+  p.k_new = a->k_new.ptr; p.v_new = a->v_new.ptr;
+  for (int i = 0; i < 2; ++i) { p.kn[i] = a->k_new.stride[i + 1]; p.vn[i] = a->v_new.stride[i + 1]; }
+  p.row_start = a->row_start;
+  p.rows = a->rows;
+  p.src_dtype = a->src_dtype;
+  p.dtype = a->kv.dtype;
+  kv_append_kernel<<<grid_for(dev, a->rows * a->kv.kv_heads * 32, APPEND_WARPS * 32), APPEND_WARPS * 32, 0, dev->stream>>>(p);
+  return after_launch("kv_append_kernel");
+}
+
+extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* regions, int64_t num_pages, int64_t n,
+                                   const int32_t* src, const int32_t* dst) {
+  MIRA_GET_DEVICE(dev);
+  MIRA_CHECK_ARG(n_regions > 0 && n_regions <= MIRA_PAGE_REGIONS && regions != nullptr, "1 to 4 page regions");
+  MIRA_CHECK_ARG(num_pages > 0 && num_pages <= INT32_MAX && n >= 0 && n <= num_pages, "bad page counts");
+  MIRA_CHECK_ARG(n == 0 || (src != nullptr && dst != nullptr), "null page lists");
+  PageCopyParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.n_regions = int(n_regions);
+  for (int i = 0; i < p.n_regions; ++i) {
+    const mira_page_region& r = regions[i];
+    MIRA_CHECK_ARG(r.base != nullptr && r.planes > 0 && r.planes <= INT32_MAX && r.page_bytes > 0 &&
+                       r.page_stride >= r.page_bytes && r.plane_stride >= 0,
+                   "bad page region");
+    const int64_t chunks = (r.page_bytes + PAGE_COPY_CHUNK - 1) / PAGE_COPY_CHUNK;
+    MIRA_CHECK_ARG(chunks <= INT32_MAX, "pages too large");
+    p.r[i].base = static_cast<uint8_t*>(r.base);
+    p.r[i].plane_stride = r.plane_stride; p.r[i].page_stride = r.page_stride; p.r[i].page_bytes = r.page_bytes;
+    p.r[i].planes = int(r.planes); p.r[i].chunks = int(chunks);
+    p.r[i].first = p.tasks;
+    p.r[i].vec = aligned_to(r.base, 16) && r.plane_stride % 16 == 0 && r.page_stride % 16 == 0;
+    p.tasks += r.planes * chunks;
+  }
+  // no page may be written twice, or written and read: the pairs run in any order
+  try {
+    std::vector<uint8_t> role(static_cast<size_t>(num_pages), 0);
+    for (int64_t i = 0; i < n; ++i) {
+      MIRA_CHECK_ARG(src[i] >= 0 && src[i] < num_pages && dst[i] >= 0 && dst[i] < num_pages, "page id out of range");
+      MIRA_CHECK_ARG(role[dst[i]] == 0, "a page is a destination twice");
+      role[dst[i]] = 1;
+    }
+    for (int64_t i = 0; i < n; ++i) MIRA_CHECK_ARG(role[src[i]] == 0, "a page is a destination and a source");
+  } catch (const std::exception&) {
+    return set_error(MIRA_CUDA_EINVAL, "out of host memory while checking the page lists");
+  }
+  for (int64_t at = 0; at < n; at += PAGE_COPY_PAIRS) {
+    p.n = int(n - at < PAGE_COPY_PAIRS ? n - at : PAGE_COPY_PAIRS);
+    std::memcpy(p.src, src + at, size_t(p.n) * 4);
+    std::memcpy(p.dst, dst + at, size_t(p.n) * 4);
+    const int64_t blocks = p.tasks * p.n, cap = int64_t(dev->sm_count) * 64;
+    page_copy_kernel<<<unsigned(blocks < cap ? blocks : cap), PAGE_COPY_THREADS, 0, dev->stream>>>(p);
+    const int rc = after_launch("page_copy_kernel");
+    if (rc != MIRA_CUDA_OK) return rc;
+  }
+  return MIRA_CUDA_OK;
+}
+
+namespace mira {
+
+constexpr int PA_BLOCKS_PER_SM = 2;
+
+// Query heads of one pass over a row: the smallest of 1, 2, 4, 8 that holds the group, else 8.
+static int pa_heads_per_pass(int64_t group) { return group >= 5 ? 8 : group >= 3 ? 4 : int(group); }
+
+static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch * units * 4, 256); }
+
+template <typename T, int DHP, int GP, int VB>
+static int launch_paged_attention(DeviceState* dev, PagedAttnParams& p) {
+  using C = PaCfg<T, DHP, GP, VB>;
+  auto kern = paged_attention_kernel<T, DHP, GP, VB>;
+  static bool configured[kMaxDevices] = {};
+  if (!configured[dev->device]) {
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
+                  "cudaFuncSetAttribute(paged attention)");
+    configured[dev->device] = true;
+  }
+  p.head_blocks = (p.group + GP - 1) / GP;
+  p.units = p.kv.kv_heads * p.head_blocks;
+  kern<<<unsigned(dev->sm_count * PA_BLOCKS_PER_SM), PA_THREADS, C::SMEM, dev->stream>>>(p);
+  return after_launch("paged_attention_kernel");
+}
+
+template <typename T, int GP, int VB>
+static int launch_paged_dh(DeviceState* dev, PagedAttnParams& p) {
+  if (p.kv.dh <= 32) return launch_paged_attention<T, 32, GP, VB>(dev, p);
+  if (p.kv.dh <= 64) return launch_paged_attention<T, 64, GP, VB>(dev, p);
+  if (p.kv.dh <= 128) return launch_paged_attention<T, 128, GP, VB>(dev, p);
+  return launch_paged_attention<T, 256, GP, VB>(dev, p);
+}
+
+template <typename T>
+static int launch_paged_type(DeviceState* dev, PagedAttnParams& p, bool vec) {
+  if (!vec) return launch_paged_attention<T, 256, 1, int(sizeof(T))>(dev, p);
+  if (p.group == 1) return launch_paged_dh<T, 1, 16>(dev, p);
+  if (p.group == 2) return launch_paged_dh<T, 2, 16>(dev, p);
+  return launch_paged_dh<T, 4, 16>(dev, p);
+}
+
+}  // namespace mira
+
+extern "C" int64_t mira_cuda_paged_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh) {
+  DeviceState* dev = current_device();
+  if (dev == nullptr || batch <= 0 || batch > (1 << 24) || heads <= 0 || kv_heads <= 0 || kv_heads > 65535 ||
+      heads % kv_heads != 0 || heads > 65535 || dh <= 0 || dh > MIRA_PAGED_DH_MAX)
+    return 0;
+  int64_t dhp = 32;
+  while (dhp < dh) dhp *= 2;
+  const int64_t slot = 8 * (256 + 2) * 4;
+  return pa_counters(batch, heads) + int64_t(dev->sm_count) * PA_BLOCKS_PER_SM * 2 * slot;
+}
+
+extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
+  MIRA_GET_DEVICE(dev);
+  MIRA_CHECK_ARG(a != nullptr, "null paged attention descriptor");
+  PagedAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int rc = paged_fill(a->kv, p.kv);
+  if (rc != MIRA_CUDA_OK) return rc;
+  MIRA_CHECK_ARG(a->heads > 0 && a->heads <= 65535 && a->heads % a->kv.kv_heads == 0,
+                 "query heads must be a multiple of the key/value heads");
+  MIRA_CHECK_ARG(row_dtype(a->q_dtype) && a->reserved == 0, "queries are f32, f16 or bf16");
+  MIRA_CHECK_ARG(std::isfinite(a->scale), "the scale must be finite");
+  MIRA_CHECK_ARG(a->window >= 0 && a->sinks >= 0, "bad window");
+  MIRA_CHECK_ARG(a->out.ptr != nullptr || a->out_i8.ptr != nullptr, "paged attention has no output");
+  if (a->out_i8.ptr != nullptr)
+    MIRA_CHECK_ARG(a->out_scale > 0.0f && std::isfinite(a->out_scale), "requant scale must be positive");
+  if (a->kv.batch == 0) return MIRA_CUDA_OK;
+  MIRA_CHECK_ARG(a->q.ptr != nullptr && aligned_to(a->q.ptr, dt_size(a->q_dtype)) &&
+                     aligned_to(a->out.ptr, dt_size(a->q_dtype)) && aligned_to(a->lse, 4),
+                 "null or misaligned queries or outputs");
+  const int64_t need = mira_cuda_paged_attention_workspace(a->kv.batch, a->heads, a->kv.kv_heads, a->kv.dh);
+  MIRA_CHECK_ARG(a->workspace != nullptr && aligned_to(a->workspace, 16) && a->workspace_bytes >= need && need > 0,
+                 "workspace smaller than mira_cuda_paged_attention_workspace()");
+  p.q = a->q.ptr;
+  p.qs[0] = a->q.stride[0]; p.qs[1] = a->q.stride[1]; p.qs[2] = a->q.stride[3];
+  p.os[0] = a->out.stride[0]; p.os[1] = a->out.stride[1]; p.os[2] = a->out.stride[3];
+  p.is[0] = a->out_i8.stride[0]; p.is[1] = a->out_i8.stride[1]; p.is[2] = a->out_i8.stride[3];
+  p.q_dtype = a->q_dtype;
+  p.scale_log2 = float(double(a->scale) * 1.4426950408889634);
+  p.heads = int(a->heads);
+  p.group = int(a->heads / a->kv.kv_heads);
+  const int64_t most = int64_t(1) << 31;
+  p.window = a->window >= most ? 0 : int(a->window);
+  p.sinks = a->sinks >= most ? int(most - 1) : int(a->sinks);
+  p.out = a->out.ptr;
+  p.out_i8 = static_cast<int8_t*>(a->out_i8.ptr);
+  p.q8 = make_qscale(p.out_i8 != nullptr ? a->out_scale : 1.0f);
+  p.lse = a->lse;
+  p.counters = static_cast<int*>(a->workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pa_counters(a->kv.batch, a->heads));
+  const bool vec = paged_rows_aligned(a->kv, 16);
+  switch (a->kv.dtype) {
+    case MIRA_DT_F32: return launch_paged_type<float>(dev, p, vec);
+    case MIRA_DT_F16: return launch_paged_type<__half>(dev, p, vec);
+    case MIRA_DT_BF16: return launch_paged_type<__nv_bfloat16>(dev, p, vec);
+    default: return launch_paged_type<int8_t>(dev, p, vec);
+  }
+}
+
+extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k) {
+  (void)m; (void)n; (void)k;
+  return 0;
+}
+
+extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
+  MIRA_GET_DEVICE(dev);
+  MIRA_CHECK_ARG(a != nullptr, "null matvec descriptor");
+  MIRA_CHECK_ARG(a->m >= 0 && a->m <= INT32_MAX && a->n >= 0 && a->n <= INT32_MAX && a->k > 0 && a->k <= (1 << 30),
+                 "bad matvec shape");
+  MIRA_CHECK_ARG(a->group > 0 && a->group % 32 == 0, "the group must be a multiple of 32");
+  MIRA_CHECK_ARG(row_dtype(a->x_dtype) && row_dtype(a->scale_dtype) && row_dtype(a->out_dtype),
+                 "rows, scales and results are f32, f16 or bf16");
+  MIRA_CHECK_ARG(a->ld_x >= a->k && a->ld_w % 16 == 0 && a->ld_w >= (a->k + 1) / 2 &&
+                     a->ld_scales >= (a->k + a->group - 1) / a->group && a->ld_out >= a->n,
+                 "bad row strides");
+  MIRA_CHECK_ARG(a->n_steps >= 0 && a->n_steps <= MIRA_EPI_MAX_STEPS, "too many epilogue steps");
+  if (a->m == 0 || a->n == 0) return MIRA_CUDA_OK;
+  MIRA_CHECK_ARG(a->x != nullptr && a->w != nullptr && a->scales != nullptr && a->out != nullptr, "null operand");
+  MIRA_CHECK_ARG(aligned_to(a->x, dt_size(a->x_dtype)) && aligned_to(a->w, 16) && aligned_to(a->scales, dt_size(a->scale_dtype)) &&
+                     aligned_to(a->out, dt_size(a->out_dtype)),
+                 "misaligned operand (weights: 16 bytes)");
+  W4Params p;
+  std::memset(&p, 0, sizeof(p));
+  for (int s = 0; s < a->n_steps; ++s) {
+    const mira_epi_step& st = a->steps[s];
+    const bool unary = st.op >= MIRA_EPI_RELU && st.op <= MIRA_EPI_TANH;
+    MIRA_CHECK_ARG(unary || (st.op >= MIRA_EPI_ADD && st.op <= MIRA_EPI_MINIMUM), "unknown epilogue op");
+    MIRA_CHECK_ARG(unary == (st.operand == MIRA_OPND_NONE) && st.operand >= MIRA_OPND_NONE && st.operand <= MIRA_OPND_ROW,
+                   "epilogue operand kind does not match the op");
+    MIRA_CHECK_ARG(st.operand < MIRA_OPND_CHANNEL || (st.ptr != nullptr && aligned_to(st.ptr, 4)), "operand pointer missing");
+    p.steps[s] = st;
+  }
+  p.n_steps = a->n_steps;
+  p.x = a->x; p.w = a->w; p.scales = a->scales; p.out = a->out;
+  p.ld_x = a->ld_x; p.ld_w = a->ld_w; p.ld_scales = a->ld_scales; p.ld_out = a->ld_out;
+  p.m = int(a->m); p.n = int(a->n); p.k = int(a->k);
+  p.group = int(a->group > (1 << 30) ? (1 << 30) : a->group);
+  p.x_dtype = a->x_dtype; p.scale_dtype = a->scale_dtype; p.out_dtype = a->out_dtype;
+  const int64_t gy = (a->m + W4_ROWS - 1) / W4_ROWS;
+  const dim3 grid(unsigned((a->n + W4_WARPS - 1) / W4_WARPS), unsigned(gy < 65535 ? gy : 65535));
+  w4_matvec_kernel<<<grid, W4_WARPS * 32, 0, dev->stream>>>(p);
+  return after_launch("w4_matvec_kernel");
 }

@@ -158,6 +158,22 @@ _OPND = {"none": _lib.OPND_NONE, "scalar": _lib.OPND_SCALAR, "channel": _lib.OPN
          "full": _lib.OPND_FULL, "row": _lib.OPND_ROW}
 
 
+def _fill_steps(dst, steps: Sequence[Step]) -> int:
+    if len(steps) > _lib.EPI_MAX_STEPS:
+        raise ValueError(f"at most {_lib.EPI_MAX_STEPS} fused epilogue steps")
+    for i, s in enumerate(steps):
+        code = _lib.UNARY_CODES.get(s.op) or _lib.BINARY_CODES.get(s.op)
+        if code is None:
+            raise ValueError(f"epilogue op {s.op!r} has no device implementation")
+        dst[i].op = code
+        dst[i].operand = _OPND[s.operand]
+        dst[i].swapped = int(bool(s.swapped))
+        dst[i].scalar = float(np.float32(s.scalar))
+        dst[i].ptr = ptr(s.ptr).value or 0
+        dst[i].ld = int(s.ld)
+    return len(steps)
+
+
 @dataclass
 class Epi:
     steps: Sequence[Step] = field(default_factory=list)
@@ -170,19 +186,7 @@ class Epi:
 
     def struct(self) -> _lib.Epilogue:
         e = _lib.Epilogue()
-        if len(self.steps) > _lib.EPI_MAX_STEPS:
-            raise ValueError(f"at most {_lib.EPI_MAX_STEPS} fused epilogue steps")
-        e.n_steps = len(self.steps)
-        for i, s in enumerate(self.steps):
-            code = _lib.UNARY_CODES.get(s.op) or _lib.BINARY_CODES.get(s.op)
-            if code is None:
-                raise ValueError(f"epilogue op {s.op!r} has no device implementation")
-            e.steps[i].op = code
-            e.steps[i].operand = _OPND[s.operand]
-            e.steps[i].swapped = int(bool(s.swapped))
-            e.steps[i].scalar = float(np.float32(s.scalar))
-            e.steps[i].ptr = ptr(s.ptr).value or 0
-            e.steps[i].ld = int(s.ld)
+        e.n_steps = _fill_steps(e.steps, self.steps)
         e.out_f32 = ptr(self.out_f32).value or 0
         e.ld_f32 = int(self.ld_f32)
         e.out_i8 = ptr(self.out_i8).value or 0
@@ -518,3 +522,231 @@ def absmax_f32(shape4, x: View, out) -> None:
     xv = x.struct()
     n0, n1, n2, n3 = (int(v) for v in shape4)
     _lib.call("mira_cuda_absmax_f32", n0, n1, n2, n3, C.byref(xv), ptr(out))
+
+
+# ----------------------------------------------------------------------------- paged decoding
+
+DTYPES = {"f32": _lib.DT_F32, "f16": _lib.DT_F16, "bf16": _lib.DT_BF16, "i8": _lib.DT_I8}
+
+
+def _dtype(name: str) -> int:
+    if name not in DTYPES:
+        raise ValueError(f"unknown element type {name!r}: one of {', '.join(DTYPES)}")
+    return DTYPES[name]
+
+
+@dataclass
+class PagedKV:
+    """One layer's keys and values in pages (mira_paged_kv): `k` / `v` view the pages over (page, kv
+    head, slot, element), `table` and `lengths` are int32 device memory."""
+    num_pages: int
+    page_size: int
+    kv_heads: int
+    dh: int
+    dtype: str
+    k: View
+    v: View
+    batch: int
+    table: object
+    table_ld: int
+    max_pages: int
+    lengths: object
+    k_scale: Optional[View] = None
+    v_scale: Optional[View] = None
+
+    def struct(self) -> _lib.PagedKV:
+        p = _lib.PagedKV()
+        p.num_pages, p.page_size, p.kv_heads, p.dh = (int(x) for x in (self.num_pages, self.page_size, self.kv_heads, self.dh))
+        p.batch, p.max_pages, p.table_ld = int(self.batch), int(self.max_pages), int(self.table_ld)
+        p.k, p.v = self.k.struct(), self.v.struct()
+        if self.k_scale is not None:
+            p.k_scale = self.k_scale.struct()
+        if self.v_scale is not None:
+            p.v_scale = self.v_scale.struct()
+        p.table = ptr(self.table).value or 0
+        p.lengths = ptr(self.lengths).value or 0
+        p.dtype = _dtype(self.dtype)
+        return p
+
+
+@dataclass
+class KvAppend:
+    """New rows into the pages (mira_kv_append): `k_new` / `v_new` over (-, kv head, row, element)."""
+    kv: PagedKV
+    rows: int
+    k_new: View
+    v_new: View
+    src_dtype: str = "f32"
+    row_start: object = None
+
+    def struct(self) -> _lib.KvAppend:
+        a = _lib.KvAppend()
+        a.kv = self.kv.struct()
+        a.rows = int(self.rows)
+        a.k_new, a.v_new = self.k_new.struct(), self.v_new.struct()
+        a.row_start = ptr(self.row_start).value or 0
+        a.src_dtype = _dtype(self.src_dtype)
+        return a
+
+
+@dataclass
+class PagedAttn:
+    """One token per sequence against its pages (mira_paged_attention): `q` and `out` over (batch,
+    head, -, element); `lse` f32 [batch, heads] or None; workspace of paged_attention_workspace()
+    bytes, zeroed once."""
+    kv: PagedKV
+    heads: int
+    q: View
+    scale: float
+    out: Optional[View] = None
+    q_dtype: str = "f32"
+    window: int = 0
+    sinks: int = 0
+    out_i8: Optional[View] = None
+    out_scale: float = 1.0
+    lse: object = None
+    workspace: object = None
+    workspace_bytes: int = 0
+
+    def struct(self) -> _lib.PagedAttention:
+        a = _lib.PagedAttention()
+        a.kv = self.kv.struct()
+        a.heads = int(self.heads)
+        a.q = self.q.struct()
+        a.q_dtype = _dtype(self.q_dtype)
+        a.scale = float(np.float32(self.scale))
+        a.window, a.sinks = int(self.window), int(self.sinks)
+        if self.out is not None:
+            a.out = self.out.struct()
+        if self.out_i8 is not None:
+            a.out_i8 = self.out_i8.struct()
+        a.out_scale = float(np.float32(self.out_scale))
+        a.lse = ptr(self.lse).value or 0
+        a.workspace = ptr(self.workspace).value or 0
+        a.workspace_bytes = int(self.workspace_bytes)
+        return a
+
+
+@dataclass
+class PageRegion:
+    """Pages of a pool for page_copy (mira_page_region): `planes` layers of pages, strides in bytes."""
+    base: object
+    page_bytes: int
+    page_stride: int
+    planes: int = 1
+    plane_stride: int = 0
+
+    def struct(self) -> _lib.PageRegion:
+        return _lib.PageRegion(ptr(self.base).value or 0, int(self.planes), int(self.plane_stride), int(self.page_stride),
+                               int(self.page_bytes))
+
+
+@dataclass
+class W4Matvec:
+    """y = steps(x @ (s (w - 8))^T) with 4-bit weights (mira_w4_matvec); see w4_weight for the layout."""
+    m: int
+    n: int
+    k: int
+    group: int
+    x: object
+    ld_x: int
+    w: object
+    ld_w: int
+    scales: object
+    ld_scales: int
+    out: object
+    ld_out: int
+    x_dtype: str = "f32"
+    scale_dtype: str = "f32"
+    out_dtype: str = "f32"
+    steps: Sequence[Step] = field(default_factory=list)
+    workspace: object = None
+    workspace_bytes: int = 0
+
+    def struct(self) -> _lib.W4Matvec:
+        a = _lib.W4Matvec()
+        a.m, a.n, a.k, a.group = int(self.m), int(self.n), int(self.k), int(self.group)
+        a.x, a.ld_x = ptr(self.x).value or 0, int(self.ld_x)
+        a.w, a.ld_w = ptr(self.w).value or 0, int(self.ld_w)
+        a.scales, a.ld_scales = ptr(self.scales).value or 0, int(self.ld_scales)
+        a.x_dtype, a.scale_dtype, a.out_dtype = _dtype(self.x_dtype), _dtype(self.scale_dtype), _dtype(self.out_dtype)
+        a.n_steps = _fill_steps(a.steps, self.steps)
+        a.out, a.ld_out = ptr(self.out).value or 0, int(self.ld_out)
+        a.workspace = ptr(self.workspace).value or 0
+        a.workspace_bytes = int(self.workspace_bytes)
+        return a
+
+
+def _struct(desc, cls):
+    """A descriptor's C struct; a struct built before (desc.struct()) is taken as it is, so that a
+    loop that keeps its buffers builds it once."""
+    return desc if isinstance(desc, cls) else desc.struct()
+
+
+def kv_append(desc) -> None:
+    """Appends rows to the pages; `desc` a KvAppend or its struct()."""
+    _lib.call("mira_cuda_kv_append", C.byref(_struct(desc, _lib.KvAppend)))
+
+
+def paged_attention_workspace(batch: int, heads: int, kv_heads: int, dh: int) -> int:
+    """Bytes of scratch for paged_attention (to be zeroed once); 0 for sizes it does not take."""
+    return int(_lib.load().mira_cuda_paged_attention_workspace(batch, heads, kv_heads, dh))
+
+
+def paged_attention(desc) -> None:
+    """Attention of one new token per sequence; `desc` a PagedAttn or its struct()."""
+    _lib.call("mira_cuda_paged_attention", C.byref(_struct(desc, _lib.PagedAttention)))
+
+
+def page_regions(regions: Sequence[PageRegion]):
+    """The C array of up to 4 regions, for page_copy."""
+    if not 0 < len(regions) <= _lib.PAGE_REGIONS:
+        raise ValueError(f"1 to {_lib.PAGE_REGIONS} page regions")
+    return (_lib.PageRegion * len(regions))(*[r.struct() for r in regions])
+
+
+def page_copy(regions, num_pages: int, src, dst) -> None:
+    """Page dst[i] becomes a copy of page src[i] in every plane of every region (a sequence of
+    PageRegion, or page_regions() of it); src and dst are host integers."""
+    if not isinstance(regions, C.Array):
+        regions = page_regions(regions)
+    src = np.ascontiguousarray(src, np.int32)
+    dst = np.ascontiguousarray(dst, np.int32)
+    if src.ndim != 1 or src.shape != dst.shape:
+        raise ValueError("src and dst are lists of the same length")
+    _lib.call("mira_cuda_page_copy", len(regions), regions, num_pages, len(src), src.ctypes.data, dst.ctypes.data)
+
+
+def w4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
+    """Symmetric 4-bit codes int8 [n, k] in [-7, 7] and f32 scales [n, ceil(k / group)] of f32 weights
+    [n, k]: scale = absmax / 7 of each group (1 for a group of zeros)."""
+    w = np.asarray(w, np.float32)
+    n, k = w.shape
+    groups = -(-k // group)
+    padded = np.zeros((n, groups * group), np.float32)
+    padded[:, :k] = w
+    blocks = padded.reshape(n, groups, group)
+    top = np.abs(blocks).max(axis=2)
+    scales = np.where(top > 0, top / np.float32(7), np.float32(1)).astype(np.float32)
+    q = np.clip(np.round(blocks / scales[:, :, None]), -7, 7).astype(np.int8)
+    return q.reshape(n, -1)[:, :k].copy(), scales
+
+
+def w4_weight(q: np.ndarray) -> np.ndarray:
+    """4-bit codes int8 [n, k] in [-8, 7] -> uint8 [n, ld], ld = round_up(ceil(k / 2), 16): byte j
+    holds q[2 j] + 8 in its low and q[2 j + 1] + 8 in its high four bits."""
+    n, k = q.shape
+    ld = round_up(-(-k // 2), 16)
+    u = np.full((n, 2 * ld), 8, np.uint8)
+    u[:, :k] = (q.astype(np.int16) + 8).astype(np.uint8)
+    return u[:, 0::2] | (u[:, 1::2] << 4)
+
+
+def w4_matvec_workspace(m: int, n: int, k: int) -> int:
+    """Bytes of scratch for w4_matvec (to be zeroed once; 0: none)."""
+    return int(_lib.load().mira_cuda_w4_matvec_workspace(m, n, k))
+
+
+def w4_matvec(desc) -> None:
+    """Products with 4-bit weights; `desc` a W4Matvec or its struct()."""
+    _lib.call("mira_cuda_w4_matvec", C.byref(_struct(desc, _lib.W4Matvec)))
