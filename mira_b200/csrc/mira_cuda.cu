@@ -2181,6 +2181,51 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
   }
 }
 
+namespace mira {
+
+// Row tiles of a block and stages of its panel of x.  More row tiles share one panel, fewer make more
+// blocks: the choice is the least of (blocks an SM runs one after the other) x (bytes a block brings in).
+static int w4_plan(const DeviceState* dev, W4Params& p) {
+  const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
+  const int most = (w4_panel_bytes(columns) / columns - 64) / (W4_STAGE_K * 2);      // stages that fit the panel
+  const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;
+  const int64_t tiles = (int64_t(p.n) + 15) / 16;
+  int64_t best = INT64_MAX;
+  for (int wr = 8; wr >= 1; wr /= 2) {
+    const int share = 8 / wr;
+    if (share > most && wr < 8) break;
+    const int64_t blocks = (tiles + wr - 1) / wr;
+    const int64_t cost = (blocks + dev->sm_count - 1) / dev->sm_count * (int64_t(wr) * 8 + rows * dt_size(p.x_dtype));
+    if (cost >= best) continue;
+    best = cost;
+    p.wr = wr;
+    const int want = (stages + share - 1) / share * share, fit = most / share * share;
+    p.panel = want < fit ? want : fit;
+  }
+  return p.panel > 0 ? MIRA_CUDA_OK : set_error(MIRA_CUDA_EINVAL, "no room for the rows of x");
+}
+
+template <int XT, int NB>
+static int launch_w4(DeviceState* dev, const W4Params& p) {
+  auto kern = w4_matvec_kernel<XT, NB>;
+  static bool configured[kMaxDevices] = {};
+  const int join = W4_WARPS * NB * 8 * 16 * 4;
+  const int columns = (p.m < W4_ROWS ? p.m : W4_ROWS) * w4_pieces(p.x_dtype);
+  const int panel = columns * w4_pitch(p.panel);
+  const int most = W4_RING + (w4_panel_bytes(NB * 8) > join ? w4_panel_bytes(NB * 8) : join);
+  if (!configured[dev->device]) {
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "cudaFuncSetAttribute(w4)");
+    configured[dev->device] = true;
+  }
+  const int64_t gx = (int64_t(p.n) + 16 * p.wr - 1) / (16 * p.wr), gy = (int64_t(p.m) + W4_ROWS - 1) / W4_ROWS;
+  MIRA_CHECK_ARG(gy <= 65535, "matvec has too many rows");
+  const int smem = W4_RING + (panel > join ? panel : join);
+  kern<<<dim3(unsigned(gx), unsigned(gy)), W4_THREADS, smem, dev->stream>>>(p);
+  return after_launch("w4_matvec_kernel");
+}
+
+}  // namespace mira
+
 extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k) {
   (void)m; (void)n; (void)k;
   return 0;
@@ -2218,10 +2263,21 @@ extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   p.x = a->x; p.w = a->w; p.scales = a->scales; p.out = a->out;
   p.ld_x = a->ld_x; p.ld_w = a->ld_w; p.ld_scales = a->ld_scales; p.ld_out = a->ld_out;
   p.m = int(a->m); p.n = int(a->n); p.k = int(a->k);
-  p.group = int(a->group > (1 << 30) ? (1 << 30) : a->group);
+  const int64_t group = a->group > (int64_t(1) << 30) ? int64_t(1) << 30 : a->group;   // one group past k <= 2^30
+  p.groups = int((a->k + group - 1) / group);
+  p.slices_per_group = make_div(group / 32);
   p.x_dtype = a->x_dtype; p.scale_dtype = a->scale_dtype; p.out_dtype = a->out_dtype;
-  const int64_t gy = (a->m + W4_ROWS - 1) / W4_ROWS;
-  const dim3 grid(unsigned((a->n + W4_WARPS - 1) / W4_WARPS), unsigned(gy < 65535 ? gy : 65535));
-  w4_matvec_kernel<<<grid, W4_WARPS * 32, 0, dev->stream>>>(p);
-  return after_launch("w4_matvec_kernel");
+  p.x_vec = aligned_to(a->x, 16) && a->ld_x * dt_size(a->x_dtype) % 16 == 0;
+  const int rc = w4_plan(dev, p);
+  if (rc != MIRA_CUDA_OK) return rc;
+  const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
+  switch (p.x_dtype) {
+    case MIRA_DT_F16: return columns <= 8 ? launch_w4<MIRA_DT_F16, 1>(dev, p) : launch_w4<MIRA_DT_F16, 2>(dev, p);
+    case MIRA_DT_BF16: return columns <= 8 ? launch_w4<MIRA_DT_BF16, 1>(dev, p) : launch_w4<MIRA_DT_BF16, 2>(dev, p);
+    default:
+      if (columns <= 8) return launch_w4<MIRA_DT_F32, 1>(dev, p);
+      if (columns <= 16) return launch_w4<MIRA_DT_F32, 2>(dev, p);
+      if (columns <= 24) return launch_w4<MIRA_DT_F32, 3>(dev, p);
+      return launch_w4<MIRA_DT_F32, 6>(dev, p);
+  }
 }

@@ -1,9 +1,27 @@
 // Products of a few rows with 4-bit weights under group scales:
 //   y[m, n] = steps(sum_g s[n, g] sum_{k in g} x[m, k] (w[n, k] - 8)).
+//
+// Bound: the weights are read once, n k / 2 bytes (+ scales); everything else has to hide behind that.
+// An SM's share of the memory bandwidth is about 23 bytes a clock, i.e. 46 weights a clock that must
+// be unpacked and multiplied by every row of x.  FMA units need two to three instructions per weight
+// and row; the tensor path needs 1.4 for the unpacking and next to nothing per row: a word of eight
+// weights becomes four registers of exact bf16 (or f16) pairs, which ARE the left operand's fragment
+// of two 16x8x16 products (16 weight rows x 16 k).  x is the right operand, its rows in the eight
+// columns: bf16 and f16 rows as they are, an f32 row as three columns whose bf16 values add up to it
+// exactly, so every product is exact and sums are f32.
+//
+// Layout.  A warp owns 16 weight rows and walks along k in stages of 256 (16 rows x 128 bytes), brought
+// to its own ring in shared memory by cp.async (16-byte chunks, chunk c of row r at c ^ (r % 8), so
+// that the fragment reads of eight rows are free of bank conflicts).  A slice of 32 k is one chunk and
+// lies in one group: its two products start from zero and are added scaled.  The eight warps of a
+// block are WR row tiles times 8 / WR interleaved shares of k (joined in shared memory at the end); the
+// block's x is staged in a panel, whole where it fits, k in the fragments' order.
 #pragma once
 #include <cstdint>
 
+#include "mma_sm80.cuh"
 #include "paged_kv.cuh"
+#include "ptx_sm100.cuh"
 
 namespace mira {
 
@@ -13,7 +31,11 @@ struct W4Params {
   const void* scales;
   void* out;
   int64_t ld_x, ld_w, ld_scales, ld_out;
-  int m, n, k, group;
+  int m, n, k, groups;
+  QgDiv slices_per_group;     // group / 32
+  int wr;                     // row tiles of a block: 1, 2, 4 or 8
+  int panel;                  // stages of x in shared memory, a multiple of 8 / wr
+  int x_vec;                  // rows of x can be read 16 bytes at a time
   int x_dtype, scale_dtype, out_dtype;
   int n_steps;
   mira_epi_step steps[MIRA_EPI_MAX_STEPS];
@@ -37,39 +59,187 @@ __device__ __forceinline__ float w4_steps(const W4Params& p, float y, int m, int
 }
 
 constexpr int W4_WARPS = 8;
-constexpr int W4_ROWS = 4;     // rows of x per pass over the weights
+constexpr int W4_THREADS = W4_WARPS * 32;
+constexpr int W4_ROWS = 16;                  // rows of x per pass over the weights
+constexpr int W4_STAGES = 4;
+constexpr int W4_STAGE_K = 256;
+constexpr int W4_STAGE_BYTES = 16 * W4_STAGE_K / 2;
+constexpr int W4_RING = W4_WARPS * W4_STAGES * W4_STAGE_BYTES;
+// Bytes of the panel: two blocks per SM while x is narrow, one for many columns, whose panels would
+// otherwise be a stage or two long.
+__host__ __device__ constexpr int w4_panel_bytes(int columns) { return columns <= 16 ? 48 << 10 : 128 << 10; }
 
-// One warp per weight row: lanes stride over words of eight weights, each group's sum is scaled once.
-__global__ void __launch_bounds__(W4_WARPS * 32) w4_matvec_kernel(const __grid_constant__ W4Params p) {
-  const int lane = threadIdx.x & 31;
-  const int n = blockIdx.x * W4_WARPS + (threadIdx.x >> 5);
-  if (n >= p.n) return;
-  for (int m0 = blockIdx.y * W4_ROWS; m0 < p.m; m0 += gridDim.y * W4_ROWS) {
-    float acc[W4_ROWS] = {};
-    const int words = (p.k + 7) / 8;
-    for (int j = lane; j < words; j += 32) {
-      const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p.w + n * p.ld_w) + j);
-      const float s = dt_load(p.scales, n * p.ld_scales + j * 8 / p.group, p.scale_dtype);
+// Columns of the right operand that a row of x takes, and bytes of a column with `stages` stages (64
+// more than a multiple of 128: the fragment reads of two columns then cover all banks).
+__host__ __device__ constexpr int w4_pieces(int x_dtype) { return x_dtype == MIRA_DT_F32 ? 3 : 1; }
+__host__ __device__ constexpr int w4_pitch(int stages) { return stages * W4_STAGE_K * 2 + 64; }
+
+// A word of eight weights as four registers of pairs (w0, w4), (w1, w5), (w2, w6), (w3, w7), each
+// w - 8: the nibble is or-ed under the exponent of 1024 (f16) or 128 (bf16), whose last mantissa bit
+// is worth 1, and the offset is subtracted exactly; f16 has room for a nibble shifted by four.
+template <bool BF16>
+__device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&a)[4]) {
+  if (BF16) {
+    const __nv_bfloat162 off = bits_b2(0x43084308u);     // 136
 #pragma unroll
-      for (int r = 0; r < W4_ROWS; ++r) {
-        if (m0 + r >= p.m) break;
-        float part = 0.0f;
+    for (int i = 0; i < 4; ++i) a[i] = b2_bits(__hsub2(bits_b2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u), off));
+  } else {
+    const __half2 off = bits_h2(0x64086408u);            // 1032
+    const __half2 sixteenth = bits_h2(0x2c002c00u), off16 = bits_h2(0xd480d480u);   // 1 / 16, -72
+    const uint32_t v = w >> 8;
+    a[0] = h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), off));
+    a[1] = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
+    a[2] = h2_bits(__hsub2(bits_h2((v & 0x000f000fu) | 0x64006400u), off));
+    a[3] = h2_bits(__hfma2(bits_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
+  }
+}
+
+// Eight values of a row of x from element k on (0 past the end), in the order of the fragments.
+template <int XT>
+__device__ __forceinline__ void w4_stage_x(const W4Params& p, int row, int k, uint8_t* col, int pitch) {
+  if (XT == MIRA_DT_F32) {
+    const float* src = static_cast<const float*>(p.x) + row * p.ld_x + k;
+    float v[8];
+    if (p.x_vec && k + 8 <= p.k) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = j * 8 + e;
-          if (k < p.k)
-            part = fmaf(dt_load(p.x, (m0 + r) * p.ld_x + k, p.x_dtype), float(int((w >> (4 * e)) & 15) - 8), part);
-        }
-        acc[r] = fmaf(part, s, acc[r]);
+      for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? __ldg(src + i) : 0.0f;
+    }
+    uint32_t c[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h0, m0, l0, h1, m1, l1;
+      split3_bf16(v[i], h0, m0, l0);
+      split3_bf16(v[i + 4], h1, m1, l1);
+      c[0][i] = __byte_perm(h0, h1, 0x7632);
+      c[1][i] = __byte_perm(m0, m1, 0x7632);
+      c[2][i] = __byte_perm(l0, l1, 0x7632);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      *reinterpret_cast<uint4*>(col + j * pitch) = make_uint4(c[j][0], c[j][1], c[j][2], c[j][3]);
+  } else {
+    const uint16_t* src = static_cast<const uint16_t*>(p.x) + row * p.ld_x + k;
+    uint32_t v[4];      // pairs (0, 1), (2, 3), ..
+    if (p.x_vec && k + 8 <= p.k) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = (k + 2 * i < p.k ? uint32_t(__ldg(src + 2 * i)) : 0u) |
+               (k + 2 * i + 1 < p.k ? uint32_t(__ldg(src + 2 * i + 1)) << 16 : 0u);
+    }
+    *reinterpret_cast<uint4*>(col) = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632),
+                                                __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632));
+  }
+}
+
+// XT: type of x; NB: blocks of eight columns.
+template <int XT, int NB>
+__global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_constant__ W4Params p) {
+  constexpr bool BF16 = XT != MIRA_DT_F16;
+  constexpr int PIECES = w4_pieces(XT);
+  extern __shared__ __align__(128) uint8_t w4_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int wk_n = W4_WARPS / p.wr, wr = warp % p.wr, wk = warp / p.wr;
+  uint8_t* ring = w4_smem + warp * (W4_STAGES * W4_STAGE_BYTES);
+  uint8_t* panel = w4_smem + W4_RING;
+  const int pitch = w4_pitch(p.panel);
+  const int n0 = (blockIdx.x * p.wr + wr) * 16;
+  const int m0 = blockIdx.y * W4_ROWS, rows = min(W4_ROWS, p.m - m0);
+  const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;       // along k
+  const int mine = stages > wk ? (stages - wk - 1) / wk_n + 1 : 0;
+
+  // this lane's four chunks of a stage: rows lane / 8 + 4 i, chunk lane % 8
+  auto fetch = [&](int i) {
+    if (i < mine) {
+      const int64_t at = int64_t(wk + i * wk_n) * (W4_STAGE_K / 2) + (lane & 7) * 16;
+      const uint32_t dst = smem_u32(ring + (i % W4_STAGES) * W4_STAGE_BYTES);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = (lane >> 3) + 4 * j;
+        const bool in = n0 + r < p.n && at < p.ld_w;
+        cp_async_16(dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4), in ? p.w + (n0 + r) * p.ld_w + at : p.w, in ? 16u : 0u);
       }
     }
+    cp_async_commit();
+  };
 #pragma unroll
-    for (int r = 0; r < W4_ROWS; ++r) {
+  for (int i = 0; i < W4_STAGES - 1; ++i) fetch(i);
+
+  float acc[NB][4];
+  int col[NB];       // this lane's columns; those past the last row of x repeat it and are not used
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-      if (lane == 0 && m0 + r < p.m)
-        dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, acc[r], m0 + r, n));
+  for (int b = 0; b < NB; ++b) col[b] = min(b * 8 + g, rows * PIECES - 1) * pitch;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
+  const int64_t s0 = int64_t(min(n0 + g, p.n - 1)) * p.ld_scales, s1 = int64_t(min(n0 + g + 8, p.n - 1)) * p.ld_scales;
+
+  int i = 0;
+  for (int p0 = 0; p0 < stages; p0 += p.panel) {
+    const int in_panel = min(p.panel, stages - p0);
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * in_panel * 32; e += W4_THREADS) {
+      const int r = e / (in_panel * 32), word = e - r * (in_panel * 32);
+      w4_stage_x<XT>(p, m0 + r, (p0 * 32 + word) * 8, panel + r * PIECES * pitch + word * 16, pitch);
     }
+    __syncthreads();
+    for (; i < mine && wk + i * wk_n < p0 + in_panel; ++i) {
+      const int kb = wk + i * wk_n;
+      float sc[8][2];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const int gi = min(qg_div(kb * 8 + s, p.slices_per_group), p.groups - 1);
+        sc[s][0] = dt_load(p.scales, s0 + gi, p.scale_dtype);
+        sc[s][1] = dt_load(p.scales, s1 + gi, p.scale_dtype);
+      }
+      cp_async_wait<W4_STAGES - 2>();
+      __syncwarp();
+      fetch(i + W4_STAGES - 1);
+      const uint8_t* st = ring + (i % W4_STAGES) * W4_STAGE_BYTES + g * 128 + t * 4;
+      const uint8_t* xs = panel + (kb - p0) * (W4_STAGE_K * 2) + t * 16;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        uint32_t a[4], c[4];
+        w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + ((s ^ g) << 4)), a);
+        w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + 1024 + ((s ^ g) << 4)), c);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint4 x = *reinterpret_cast<const uint4*>(xs + col[b] + s * 64);
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_16816<BF16>(d, a[0], c[0], a[1], c[1], x.x, x.y);
+          mma_16816<BF16>(d, a[2], c[2], a[3], c[3], x.z, x.w);
+          acc[b][0] = fmaf(sc[s][0], d[0], acc[b][0]);
+          acc[b][1] = fmaf(sc[s][0], d[1], acc[b][1]);
+          acc[b][2] = fmaf(sc[s][1], d[2], acc[b][2]);
+          acc[b][3] = fmaf(sc[s][1], d[3], acc[b][3]);
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // the shares of k and the pieces of x, joined in the panel: [warp][column][16 rows]
+  float* red = reinterpret_cast<float*>(panel);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[(warp * NB * 8 + b * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = acc[b][j];
+  __syncthreads();
+  const int tile_n = p.wr * 16;
+  for (int e = threadIdx.x; e < rows * tile_n; e += W4_THREADS) {
+    const int r = e / tile_n, c = e - r * tile_n, n = blockIdx.x * tile_n + c;
+    if (n >= p.n) continue;
+    float y = 0.0f;
+    for (int q = PIECES - 1; q >= 0; --q)
+      for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + (c >> 4)) * NB * 8 + r * PIECES + q) * 16 + (c & 15)];
+    dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
   }
 }
 
