@@ -16,7 +16,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
-    "--expt-relaxed-constexpr",
+    "--expt-relaxed-constexpr", "--split-compile=0",
     # no --use_fast_math: the epilogue relies on IEEE division/rounding and explicit intrinsics
 ]
 

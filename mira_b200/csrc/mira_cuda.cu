@@ -2205,9 +2205,9 @@ static int w4_plan(const DeviceState* dev, W4Params& p) {
   return p.panel > 0 ? MIRA_CUDA_OK : set_error(MIRA_CUDA_EINVAL, "no room for the rows of x");
 }
 
-template <int XT, int NB>
-static int launch_w4(DeviceState* dev, const W4Params& p) {
-  auto kern = w4_matvec_kernel<XT, NB>;
+template <int XT, int NB, int GS>
+static int launch_w4_gs(DeviceState* dev, const W4Params& p) {
+  auto kern = w4_matvec_kernel<XT, NB, GS>;
   static bool configured[kMaxDevices] = {};
   const int join = W4_WARPS * NB * 8 * 16 * 4;
   const int columns = (p.m < W4_ROWS ? p.m : W4_ROWS) * w4_pieces(p.x_dtype);
@@ -2222,6 +2222,14 @@ static int launch_w4(DeviceState* dev, const W4Params& p) {
   const int smem = W4_RING + (panel > join ? panel : join);
   kern<<<dim3(unsigned(gx), unsigned(gy)), W4_THREADS, smem, dev->stream>>>(p);
   return after_launch("w4_matvec_kernel");
+}
+
+template <int XT, int NB>
+static int launch_w4(DeviceState* dev, const W4Params& p, int64_t group) {
+  if (group % 256 == 0) return launch_w4_gs<XT, NB, 8>(dev, p);
+  if (group % 128 == 0) return launch_w4_gs<XT, NB, 4>(dev, p);
+  if (group % 64 == 0) return launch_w4_gs<XT, NB, 2>(dev, p);
+  return launch_w4_gs<XT, NB, 1>(dev, p);
 }
 
 }  // namespace mira
@@ -2272,12 +2280,12 @@ extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   if (rc != MIRA_CUDA_OK) return rc;
   const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
   switch (p.x_dtype) {
-    case MIRA_DT_F16: return columns <= 8 ? launch_w4<MIRA_DT_F16, 1>(dev, p) : launch_w4<MIRA_DT_F16, 2>(dev, p);
-    case MIRA_DT_BF16: return columns <= 8 ? launch_w4<MIRA_DT_BF16, 1>(dev, p) : launch_w4<MIRA_DT_BF16, 2>(dev, p);
+    case MIRA_DT_F16: return columns <= 8 ? launch_w4<MIRA_DT_F16, 1>(dev, p, group) : launch_w4<MIRA_DT_F16, 2>(dev, p, group);
+    case MIRA_DT_BF16: return columns <= 8 ? launch_w4<MIRA_DT_BF16, 1>(dev, p, group) : launch_w4<MIRA_DT_BF16, 2>(dev, p, group);
     default:
-      if (columns <= 8) return launch_w4<MIRA_DT_F32, 1>(dev, p);
-      if (columns <= 16) return launch_w4<MIRA_DT_F32, 2>(dev, p);
-      if (columns <= 24) return launch_w4<MIRA_DT_F32, 3>(dev, p);
-      return launch_w4<MIRA_DT_F32, 6>(dev, p);
+      if (columns <= 8) return launch_w4<MIRA_DT_F32, 1>(dev, p, group);
+      if (columns <= 16) return launch_w4<MIRA_DT_F32, 2>(dev, p, group);
+      if (columns <= 24) return launch_w4<MIRA_DT_F32, 3>(dev, p, group);
+      return launch_w4<MIRA_DT_F32, 6>(dev, p, group);
   }
 }

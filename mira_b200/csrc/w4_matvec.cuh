@@ -137,12 +137,15 @@ __device__ __forceinline__ void w4_stage_x(const W4Params& p, int row, int k, ui
   }
 }
 
-// XT: type of x; NB: blocks of eight columns.
-template <int XT, int NB>
+// XT: type of x; NB: blocks of eight columns; GS: slices whose products are summed before the scale is
+// applied, a divisor of the slices of a group.
+template <int XT, int NB, int GS>
 __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_constant__ W4Params p) {
   constexpr bool BF16 = XT != MIRA_DT_F16;
   constexpr int PIECES = w4_pieces(XT);
+  constexpr int NS = 8 / GS;               // scales of a row per stage
   extern __shared__ __align__(128) uint8_t w4_smem[];
+  __shared__ float w4_scale[W4_WARPS][2][NS][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int wk_n = W4_WARPS / p.wr, wr = warp % p.wr, wk = warp / p.wr;
   uint8_t* ring = w4_smem + warp * (W4_STAGES * W4_STAGE_BYTES);
@@ -153,22 +156,49 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
   const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;       // along k
   const int mine = stages > wk ? (stages - wk - 1) / wk_n + 1 : 0;
 
-  // this lane's four chunks of a stage: rows lane / 8 + 4 i, chunk lane % 8
-  auto fetch = [&](int i) {
-    if (i < mine) {
-      const int64_t at = int64_t(wk + i * wk_n) * (W4_STAGE_K / 2) + (lane & 7) * 16;
-      const uint32_t dst = smem_u32(ring + (i % W4_STAGES) * W4_STAGE_BYTES);
+  // this lane's four chunks of a stage: rows lane / 8 + 4 j, chunk lane % 8; rows past the last one
+  // read the last one and are not used
+  const uint8_t* from[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    from[j] = p.w + int64_t(min(n0 + (lane >> 3) + 4 * j, p.n - 1)) * p.ld_w + (wk * (W4_STAGE_K / 2) + (lane & 7) * 16);
+  const uint32_t to = smem_u32(ring) + (lane >> 3) * 128;
+  const uint32_t swz = ((lane & 7) ^ (lane >> 3)) << 4;          // rows r and r + 4 differ in bit 6
+  int64_t left = p.ld_w - (wk * (W4_STAGE_K / 2) + (lane & 7) * 16);   // bytes of the rows from here on
+  int fetched = 0;
+  auto fetch = [&]() {
+    if (fetched < mine) {
+      const uint32_t dst = to + (fetched % W4_STAGES) * W4_STAGE_BYTES;
+      const uint32_t bytes = left > 0 ? 16u : 0u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = (lane >> 3) + 4 * j;
-        const bool in = n0 + r < p.n && at < p.ld_w;
-        cp_async_16(dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4), in ? p.w + (n0 + r) * p.ld_w + at : p.w, in ? 16u : 0u);
+        cp_async_16(dst + j * 512 + (j & 1 ? swz ^ 64 : swz), left > 0 ? from[j] : p.w, bytes);
+        from[j] += wk_n * (W4_STAGE_K / 2);
       }
+      left -= wk_n * (W4_STAGE_K / 2);
     }
+    ++fetched;
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < W4_STAGES - 1; ++i) fetch(i);
+  for (int i = 0; i < W4_STAGES - 1; ++i) fetch();
+
+  // scales of a stage: lane has row lane / 2, every second of the NS scales; read a stage ahead, they
+  // pass through shared memory as f32
+  const int64_t srow = int64_t(min(n0 + (lane >> 1), p.n - 1)) * p.ld_scales;
+  constexpr int PER = (NS + 1) / 2;
+  float next[PER];
+  auto scales = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int s = (lane & 1) + 2 * j;
+      if (s < NS) {
+        const int gi = min(qg_div(kb * 8 + s * GS, p.slices_per_group), p.groups - 1);
+        next[j] = dt_load(p.scales, srow + gi, p.scale_dtype);
+      }
+    }
+  };
+  if (mine > 0) scales(wk);
 
   float acc[NB][4];
   int col[NB];       // this lane's columns; those past the last row of x repeat it and are not used
@@ -178,7 +208,6 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
-  const int64_t s0 = int64_t(min(n0 + g, p.n - 1)) * p.ld_scales, s1 = int64_t(min(n0 + g + 8, p.n - 1)) * p.ld_scales;
 
   int i = 0;
   for (int p0 = 0; p0 < stages; p0 += p.panel) {
@@ -191,18 +220,17 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
     __syncthreads();
     for (; i < mine && wk + i * wk_n < p0 + in_panel; ++i) {
       const int kb = wk + i * wk_n;
-      float sc[8][2];
+      float (*sc)[16] = w4_scale[warp][i & 1];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const int gi = min(qg_div(kb * 8 + s, p.slices_per_group), p.groups - 1);
-        sc[s][0] = dt_load(p.scales, s0 + gi, p.scale_dtype);
-        sc[s][1] = dt_load(p.scales, s1 + gi, p.scale_dtype);
-      }
+      for (int j = 0; j < PER; ++j)
+        if ((lane & 1) + 2 * j < NS) sc[(lane & 1) + 2 * j][lane >> 1] = next[j];
       cp_async_wait<W4_STAGES - 2>();
       __syncwarp();
-      fetch(i + W4_STAGES - 1);
+      fetch();
+      if (i + 1 < mine) scales(kb + wk_n);
       const uint8_t* st = ring + (i % W4_STAGES) * W4_STAGE_BYTES + g * 128 + t * 4;
       const uint8_t* xs = panel + (kb - p0) * (W4_STAGE_K * 2) + t * 16;
+      float d[NB][4];
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         uint32_t a[4], c[4];
@@ -211,13 +239,16 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint4 x = *reinterpret_cast<const uint4*>(xs + col[b] + s * 64);
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_16816<BF16>(d, a[0], c[0], a[1], c[1], x.x, x.y);
-          mma_16816<BF16>(d, a[2], c[2], a[3], c[3], x.z, x.w);
-          acc[b][0] = fmaf(sc[s][0], d[0], acc[b][0]);
-          acc[b][1] = fmaf(sc[s][0], d[1], acc[b][1]);
-          acc[b][2] = fmaf(sc[s][1], d[2], acc[b][2]);
-          acc[b][3] = fmaf(sc[s][1], d[3], acc[b][3]);
+          if (s % GS == 0) mma_16816_first<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
+          else mma_16816<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
+          mma_16816<BF16>(d[b], a[2], c[2], a[3], c[3], x.z, x.w);
+          if (s % GS == GS - 1) {
+            const float u = sc[s / GS][g], v = sc[s / GS][g + 8];
+            acc[b][0] = fmaf(u, d[b][0], acc[b][0]);
+            acc[b][1] = fmaf(u, d[b][1], acc[b][1]);
+            acc[b][2] = fmaf(v, d[b][2], acc[b][2]);
+            acc[b][3] = fmaf(v, d[b][3], acc[b][3]);
+          }
         }
       }
     }
