@@ -2183,8 +2183,9 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
 
 namespace mira {
 
-// Row tiles of a block and stages of its panel of x.  More row tiles share one panel, fewer make more
-// blocks: the choice is the least of (blocks an SM runs one after the other) x (bytes a block brings in).
+// Row tiles of a block and stages of its panel of x.  More row tiles share one panel and need no
+// joining, fewer make more blocks: the choice is the least of (blocks an SM runs) x (bytes a block
+// brings in).
 static int w4_plan(const DeviceState* dev, W4Params& p) {
   const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
   const int most = (w4_panel_bytes(columns) / columns - 64) / (W4_STAGE_K * 2);      // stages that fit the panel
@@ -2209,18 +2210,20 @@ template <int XT, int NB, int GS>
 static int launch_w4_gs(DeviceState* dev, const W4Params& p) {
   auto kern = w4_matvec_kernel<XT, NB, GS>;
   static bool configured[kMaxDevices] = {};
-  const int join = W4_WARPS * NB * 8 * 16 * 4;
+  const int fixed = W4_RING + W4_WARPS * NB * 8 * 16 * 4;
   const int columns = (p.m < W4_ROWS ? p.m : W4_ROWS) * w4_pieces(p.x_dtype);
-  const int panel = columns * w4_pitch(p.panel);
-  const int most = W4_RING + (w4_panel_bytes(NB * 8) > join ? w4_panel_bytes(NB * 8) : join);
   if (!configured[dev->device]) {
-    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "cudaFuncSetAttribute(w4)");
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + w4_panel_bytes(NB * 8)),
+                  "cudaFuncSetAttribute(w4)");
     configured[dev->device] = true;
   }
-  const int64_t gx = (int64_t(p.n) + 16 * p.wr - 1) / (16 * p.wr), gy = (int64_t(p.m) + W4_ROWS - 1) / W4_ROWS;
+  const int64_t groups = (int64_t(p.n) + 16 * p.wr - 1) / (16 * p.wr), gy = (int64_t(p.m) + W4_ROWS - 1) / W4_ROWS;
   MIRA_CHECK_ARG(gy <= 65535, "matvec has too many rows");
-  const int smem = W4_RING + (panel > join ? panel : join);
-  kern<<<dim3(unsigned(gx), unsigned(gy)), W4_THREADS, smem, dev->stream>>>(p);
+  // as many blocks as run at once, each with the same number of row groups
+  const int64_t at_once = int64_t(dev->sm_count) * (columns <= 16 ? 2 : 1);
+  const int64_t rounds = (groups + at_once - 1) / at_once;
+  const int64_t gx = (groups + rounds - 1) / rounds;
+  kern<<<dim3(unsigned(gx), unsigned(gy)), W4_THREADS, fixed + columns * w4_pitch(p.panel), dev->stream>>>(p);
   return after_launch("w4_matvec_kernel");
 }
 

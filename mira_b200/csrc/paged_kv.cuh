@@ -59,6 +59,17 @@ __device__ __forceinline__ float dt_load(const void* p, int64_t i, int dtype) {
   return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
 }
 
+// The same in two steps, for a load that is issued well before its value is used: converting at once
+// would wait for it.
+__device__ __forceinline__ uint32_t dt_load_raw(const void* p, int64_t i, int dtype) {
+  return dtype == MIRA_DT_F32 ? __ldg(static_cast<const uint32_t*>(p) + i)
+                              : uint32_t(__ldg(static_cast<const uint16_t*>(p) + i));
+}
+__device__ __forceinline__ float dt_from_raw(uint32_t raw, int dtype) {
+  const float h = __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
+  return __uint_as_float(dtype == MIRA_DT_F32 ? raw : dtype == MIRA_DT_F16 ? __float_as_uint(h) : raw << 16);
+}
+
 __device__ __forceinline__ void dt_store(void* p, int64_t i, int dtype, float v) {
   if (dtype == MIRA_DT_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == MIRA_DT_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);

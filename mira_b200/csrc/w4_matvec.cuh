@@ -74,6 +74,13 @@ __host__ __device__ constexpr int w4_panel_bytes(int columns) { return columns <
 __host__ __device__ constexpr int w4_pieces(int x_dtype) { return x_dtype == MIRA_DT_F32 ? 3 : 1; }
 __host__ __device__ constexpr int w4_pitch(int stages) { return stages * W4_STAGE_K * 2 + 64; }
 
+// (w & mask) | base as one instruction: written in C it becomes two, each with its constant inside.
+__device__ __forceinline__ uint32_t w4_or(uint32_t w, uint32_t mask, uint32_t base) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(base));
+  return r;
+}
+
 // A word of eight weights as four registers of pairs (w0, w4), (w1, w5), (w2, w6), (w3, w7), each
 // w - 8: the nibble is or-ed under the exponent of 1024 (f16) or 128 (bf16), whose last mantissa bit
 // is worth 1, and the offset is subtracted exactly; f16 has room for a nibble shifted by four.
@@ -82,15 +89,15 @@ __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&a)[4]) {
   if (BF16) {
     const __nv_bfloat162 off = bits_b2(0x43084308u);     // 136
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = b2_bits(__hsub2(bits_b2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u), off));
+    for (int i = 0; i < 4; ++i) a[i] = b2_bits(__hsub2(bits_b2(w4_or(w >> (4 * i), 0x000f000fu, 0x43004300u)), off));
   } else {
     const __half2 off = bits_h2(0x64086408u);            // 1032
     const __half2 sixteenth = bits_h2(0x2c002c00u), off16 = bits_h2(0xd480d480u);   // 1 / 16, -72
     const uint32_t v = w >> 8;
-    a[0] = h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), off));
-    a[1] = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
-    a[2] = h2_bits(__hsub2(bits_h2((v & 0x000f000fu) | 0x64006400u), off));
-    a[3] = h2_bits(__hfma2(bits_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
+    a[0] = h2_bits(__hsub2(bits_h2(w4_or(w, 0x000f000fu, 0x64006400u)), off));
+    a[1] = h2_bits(__hfma2(bits_h2(w4_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
+    a[2] = h2_bits(__hsub2(bits_h2(w4_or(v, 0x000f000fu, 0x64006400u)), off));
+    a[3] = h2_bits(__hfma2(bits_h2(w4_or(v, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
   }
 }
 
@@ -149,129 +156,151 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int wk_n = W4_WARPS / p.wr, wr = warp % p.wr, wk = warp / p.wr;
   uint8_t* ring = w4_smem + warp * (W4_STAGES * W4_STAGE_BYTES);
-  uint8_t* panel = w4_smem + W4_RING;
+  float* red = reinterpret_cast<float*>(w4_smem + W4_RING);        // [warp][column][16 rows]
+  uint8_t* panel = w4_smem + W4_RING + W4_WARPS * NB * 8 * 16 * 4;
   const int pitch = w4_pitch(p.panel);
-  const int n0 = (blockIdx.x * p.wr + wr) * 16;
   const int m0 = blockIdx.y * W4_ROWS, rows = min(W4_ROWS, p.m - m0);
   const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;       // along k
   const int mine = stages > wk ? (stages - wk - 1) / wk_n + 1 : 0;
+  const int row_groups = (p.n + p.wr * 16 - 1) / (p.wr * 16);
+  const int rounds = (row_groups - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x);   // row groups of this block
 
   // this lane's four chunks of a stage: rows lane / 8 + 4 j, chunk lane % 8; rows past the last one
-  // read the last one and are not used
+  // read the last one and are not used.  The ring runs ahead over the row groups' ends.
   const uint8_t* from[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    from[j] = p.w + int64_t(min(n0 + (lane >> 3) + 4 * j, p.n - 1)) * p.ld_w + (wk * (W4_STAGE_K / 2) + (lane & 7) * 16);
+  const int first_byte = wk * (W4_STAGE_K / 2) + (lane & 7) * 16;
   const uint32_t to = smem_u32(ring) + (lane >> 3) * 128;
   const uint32_t swz = ((lane & 7) ^ (lane >> 3)) << 4;          // rows r and r + 4 differ in bit 6
-  int64_t left = p.ld_w - (wk * (W4_STAGE_K / 2) + (lane & 7) * 16);   // bytes of the rows from here on
-  int fetched = 0;
+  int f_round = 0, f_stage = 0, f_slot = 0;
+  int64_t left = 0;      // bytes of the rows from here on
+  auto aim = [&]() {
+    const int n0 = ((int(blockIdx.x) + f_round * int(gridDim.x)) * p.wr + wr) * 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) from[j] = p.w + int64_t(min(n0 + (lane >> 3) + 4 * j, p.n - 1)) * p.ld_w + first_byte;
+    left = p.ld_w - first_byte;
+  };
   auto fetch = [&]() {
-    if (fetched < mine) {
-      const uint32_t dst = to + (fetched % W4_STAGES) * W4_STAGE_BYTES;
-      const uint32_t bytes = left > 0 ? 16u : 0u;
+    if (f_round < rounds && mine > 0) {
+      const uint32_t dst = to + f_slot * W4_STAGE_BYTES;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        cp_async_16(dst + j * 512 + (j & 1 ? swz ^ 64 : swz), left > 0 ? from[j] : p.w, bytes);
+        cp_async_16(dst + j * 512 + (j & 1 ? swz ^ 64 : swz), left > 0 ? from[j] : p.w, left > 0 ? 16u : 0u);
         from[j] += wk_n * (W4_STAGE_K / 2);
       }
       left -= wk_n * (W4_STAGE_K / 2);
+      f_slot = f_slot + 1 == W4_STAGES ? 0 : f_slot + 1;
+      if (++f_stage == mine) {
+        f_stage = 0;
+        ++f_round;
+        aim();
+      }
     }
-    ++fetched;
     cp_async_commit();
   };
+  aim();
 #pragma unroll
   for (int i = 0; i < W4_STAGES - 1; ++i) fetch();
 
   // scales of a stage: lane has row lane / 2, every second of the NS scales; read a stage ahead, they
   // pass through shared memory as f32
-  const int64_t srow = int64_t(min(n0 + (lane >> 1), p.n - 1)) * p.ld_scales;
   constexpr int PER = (NS + 1) / 2;
-  float next[PER];
-  auto scales = [&](int kb) {
+  uint32_t next[PER];
+  auto scales = [&](int64_t srow, int kb) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int s = (lane & 1) + 2 * j;
       if (s < NS) {
         const int gi = min(qg_div(kb * 8 + s * GS, p.slices_per_group), p.groups - 1);
-        next[j] = dt_load(p.scales, srow + gi, p.scale_dtype);
+        next[j] = dt_load_raw(p.scales, srow + gi, p.scale_dtype);
       }
     }
   };
-  if (mine > 0) scales(wk);
 
-  float acc[NB][4];
   int col[NB];       // this lane's columns; those past the last row of x repeat it and are not used
 #pragma unroll
   for (int b = 0; b < NB; ++b) col[b] = min(b * 8 + g, rows * PIECES - 1) * pitch;
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
+  int slot = 0;
 
-  int i = 0;
-  for (int p0 = 0; p0 < stages; p0 += p.panel) {
-    const int in_panel = min(p.panel, stages - p0);
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows * in_panel * 32; e += W4_THREADS) {
-      const int r = e / (in_panel * 32), word = e - r * (in_panel * 32);
-      w4_stage_x<XT>(p, m0 + r, (p0 * 32 + word) * 8, panel + r * PIECES * pitch + word * 16, pitch);
-    }
-    __syncthreads();
-    for (; i < mine && wk + i * wk_n < p0 + in_panel; ++i) {
-      const int kb = wk + i * wk_n;
-      float (*sc)[16] = w4_scale[warp][i & 1];
+  for (int round = 0; round < rounds; ++round) {
+    const int n0 = ((int(blockIdx.x) + round * int(gridDim.x)) * p.wr + wr) * 16;
+    const int64_t srow = int64_t(min(n0 + (lane >> 1), p.n - 1)) * p.ld_scales;
+    if (mine > 0) scales(srow, wk);
+    float acc[NB][4];
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if ((lane & 1) + 2 * j < NS) sc[(lane & 1) + 2 * j][lane >> 1] = next[j];
-      cp_async_wait<W4_STAGES - 2>();
-      __syncwarp();
-      fetch();
-      if (i + 1 < mine) scales(kb + wk_n);
-      const uint8_t* st = ring + (i % W4_STAGES) * W4_STAGE_BYTES + g * 128 + t * 4;
-      const uint8_t* xs = panel + (kb - p0) * (W4_STAGE_K * 2) + t * 16;
-      float d[NB][4];
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        uint32_t a[4], c[4];
-        w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + ((s ^ g) << 4)), a);
-        w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + 1024 + ((s ^ g) << 4)), c);
+      for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
+
+    int i = 0;
+    for (int p0 = 0; p0 < stages; p0 += p.panel) {
+      const int in_panel = min(p.panel, stages - p0);
+      if (round == 0 || p.panel < stages) {       // else all of x is there already
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * in_panel * 32; e += W4_THREADS) {
+          const int r = e / (in_panel * 32), word = e - r * (in_panel * 32);
+          w4_stage_x<XT>(p, m0 + r, (p0 * 32 + word) * 8, panel + r * PIECES * pitch + word * 16, pitch);
+        }
+        __syncthreads();
+      }
+      for (; i < mine && wk + i * wk_n < p0 + in_panel; ++i) {
+        const int kb = wk + i * wk_n;
+        float (*sc)[16] = w4_scale[warp][i & 1];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint4 x = *reinterpret_cast<const uint4*>(xs + col[b] + s * 64);
-          if (s % GS == 0) mma_16816_first<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
-          else mma_16816<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
-          mma_16816<BF16>(d[b], a[2], c[2], a[3], c[3], x.z, x.w);
-          if (s % GS == GS - 1) {
-            const float u = sc[s / GS][g], v = sc[s / GS][g + 8];
-            acc[b][0] = fmaf(u, d[b][0], acc[b][0]);
-            acc[b][1] = fmaf(u, d[b][1], acc[b][1]);
-            acc[b][2] = fmaf(v, d[b][2], acc[b][2]);
-            acc[b][3] = fmaf(v, d[b][3], acc[b][3]);
+        for (int j = 0; j < PER; ++j)
+          if ((lane & 1) + 2 * j < NS) sc[(lane & 1) + 2 * j][lane >> 1] = dt_from_raw(next[j], p.scale_dtype);
+        cp_async_wait<W4_STAGES - 2>();
+        __syncwarp();
+        fetch();
+        if (i + 1 < mine) scales(srow, kb + wk_n);
+        const uint8_t* st = ring + slot * W4_STAGE_BYTES + g * 128 + t * 4;
+        slot = slot + 1 == W4_STAGES ? 0 : slot + 1;
+        const uint8_t* xs = panel + (kb - p0) * (W4_STAGE_K * 2) + t * 16;
+        float d[NB][4];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          uint32_t a[4], c[4];
+          w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + ((s ^ g) << 4)), a);
+          w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + 1024 + ((s ^ g) << 4)), c);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint4 x = *reinterpret_cast<const uint4*>(xs + col[b] + s * 64);
+            if (s % GS == 0) mma_16816_first<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
+            else mma_16816<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
+            mma_16816<BF16>(d[b], a[2], c[2], a[3], c[3], x.z, x.w);
+            if (s % GS == GS - 1) {
+              const float u = sc[s / GS][g], v = sc[s / GS][g + 8];
+              acc[b][0] = fmaf(u, d[b][0], acc[b][0]);
+              acc[b][1] = fmaf(u, d[b][1], acc[b][1]);
+              acc[b][2] = fmaf(v, d[b][2], acc[b][2]);
+              acc[b][3] = fmaf(v, d[b][3], acc[b][3]);
+            }
           }
         }
       }
     }
+
+    // the shares of k and the pieces of x, joined through shared memory; a warp that owns all of k
+    // waits for no other
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) red[(warp * NB * 8 + b * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = acc[b][j];
+    if (wk_n > 1) __syncthreads();
+    else __syncwarp();
+    const int tile_n = wk_n > 1 ? p.wr * 16 : 16, tile0 = wk_n > 1 ? n0 - wr * 16 : n0;
+    for (int e = wk_n > 1 ? threadIdx.x : lane; e < rows * tile_n; e += wk_n > 1 ? W4_THREADS : 32) {
+      const int r = e / tile_n, c = e - r * tile_n, n = tile0 + c;
+      if (n >= p.n) continue;
+      const int w0 = wk_n > 1 ? c >> 4 : warp;
+      float y = 0.0f;
+      for (int q = PIECES - 1; q >= 0; --q)
+        for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + w0) * NB * 8 + r * PIECES + q) * 16 + (c & 15)];
+      dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
+    }
+    if (wk_n > 1) __syncthreads();
+    else __syncwarp();
   }
   cp_async_wait<0>();
-  __syncthreads();
-
-  // the shares of k and the pieces of x, joined in the panel: [warp][column][16 rows]
-  float* red = reinterpret_cast<float*>(panel);
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) red[(warp * NB * 8 + b * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = acc[b][j];
-  __syncthreads();
-  const int tile_n = p.wr * 16;
-  for (int e = threadIdx.x; e < rows * tile_n; e += W4_THREADS) {
-    const int r = e / tile_n, c = e - r * tile_n, n = blockIdx.x * tile_n + c;
-    if (n >= p.n) continue;
-    float y = 0.0f;
-    for (int q = PIECES - 1; q >= 0; --q)
-      for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + (c >> 4)) * NB * 8 + r * PIECES + q) * 16 + (c & 15)];
-    dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
-  }
 }
 
 }  // namespace mira
