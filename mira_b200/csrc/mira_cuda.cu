@@ -2183,63 +2183,94 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
 
 namespace mira {
 
-// Row tiles of a block and stages of its panel of x.  More row tiles share one panel and need no
-// joining, fewer make more blocks: the choice is the least of (blocks an SM runs) x (bytes a block
-// brings in).
-static int w4_plan(const DeviceState* dev, W4Params& p) {
-  const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
-  const int most = (w4_panel_bytes(columns) / columns - 64) / (W4_STAGE_K * 2);      // stages that fit the panel
+static int w4_nb(int x_dtype, int m) {
+  if (x_dtype == MIRA_DT_F32) return m <= 2 ? 1 : 3;
+  return m <= 8 ? 1 : 2;
+}
+static int w4_gs(int64_t group) { return group % 256 == 0 ? 8 : group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1; }
+
+// Row tiles of a block, blocks along k, and stages of the panel of x.  More row tiles share one panel
+// and need less joining, fewer divide the rows more evenly; cuts along k do both at the price of a
+// second pass over the sums.  The choice is the least of what a block brings in, in bytes per SM: its
+// weights and x, and for cut sums about what an SM could read in the time of writing, signalling and
+// adding them (1.5 us at 50 bytes a clock).  `gs` as for the kernel; 1 holds for every group.
+static int w4_plan(int sm_count, int gs, W4Params& p) {
+  const int at_once = sm_count * W4_BLOCKS;
+  const int pass = w4_rows(p.x_dtype), rows = p.m < pass ? p.m : pass, columns = rows * w4_pieces(p.x_dtype);
+  const int room = W4_SMEM - w4_fixed(w4_nb(p.x_dtype, rows), gs);
+  const int most = (room / columns - 64) / (W4_STAGE_K * 2);        // stages that fit the panel
   const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;
   const int64_t tiles = (int64_t(p.n) + 15) / 16;
   int64_t best = INT64_MAX;
-  for (int wr = 8; wr >= 1; wr /= 2) {
-    const int share = 8 / wr;
-    if (share > most && wr < 8) break;
-    const int64_t blocks = (tiles + wr - 1) / wr;
-    const int64_t cost = (blocks + dev->sm_count - 1) / dev->sm_count * (int64_t(wr) * 8 + rows * dt_size(p.x_dtype));
-    if (cost >= best) continue;
-    best = cost;
-    p.wr = wr;
-    const int want = (stages + share - 1) / share * share, fit = most / share * share;
-    p.panel = want < fit ? want : fit;
+  for (int cuts = 1; cuts <= (p.m <= pass ? 8 : 1); cuts *= 2) {
+    const int per = (stages + cuts - 1) / cuts;
+    if (cuts > 1 && (cuts - 1) * per >= stages) break;               // a cut without work
+    for (int wr = W4_WARPS; wr >= 1; wr /= 2) {
+      const int share = W4_WARPS / wr;
+      if (share > most) break;
+      const int64_t groups = (tiles + wr - 1) / wr;
+      const int64_t rounds = (groups * cuts + at_once - 1) / at_once;
+      const bool whole = most / share * share >= per;
+      const int64_t weights = rounds * wr * 16 * per * (W4_STAGE_K / 2);
+      const int64_t x = int64_t(rows) * per * W4_STAGE_K * dt_size(p.x_dtype) * (whole ? 1 : rounds);
+      const int64_t cost = weights + x + (cuts > 1 ? 140000 : 0);
+      if (cost >= best) continue;
+      best = cost;
+      p.wr = wr;
+      p.cuts = cuts;
+      p.cut_stages = per;
+      const int want = (per + share - 1) / share * share, fit = most / share * share;
+      p.panel = want < fit ? want : fit;
+    }
   }
   return p.panel > 0 ? MIRA_CUDA_OK : set_error(MIRA_CUDA_EINVAL, "no room for the rows of x");
 }
 
-template <int XT, int NB, int GS>
-static int launch_w4_gs(DeviceState* dev, const W4Params& p) {
-  auto kern = w4_matvec_kernel<XT, NB, GS>;
+static int64_t w4_counters(int64_t n) { return round_up((n + 15) / 16 * 4, 256); }
+
+template <int XT, int NB, int GS, bool EXACT>
+static int launch_w4_kernel(DeviceState* dev, const W4Params& p) {
+  auto kern = w4_matvec_kernel<XT, NB, GS, EXACT>;
   static bool configured[kMaxDevices] = {};
-  const int fixed = W4_RING + W4_WARPS * NB * 8 * 16 * 4;
-  const int columns = (p.m < W4_ROWS ? p.m : W4_ROWS) * w4_pieces(p.x_dtype);
   if (!configured[dev->device]) {
-    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + w4_panel_bytes(NB * 8)),
-                  "cudaFuncSetAttribute(w4)");
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM), "cudaFuncSetAttribute(w4)");
     configured[dev->device] = true;
   }
-  const int64_t groups = (int64_t(p.n) + 16 * p.wr - 1) / (16 * p.wr), gy = (int64_t(p.m) + W4_ROWS - 1) / W4_ROWS;
+  const int pass = w4_rows(XT), columns = (p.m < pass ? p.m : pass) * w4_pieces(XT);
+  const int64_t groups = (int64_t(p.n) + 16 * p.wr - 1) / (16 * p.wr), gy = (int64_t(p.m) + pass - 1) / pass;
   MIRA_CHECK_ARG(gy <= 65535, "matvec has too many rows");
   // as many blocks as run at once, each with the same number of row groups
-  const int64_t at_once = int64_t(dev->sm_count) * (columns <= 16 ? 2 : 1);
-  const int64_t rounds = (groups + at_once - 1) / at_once;
-  const int64_t gx = (groups + rounds - 1) / rounds;
-  kern<<<dim3(unsigned(gx), unsigned(gy)), W4_THREADS, fixed + columns * w4_pitch(p.panel), dev->stream>>>(p);
+  const int64_t at_once = int64_t(dev->sm_count) * W4_BLOCKS;
+  const int64_t rounds = (groups * p.cuts + at_once - 1) / at_once;
+  const dim3 grid(unsigned((groups + rounds - 1) / rounds), unsigned(gy), unsigned(p.cuts));
+  kern<<<grid, W4_THREADS, w4_fixed(NB, GS) + columns * w4_pitch(p.panel), dev->stream>>>(p);
   return after_launch("w4_matvec_kernel");
 }
 
 template <int XT, int NB>
 static int launch_w4(DeviceState* dev, const W4Params& p, int64_t group) {
-  if (group % 256 == 0) return launch_w4_gs<XT, NB, 8>(dev, p);
-  if (group % 128 == 0) return launch_w4_gs<XT, NB, 4>(dev, p);
-  if (group % 64 == 0) return launch_w4_gs<XT, NB, 2>(dev, p);
-  return launch_w4_gs<XT, NB, 1>(dev, p);
+  switch (w4_gs(group)) {
+    case 8: return group == 256 ? launch_w4_kernel<XT, NB, 8, true>(dev, p) : launch_w4_kernel<XT, NB, 8, false>(dev, p);
+    case 4: return group == 128 ? launch_w4_kernel<XT, NB, 4, true>(dev, p) : launch_w4_kernel<XT, NB, 4, false>(dev, p);
+    case 2: return group == 64 ? launch_w4_kernel<XT, NB, 2, true>(dev, p) : launch_w4_kernel<XT, NB, 2, false>(dev, p);
+    default: return group == 32 ? launch_w4_kernel<XT, NB, 1, true>(dev, p) : launch_w4_kernel<XT, NB, 1, false>(dev, p);
+  }
 }
 
 }  // namespace mira
 
 extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k) {
-  (void)m; (void)n; (void)k;
-  return 0;
+  DeviceState* dev = current_device();
+  if (dev == nullptr || m <= 0 || m > INT32_MAX || n <= 0 || n > INT32_MAX || k <= 0 || k > (1 << 30)) return 0;
+  int cuts = 1;
+  for (int dtype : {MIRA_DT_F32, MIRA_DT_F16, MIRA_DT_BF16})
+    for (int gs = 1; gs <= 8; gs *= 2) {
+      W4Params p;
+      std::memset(&p, 0, sizeof(p));
+      p.m = int(m); p.n = int(n); p.k = int(k); p.x_dtype = dtype;
+      if (w4_plan(dev->sm_count, gs, p) == MIRA_CUDA_OK && p.cuts > cuts) cuts = p.cuts;
+    }
+  return cuts > 1 ? w4_counters(n) + int64_t(cuts) * m * n * 4 : 0;
 }
 
 extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
@@ -2279,16 +2310,19 @@ extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   p.slices_per_group = make_div(group / 32);
   p.x_dtype = a->x_dtype; p.scale_dtype = a->scale_dtype; p.out_dtype = a->out_dtype;
   p.x_vec = aligned_to(a->x, 16) && a->ld_x * dt_size(a->x_dtype) % 16 == 0;
-  const int rc = w4_plan(dev, p);
+  const int rc = w4_plan(dev->sm_count, w4_gs(group), p);
   if (rc != MIRA_CUDA_OK) return rc;
-  const int rows = p.m < W4_ROWS ? p.m : W4_ROWS, columns = rows * w4_pieces(p.x_dtype);
+  if (p.cuts > 1) {
+    MIRA_CHECK_ARG(a->workspace != nullptr && aligned_to(a->workspace, 16) &&
+                       a->workspace_bytes >= w4_counters(p.n) + int64_t(p.cuts) * p.m * p.n * 4,
+                   "workspace smaller than mira_cuda_w4_matvec_workspace()");
+    p.counters = static_cast<int*>(a->workspace);
+    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + w4_counters(p.n));
+  }
+  const int nb = w4_nb(p.x_dtype, p.m);
   switch (p.x_dtype) {
-    case MIRA_DT_F16: return columns <= 8 ? launch_w4<MIRA_DT_F16, 1>(dev, p, group) : launch_w4<MIRA_DT_F16, 2>(dev, p, group);
-    case MIRA_DT_BF16: return columns <= 8 ? launch_w4<MIRA_DT_BF16, 1>(dev, p, group) : launch_w4<MIRA_DT_BF16, 2>(dev, p, group);
-    default:
-      if (columns <= 8) return launch_w4<MIRA_DT_F32, 1>(dev, p, group);
-      if (columns <= 16) return launch_w4<MIRA_DT_F32, 2>(dev, p, group);
-      if (columns <= 24) return launch_w4<MIRA_DT_F32, 3>(dev, p, group);
-      return launch_w4<MIRA_DT_F32, 6>(dev, p, group);
+    case MIRA_DT_F16: return nb == 1 ? launch_w4<MIRA_DT_F16, 1>(dev, p, group) : launch_w4<MIRA_DT_F16, 2>(dev, p, group);
+    case MIRA_DT_BF16: return nb == 1 ? launch_w4<MIRA_DT_BF16, 1>(dev, p, group) : launch_w4<MIRA_DT_BF16, 2>(dev, p, group);
+    default: return nb == 1 ? launch_w4<MIRA_DT_F32, 1>(dev, p, group) : launch_w4<MIRA_DT_F32, 3>(dev, p, group);
   }
 }

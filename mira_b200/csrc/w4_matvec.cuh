@@ -11,11 +11,14 @@
 // exactly, so every product is exact and sums are f32.
 //
 // Layout.  A warp owns 16 weight rows and walks along k in stages of 256 (16 rows x 128 bytes), brought
-// to its own ring in shared memory by cp.async (16-byte chunks, chunk c of row r at c ^ (r % 8), so
-// that the fragment reads of eight rows are free of bank conflicts).  A slice of 32 k is one chunk and
-// lies in one group: its two products start from zero and are added scaled.  The eight warps of a
-// block are WR row tiles times 8 / WR interleaved shares of k (joined in shared memory at the end); the
-// block's x is staged in a panel, whole where it fits, k in the fragments' order.
+// to its own ring in shared memory by cp.async (rows 144 bytes apart: the fragment reads of eight rows
+// then fall on different banks without address arithmetic).  A slice of 32 k is 16 bytes of a row and
+// lies in one group: the products of a group's slices of a stage are summed, then added scaled.  The
+// eight warps of a block are wr row tiles times 8 / wr interleaved shares of k (a remainder idles), joined in shared
+// memory; x is staged in a panel, whole where it fits, k in the fragments' order.  Blocks go through
+// row groups with the ring running ahead over their ends.  Where the rows alone would leave SMs idle,
+// or x is wide, k is also cut over blocks (blockIdx.z); the parts are joined in order by the block
+// that finishes last.
 #pragma once
 #include <cstdint>
 
@@ -35,6 +38,9 @@ struct W4Params {
   QgDiv slices_per_group;     // group / 32
   int wr;                     // row tiles of a block: 1, 2, 4 or 8
   int panel;                  // stages of x in shared memory, a multiple of 8 / wr
+  int cuts, cut_stages;       // blocks along k and the stages of each
+  float* part;                // [cut][m][n] sums of each cut
+  int* counters;              // [row group], zero between calls
   int x_vec;                  // rows of x can be read 16 bytes at a time
   int x_dtype, scale_dtype, out_dtype;
   int n_steps;
@@ -60,19 +66,26 @@ __device__ __forceinline__ float w4_steps(const W4Params& p, float y, int m, int
 
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
-constexpr int W4_ROWS = 16;                  // rows of x per pass over the weights
-constexpr int W4_STAGES = 4;
+constexpr int W4_STAGES = 3;
 constexpr int W4_STAGE_K = 256;
-constexpr int W4_STAGE_BYTES = 16 * W4_STAGE_K / 2;
+constexpr int W4_SLICES = W4_STAGE_K / 32;
+constexpr int W4_ROW_PITCH = W4_STAGE_K / 2 + 16;     // bytes of a row of a stage in shared memory
+constexpr int W4_STAGE_BYTES = 16 * W4_ROW_PITCH;
 constexpr int W4_RING = W4_WARPS * W4_STAGES * W4_STAGE_BYTES;
-// Bytes of the panel: two blocks per SM while x is narrow, one for many columns, whose panels would
-// otherwise be a stage or two long.
-__host__ __device__ constexpr int w4_panel_bytes(int columns) { return columns <= 16 ? 48 << 10 : 128 << 10; }
+constexpr int W4_BLOCKS = 2;                         // per SM
+constexpr int W4_SMEM = 112 << 10;
 
-// Columns of the right operand that a row of x takes, and bytes of a column with `stages` stages (64
-// more than a multiple of 128: the fragment reads of two columns then cover all banks).
+// Rows of x per pass over the weights, and the columns a row takes: an f32 row is three.  Up to two
+// f32 rows their columns are adjacent in one block of eight; more rows have a block per piece.
+__host__ __device__ constexpr int w4_rows(int x_dtype) { return x_dtype == MIRA_DT_F32 ? 8 : 16; }
 __host__ __device__ constexpr int w4_pieces(int x_dtype) { return x_dtype == MIRA_DT_F32 ? 3 : 1; }
+// Bytes of a column with `stages` stages: 64 more than a multiple of 128, so that the fragment reads of
+// two columns cover all banks.
 __host__ __device__ constexpr int w4_pitch(int stages) { return stages * W4_STAGE_K * 2 + 64; }
+// Shared memory beside the panel: the ring, two buffers of joined sums, a stage's scales per warp.
+__host__ __device__ constexpr int w4_fixed(int nb, int gs) {
+  return W4_RING + 2 * W4_WARPS * (nb == 3 ? 1 : nb) * 8 * 16 * 4 + W4_WARPS * (W4_SLICES / gs) * 16 * 4;
+}
 
 // (w & mask) | base as one instruction: written in C it becomes two, each with its constant inside.
 __device__ __forceinline__ uint32_t w4_or(uint32_t w, uint32_t mask, uint32_t base) {
@@ -83,23 +96,33 @@ __device__ __forceinline__ uint32_t w4_or(uint32_t w, uint32_t mask, uint32_t ba
 
 // A word of eight weights as four registers of pairs (w0, w4), (w1, w5), (w2, w6), (w3, w7), each
 // w - 8: the nibble is or-ed under the exponent of 1024 (f16) or 128 (bf16), whose last mantissa bit
-// is worth 1, and the offset is subtracted exactly; f16 has room for a nibble shifted by four.
+// is worth 1, and the offset is subtracted exactly; f16 has room for a nibble shifted by four.  The
+// constants are held in registers: the compiler would set them anew before every use.
 template <bool BF16>
-__device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&a)[4]) {
-  if (BF16) {
-    const __nv_bfloat162 off = bits_b2(0x43084308u);     // 136
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = b2_bits(__hsub2(bits_b2(w4_or(w >> (4 * i), 0x000f000fu, 0x43004300u)), off));
-  } else {
-    const __half2 off = bits_h2(0x64086408u);            // 1032
-    const __half2 sixteenth = bits_h2(0x2c002c00u), off16 = bits_h2(0xd480d480u);   // 1 / 16, -72
-    const uint32_t v = w >> 8;
-    a[0] = h2_bits(__hsub2(bits_h2(w4_or(w, 0x000f000fu, 0x64006400u)), off));
-    a[1] = h2_bits(__hfma2(bits_h2(w4_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
-    a[2] = h2_bits(__hsub2(bits_h2(w4_or(v, 0x000f000fu, 0x64006400u)), off));
-    a[3] = h2_bits(__hfma2(bits_h2(w4_or(v, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
+struct W4Unpack {
+  uint32_t low, high, base, off, sixteenth, off16;
+  __device__ __forceinline__ static uint32_t pin(uint32_t v) {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
   }
-}
+  __device__ __forceinline__ W4Unpack()
+      : low(pin(0x000f000fu)), high(pin(0x00f000f0u)), base(pin(BF16 ? 0x43004300u : 0x64006400u)),
+        off(pin(BF16 ? 0x43084308u : 0x64086408u)),                  // 136 or 1032
+        sixteenth(pin(0x2c002c00u)), off16(pin(0xd480d480u)) {}       // f16: 1 / 16, -72
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&a)[4]) const {
+    if (BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = b2_bits(__hsub2(bits_b2(w4_or(w >> (4 * i), low, base)), bits_b2(off)));
+    } else {
+      const uint32_t v = w >> 8;
+      a[0] = h2_bits(__hsub2(bits_h2(w4_or(w, low, base)), bits_h2(off)));
+      a[1] = h2_bits(__hfma2(bits_h2(w4_or(w, high, base)), bits_h2(sixteenth), bits_h2(off16)));
+      a[2] = h2_bits(__hsub2(bits_h2(w4_or(v, low, base)), bits_h2(off)));
+      a[3] = h2_bits(__hfma2(bits_h2(w4_or(v, high, base)), bits_h2(sixteenth), bits_h2(off16)));
+    }
+  }
+};
 
 // Eight values of a row of x from element k on (0 past the end), in the order of the fragments.
 template <int XT>
@@ -144,55 +167,61 @@ __device__ __forceinline__ void w4_stage_x(const W4Params& p, int row, int k, ui
   }
 }
 
-// XT: type of x; NB: blocks of eight columns; GS: slices whose products are summed before the scale is
-// applied, a divisor of the slices of a group.
-template <int XT, int NB, int GS>
-__global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_constant__ W4Params p) {
+// XT: type of x; NB: blocks of eight columns (3: one per piece); GS: slices whose products are summed
+// before the scale is applied, a divisor of the slices of a group (EXACT: all of them).
+template <int XT, int NB, int GS, bool EXACT>
+__global__ void __launch_bounds__(W4_THREADS, W4_BLOCKS) w4_matvec_kernel(const __grid_constant__ W4Params p) {
   constexpr bool BF16 = XT != MIRA_DT_F16;
-  constexpr int PIECES = w4_pieces(XT);
-  constexpr int NS = 8 / GS;               // scales of a row per stage
+  constexpr int PIECES = w4_pieces(XT), ROWS = w4_rows(XT);
+  constexpr bool SPLIT = NB == 3;                // a block of columns per piece
+  constexpr int OB = SPLIT ? 1 : NB;             // blocks of columns after the pieces are added
+  constexpr int NS = W4_SLICES / GS;             // scales of a row per stage
   extern __shared__ __align__(128) uint8_t w4_smem[];
-  __shared__ float w4_scale[W4_WARPS][2][NS][16];
+  __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int wk_n = W4_WARPS / p.wr, wr = warp % p.wr, wk = warp / p.wr;
   uint8_t* ring = w4_smem + warp * (W4_STAGES * W4_STAGE_BYTES);
-  float* red = reinterpret_cast<float*>(w4_smem + W4_RING);        // [warp][column][16 rows]
-  uint8_t* panel = w4_smem + W4_RING + W4_WARPS * NB * 8 * 16 * 4;
+  float* red0 = reinterpret_cast<float*>(w4_smem + W4_RING);        // two of [warp][column][16 rows]
+  float* sc = red0 + 2 * W4_WARPS * OB * 8 * 16 + warp * (NS * 16);  // [scale][8][row g, row g + 8]
+  uint8_t* panel = w4_smem + w4_fixed(NB, GS);
   const int pitch = w4_pitch(p.panel);
-  const int m0 = blockIdx.y * W4_ROWS, rows = min(W4_ROWS, p.m - m0);
-  const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;       // along k
+  const int m0 = blockIdx.y * ROWS, rows = min(ROWS, p.m - m0);
+  const int first = blockIdx.z * p.cut_stages;                  // this block's stages along k
+  const int stages = min(p.cut_stages, (p.k + W4_STAGE_K - 1) / W4_STAGE_K - first);
   const int mine = stages > wk ? (stages - wk - 1) / wk_n + 1 : 0;
   const int row_groups = (p.n + p.wr * 16 - 1) / (p.wr * 16);
   const int rounds = (row_groups - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x);   // row groups of this block
+  auto tile_row = [&](int round) { return ((int(blockIdx.x) + round * int(gridDim.x)) * p.wr + wr) * 16; };
 
-  // this lane's four chunks of a stage: rows lane / 8 + 4 j, chunk lane % 8; rows past the last one
-  // read the last one and are not used.  The ring runs ahead over the row groups' ends.
-  const uint8_t* from[4];
-  const int first_byte = wk * (W4_STAGE_K / 2) + (lane & 7) * 16;
-  const uint32_t to = smem_u32(ring) + (lane >> 3) * 128;
-  const uint32_t swz = ((lane & 7) ^ (lane >> 3)) << 4;          // rows r and r + 4 differ in bit 6
+  // this lane's chunks of a stage: rows lane / 8 + 4 j, chunk lane % 8; rows past the last one read the
+  // last one and are not used.  The ring runs ahead over the row groups' ends.
+  constexpr int CHUNKS = W4_STAGE_K / 32, TURNS = 16 * CHUNKS / 32;
+  const int first_byte = (first + wk) * (W4_STAGE_K / 2) + (lane % CHUNKS) * 16;
+  const uint32_t to = smem_u32(ring) + (lane / CHUNKS) * W4_ROW_PITCH + (lane % CHUNKS) * 16;
   int f_round = 0, f_stage = 0, f_slot = 0;
+  const uint8_t* from[TURNS];
   int64_t left = 0;      // bytes of the rows from here on
   auto aim = [&]() {
-    const int n0 = ((int(blockIdx.x) + f_round * int(gridDim.x)) * p.wr + wr) * 16;
+    const int n0 = tile_row(f_round);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) from[j] = p.w + int64_t(min(n0 + (lane >> 3) + 4 * j, p.n - 1)) * p.ld_w + first_byte;
+    for (int j = 0; j < TURNS; ++j)
+      from[j] = p.w + int64_t(min(n0 + lane / CHUNKS + (32 / CHUNKS) * j, p.n - 1)) * p.ld_w + first_byte;
     left = p.ld_w - first_byte;
   };
   auto fetch = [&]() {
     if (f_round < rounds && mine > 0) {
       const uint32_t dst = to + f_slot * W4_STAGE_BYTES;
+      const uint32_t bytes = left > 0 ? 16u : 0u;        // past a row's end: zeros, nothing is read
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        cp_async_16(dst + j * 512 + (j & 1 ? swz ^ 64 : swz), left > 0 ? from[j] : p.w, left > 0 ? 16u : 0u);
+      for (int j = 0; j < TURNS; ++j) {
+        cp_async_16(dst + j * (32 / CHUNKS) * W4_ROW_PITCH, from[j], bytes);
         from[j] += wk_n * (W4_STAGE_K / 2);
       }
       left -= wk_n * (W4_STAGE_K / 2);
       f_slot = f_slot + 1 == W4_STAGES ? 0 : f_slot + 1;
       if (++f_stage == mine) {
         f_stage = 0;
-        ++f_round;
-        aim();
+        if (++f_round < rounds) aim();
       }
     }
     cp_async_commit();
@@ -202,29 +231,32 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
   for (int i = 0; i < W4_STAGES - 1; ++i) fetch();
 
   // scales of a stage: lane has row lane / 2, every second of the NS scales; read a stage ahead, they
-  // pass through shared memory as f32
+  // pass through shared memory as f32.  Past the last group x is zero and so is the scale.
   constexpr int PER = (NS + 1) / 2;
   uint32_t next[PER];
-  auto scales = [&](int64_t srow, int kb) {
+  int64_t srow = 0;
+  auto scales = [&](int kb) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int s = (lane & 1) + 2 * j;
-      if (s < NS) {
-        const int gi = min(qg_div(kb * 8 + s * GS, p.slices_per_group), p.groups - 1);
-        next[j] = dt_load_raw(p.scales, srow + gi, p.scale_dtype);
-      }
+      const int gi = EXACT ? kb * NS + s : qg_div(kb * W4_SLICES + s * GS, p.slices_per_group);
+      next[j] = s < NS && gi < p.groups ? dt_load_raw(p.scales, srow + gi, p.scale_dtype) : 0u;
     }
   };
+  auto aim_scales = [&](int round) { srow = int64_t(min(tile_row(round) + (lane >> 1), p.n - 1)) * p.ld_scales; };
+  aim_scales(0);
+  scales(first + wk);
 
   int col[NB];       // this lane's columns; those past the last row of x repeat it and are not used
 #pragma unroll
-  for (int b = 0; b < NB; ++b) col[b] = min(b * 8 + g, rows * PIECES - 1) * pitch;
+  for (int b = 0; b < NB; ++b)
+    col[b] = SPLIT ? (b * rows + min(g, rows - 1)) * pitch : min(b * 8 + g, rows * PIECES - 1) * pitch;
+  const int row_step = SPLIT ? pitch : PIECES * pitch, piece_step = SPLIT ? rows * pitch : pitch;
+  const W4Unpack<BF16> unpack;
   int slot = 0;
 
   for (int round = 0; round < rounds; ++round) {
-    const int n0 = ((int(blockIdx.x) + round * int(gridDim.x)) * p.wr + wr) * 16;
-    const int64_t srow = int64_t(min(n0 + (lane >> 1), p.n - 1)) * p.ld_scales;
-    if (mine > 0) scales(srow, wk);
+    const int n0 = tile_row(round);
     float acc[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -236,43 +268,51 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
       const int in_panel = min(p.panel, stages - p0);
       if (round == 0 || p.panel < stages) {       // else all of x is there already
         __syncthreads();
-        for (int e = threadIdx.x; e < rows * in_panel * 32; e += W4_THREADS) {
-          const int r = e / (in_panel * 32), word = e - r * (in_panel * 32);
-          w4_stage_x<XT>(p, m0 + r, (p0 * 32 + word) * 8, panel + r * PIECES * pitch + word * 16, pitch);
+        const int words = in_panel * (W4_STAGE_K / 8);
+        for (int e = threadIdx.x; e < rows * words; e += W4_THREADS) {
+          const int r = e / words, word = e - r * words;
+          w4_stage_x<XT>(p, m0 + r, (first + p0) * W4_STAGE_K + word * 8, panel + r * row_step + word * 16, piece_step);
         }
         __syncthreads();
       }
       for (; i < mine && wk + i * wk_n < p0 + in_panel; ++i) {
         const int kb = wk + i * wk_n;
-        float (*sc)[16] = w4_scale[warp][i & 1];
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if ((lane & 1) + 2 * j < NS) sc[(lane & 1) + 2 * j][lane >> 1] = dt_from_raw(next[j], p.scale_dtype);
         cp_async_wait<W4_STAGES - 2>();
         __syncwarp();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int s = (lane & 1) + 2 * j;
+          if (s < NS) sc[s * 16 + ((lane >> 1) & 7) * 2 + (lane >> 4)] = dt_from_raw(next[j], p.scale_dtype);
+        }
         fetch();
-        if (i + 1 < mine) scales(srow, kb + wk_n);
-        const uint8_t* st = ring + slot * W4_STAGE_BYTES + g * 128 + t * 4;
+        const bool ends = i + 1 == mine;
+        if (ends) aim_scales(round + 1);
+        scales(first + (ends ? wk : kb + wk_n));
+        __syncwarp();
+        const uint8_t* st = ring + slot * W4_STAGE_BYTES + g * W4_ROW_PITCH + t * 4;
         slot = slot + 1 == W4_STAGES ? 0 : slot + 1;
         const uint8_t* xs = panel + (kb - p0) * (W4_STAGE_K * 2) + t * 16;
         float d[NB][4];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
+        for (int s = 0; s < W4_SLICES; ++s) {
           uint32_t a[4], c[4];
-          w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + ((s ^ g) << 4)), a);
-          w4_unpack<BF16>(*reinterpret_cast<const uint32_t*>(st + 1024 + ((s ^ g) << 4)), c);
+          unpack(*reinterpret_cast<const uint32_t*>(st + s * 16), a);
+          unpack(*reinterpret_cast<const uint32_t*>(st + 8 * W4_ROW_PITCH + s * 16), c);
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             const uint4 x = *reinterpret_cast<const uint4*>(xs + col[b] + s * 64);
             if (s % GS == 0) mma_16816_first<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
             else mma_16816<BF16>(d[b], a[0], c[0], a[1], c[1], x.x, x.y);
             mma_16816<BF16>(d[b], a[2], c[2], a[3], c[3], x.z, x.w);
-            if (s % GS == GS - 1) {
-              const float u = sc[s / GS][g], v = sc[s / GS][g + 8];
-              acc[b][0] = fmaf(u, d[b][0], acc[b][0]);
-              acc[b][1] = fmaf(u, d[b][1], acc[b][1]);
-              acc[b][2] = fmaf(v, d[b][2], acc[b][2]);
-              acc[b][3] = fmaf(v, d[b][3], acc[b][3]);
+          }
+          if (s % GS == GS - 1) {
+            const float2 u = *reinterpret_cast<const float2*>(sc + (s / GS) * 16 + g * 2);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              acc[b][0] = fmaf(u.x, d[b][0], acc[b][0]);
+              acc[b][1] = fmaf(u.x, d[b][1], acc[b][1]);
+              acc[b][2] = fmaf(u.y, d[b][2], acc[b][2]);
+              acc[b][3] = fmaf(u.y, d[b][3], acc[b][3]);
             }
           }
         }
@@ -280,11 +320,17 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
     }
 
     // the shares of k and the pieces of x, joined through shared memory; a warp that owns all of k
-    // waits for no other
+    // waits for no other.  Two buffers take turns, so one barrier a round is enough.
+    if (SPLIT) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+      for (int j = 0; j < 4; ++j) acc[0][j] = (acc[2 % NB][j] + acc[1 % NB][j]) + acc[0][j];
+    }
+    constexpr int JOIN = SPLIT ? 1 : PIECES;      // columns still to be added per row
+    float* red = red0 + (round & 1) * (W4_WARPS * OB * 8 * 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) red[(warp * NB * 8 + b * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = acc[b][j];
+    for (int b = 0; b < OB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) red[(warp * OB * 8 + b * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = acc[b][j];
     if (wk_n > 1) __syncthreads();
     else __syncwarp();
     const int tile_n = wk_n > 1 ? p.wr * 16 : 16, tile0 = wk_n > 1 ? n0 - wr * 16 : n0;
@@ -293,12 +339,30 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_matvec_kernel(const __grid_c
       if (n >= p.n) continue;
       const int w0 = wk_n > 1 ? c >> 4 : warp;
       float y = 0.0f;
-      for (int q = PIECES - 1; q >= 0; --q)
-        for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + w0) * NB * 8 + r * PIECES + q) * 16 + (c & 15)];
-      dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
+      for (int q = JOIN - 1; q >= 0; --q)
+        for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + w0) * OB * 8 + r * JOIN + q) * 16 + (c & 15)];
+      if (p.cuts == 1) dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
+      else p.part[(int64_t(blockIdx.z) * p.m + r) * p.n + n] = y;
     }
-    if (wk_n > 1) __syncthreads();
-    else __syncwarp();
+    if (p.cuts > 1) {       // one pass over the rows: m <= ROWS
+      const int group = int(blockIdx.x) + round * int(gridDim.x);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) s_last = atomicAdd(p.counters + group, 1) == p.cuts - 1;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        const int width = p.wr * 16, at = group * width;
+        for (int e = threadIdx.x; e < rows * width; e += W4_THREADS) {
+          const int r = e / width, n = at + e - r * width;
+          if (n >= p.n) continue;
+          float y = 0.0f;
+          for (int z = 0; z < p.cuts; ++z) y += __ldcg(p.part + (int64_t(z) * p.m + r) * p.n + n);
+          dt_store(p.out, r * p.ld_out + n, p.out_dtype, w4_steps(p, y, r, n));
+        }
+        if (threadIdx.x == 0) p.counters[group] = 0;
+      }
+    }
   }
   cp_async_wait<0>();
 }
