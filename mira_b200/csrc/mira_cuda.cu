@@ -11,6 +11,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/mira_cuda.h"
@@ -24,6 +25,7 @@
 #include "attention_tc.cuh"
 #include "paged_kv.cuh"
 #include "paged_attention.cuh"
+#include "paged_attention_mma.cuh"
 #include "w4_matvec.cuh"
 
 // Set by a kernel that gave up on a bounded wait or met an impossible index; read and cleared by
@@ -2081,15 +2083,12 @@ extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* re
 
 namespace mira {
 
-constexpr int PA_BLOCKS_PER_SM = 2;
-
-// Query heads of one pass over a row: the smallest of 1, 2, 4, 8 that holds the group, else 8.
-static int pa_heads_per_pass(int64_t group) { return group >= 5 ? 8 : group >= 3 ? 4 : int(group); }
+constexpr int PA_MAX_BLOCKS_PER_SM = 4;
 
 static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch * units * 4, 256); }
 
 template <typename T, int DHP, int GP, int VB>
-static int launch_paged_attention(DeviceState* dev, PagedAttnParams& p) {
+static int launch_paged_fma(DeviceState* dev, PagedAttnParams& p) {
   using C = PaCfg<T, DHP, GP, VB>;
   auto kern = paged_attention_kernel<T, DHP, GP, VB>;
   static bool configured[kMaxDevices] = {};
@@ -2100,24 +2099,50 @@ static int launch_paged_attention(DeviceState* dev, PagedAttnParams& p) {
   }
   p.head_blocks = (p.group + GP - 1) / GP;
   p.units = p.kv.kv_heads * p.head_blocks;
-  kern<<<unsigned(dev->sm_count * PA_BLOCKS_PER_SM), PA_THREADS, C::SMEM, dev->stream>>>(p);
+  kern<<<unsigned(dev->sm_count * 2), C::WARPS * 32, C::SMEM, dev->stream>>>(p);
   return after_launch("paged_attention_kernel");
 }
 
 template <typename T, int GP, int VB>
-static int launch_paged_dh(DeviceState* dev, PagedAttnParams& p) {
-  if (p.kv.dh <= 32) return launch_paged_attention<T, 32, GP, VB>(dev, p);
-  if (p.kv.dh <= 64) return launch_paged_attention<T, 64, GP, VB>(dev, p);
-  if (p.kv.dh <= 128) return launch_paged_attention<T, 128, GP, VB>(dev, p);
-  return launch_paged_attention<T, 256, GP, VB>(dev, p);
+static int launch_paged_fma_dh(DeviceState* dev, PagedAttnParams& p) {
+  if (p.kv.dh <= 32) return launch_paged_fma<T, 32, GP, VB>(dev, p);
+  if (p.kv.dh <= 64) return launch_paged_fma<T, 64, GP, VB>(dev, p);
+  if (p.kv.dh <= 128) return launch_paged_fma<T, 128, GP, VB>(dev, p);
+  return launch_paged_fma<T, 256, GP, VB>(dev, p);
 }
 
-template <typename T>
-static int launch_paged_type(DeviceState* dev, PagedAttnParams& p, bool vec) {
-  if (!vec) return launch_paged_attention<T, 256, 1, int(sizeof(T))>(dev, p);
-  if (p.group == 1) return launch_paged_dh<T, 1, 16>(dev, p);
-  if (p.group == 2) return launch_paged_dh<T, 2, 16>(dev, p);
-  return launch_paged_dh<T, 4, 16>(dev, p);
+template <typename T, int DHP, int VB, int QP>
+static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
+  using C = PaMma<T, DHP, VB, QP>;
+  auto kern = paged_attention_mma_kernel<T, DHP, VB, QP>;
+  const int rows = p.group < 16 ? p.group : 16;
+  p.head_blocks = (p.group + 15) / 16;
+  p.units = p.kv.kv_heads * p.head_blocks;
+  // A block of all the SM's warps where the sequences are fewer than the SMs: each is cut into parts
+  // for many SMs, and a part per SM is the least to join.  Else blocks of four warps, which wait for
+  // fewer others at the end of a part.
+  const int warps = int64_t(p.kv.batch) * p.units < dev->sm_count ? C::WARPS : 4;
+  const int smem = C::Q_BYTES + pa_finish_floats(warps, rows, DHP) * 4;
+  static int configured[kMaxDevices] = {};
+  if (configured[dev->device] < smem) {
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                  "cudaFuncSetAttribute(paged attention)");
+    configured[dev->device] = smem;
+  }
+  kern<<<unsigned(dev->sm_count * (C::WARPS / warps)), warps * 32, smem, dev->stream>>>(p);
+  return after_launch("paged_attention_mma_kernel");
+}
+
+template <typename T, int VB, int QP>
+static int launch_paged_mma_dh(DeviceState* dev, PagedAttnParams& p) {
+  if (p.kv.dh <= 64) return launch_paged_mma<T, 64, VB, QP>(dev, p);
+  if (p.kv.dh <= 128) return launch_paged_mma<T, 128, VB, QP>(dev, p);
+  return launch_paged_mma<T, 256, VB, QP>(dev, p);
+}
+
+template <typename T, int VB>
+static int launch_paged_mma_q(DeviceState* dev, PagedAttnParams& p, bool exact) {
+  return exact ? launch_paged_mma_dh<T, VB, 1>(dev, p) : launch_paged_mma_dh<T, VB, 3>(dev, p);
 }
 
 }  // namespace mira
@@ -2127,10 +2152,12 @@ extern "C" int64_t mira_cuda_paged_attention_workspace(int64_t batch, int64_t he
   if (dev == nullptr || batch <= 0 || batch > (1 << 24) || heads <= 0 || kv_heads <= 0 || kv_heads > 65535 ||
       heads % kv_heads != 0 || heads > 65535 || dh <= 0 || dh > MIRA_PAGED_DH_MAX)
     return 0;
-  int64_t dhp = 32;
+  // two triples per block, of at most 16 heads; the element-wise kernel takes every head dimension as 256
+  const int64_t group = heads / kv_heads, rows = group < 16 ? (group < 8 ? round_up(group, 2) : 16) : 16;
+  int dhp = 64;
   while (dhp < dh) dhp *= 2;
-  const int64_t slot = 8 * (256 + 2) * 4;
-  return pa_counters(batch, heads) + int64_t(dev->sm_count) * PA_BLOCKS_PER_SM * 2 * slot;
+  const int64_t triple = pa_triple(int(rows), dhp) > pa_triple(1, 256) ? pa_triple(int(rows), dhp) : pa_triple(1, 256);
+  return pa_counters(batch, heads) + int64_t(dev->sm_count) * PA_MAX_BLOCKS_PER_SM * 2 * triple * 4;
 }
 
 extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
@@ -2174,10 +2201,21 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pa_counters(a->kv.batch, a->heads));
   const bool vec = paged_rows_aligned(a->kv, 16);
   switch (a->kv.dtype) {
-    case MIRA_DT_F32: return launch_paged_type<float>(dev, p, vec);
-    case MIRA_DT_F16: return launch_paged_type<__half>(dev, p, vec);
-    case MIRA_DT_BF16: return launch_paged_type<__nv_bfloat16>(dev, p, vec);
-    default: return launch_paged_type<int8_t>(dev, p, vec);
+    case MIRA_DT_F32:
+      if (!vec) return launch_paged_fma<float, 256, 1, 4>(dev, p);
+      if (p.group == 1) return launch_paged_fma_dh<float, 1, 16>(dev, p);
+      if (p.group == 2) return launch_paged_fma_dh<float, 2, 16>(dev, p);
+      return launch_paged_fma_dh<float, 4, 16>(dev, p);
+    case MIRA_DT_F16:
+      if (!vec) return launch_paged_fma<__half, 256, 1, 2>(dev, p);
+      return launch_paged_mma_q<__half, 16>(dev, p, p.q_dtype == MIRA_DT_F16);
+    case MIRA_DT_BF16:
+      if (!vec) return launch_paged_fma<__nv_bfloat16, 256, 1, 2>(dev, p);
+      return launch_paged_mma_q<__nv_bfloat16, 16>(dev, p, p.q_dtype == MIRA_DT_BF16);
+    default:
+      if (vec) return launch_paged_mma_q<int8_t, 16>(dev, p, p.q_dtype == MIRA_DT_F16);
+      if (paged_rows_aligned(a->kv, 8)) return launch_paged_mma_q<int8_t, 8>(dev, p, p.q_dtype == MIRA_DT_F16);
+      return launch_paged_fma<int8_t, 256, 1, 1>(dev, p);
   }
 }
 

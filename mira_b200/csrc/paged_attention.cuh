@@ -13,8 +13,7 @@
 
 namespace mira {
 
-constexpr int PA_WARPS = 8;
-constexpr int PA_THREADS = PA_WARPS * 32;
+constexpr int PA_MAX_WARPS = 16;
 
 struct PagedAttnParams {
   PagedKv kv;
@@ -61,9 +60,9 @@ __device__ __forceinline__ int pa_block_of(int64_t total, int64_t x, int64_t g) 
   return static_cast<int>(((x + 1) * g - 1) / total);
 }
 
-// Sum of v over the block, and the sum over the lower-numbered threads (one barrier pair).
+// Sum of v over the block, and the sum over the lower-numbered threads.
 __device__ __forceinline__ int64_t pa_scan(int64_t v, int64_t& before, int64_t* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int64_t x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -74,13 +73,79 @@ __device__ __forceinline__ int64_t pa_scan(int64_t v, int64_t& before, int64_t* 
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   int64_t total = 0, base = 0;
-#pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) {
+  for (int w = 0; w < warps; ++w) {
     if (w == warp) base = total;
     total += warp_sums[w];
   }
   before = base + x - v;
   return total;
+}
+
+// A block's share of the line, and the part of a unit at its front.
+struct PaWork {
+  int64_t total, blocks;       // tiles, and blocks that share them
+  int64_t lo, hi;              // this block's
+  int64_t cur;                 // first tile not done yet
+  int b;                       // its sequence
+  int64_t base;                // first tile of that sequence
+  PaSeq seq;
+  // the part: unit and its tiles [us, ue), of which this block does those up to `end`; visible positions
+  // [t0, t1)
+  int unit;
+  int64_t us, ue, end;
+  int t0, t1;
+};
+
+// least: tiles that a block can do at once, below which more blocks would only add joining.
+template <int TILE>
+__device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, PaWork& w) {
+  __shared__ int64_t s_scan[PA_MAX_WARPS];
+  __shared__ int64_t s_found[2];
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.kv.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    int64_t before;
+    total += pa_scan(b < p.kv.batch ? pa_seq<TILE>(p, b).tiles : 0, before, s_scan);
+  }
+  w.total = total * p.units;
+  w.blocks = min(int64_t(gridDim.x), (w.total + least - 1) / least);
+  if (blockIdx.x >= w.blocks) return false;
+  w.lo = w.cur = pa_lo(w.total, blockIdx.x, w.blocks);
+  w.hi = pa_lo(w.total, blockIdx.x + 1, w.blocks);
+  int64_t run = 0;
+  for (int b0 = 0; b0 < p.kv.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    const int64_t mine = b < p.kv.batch ? int64_t(pa_seq<TILE>(p, b).tiles) * p.units : 0;
+    int64_t before;
+    const int64_t sum = pa_scan(mine, before, s_scan);
+    before += run;
+    if (mine > 0 && before <= w.lo && w.lo < before + mine) {
+      s_found[0] = b;
+      s_found[1] = before;
+    }
+    run += sum;
+  }
+  __syncthreads();
+  w.b = int(s_found[0]);
+  w.base = s_found[1];
+  w.seq = pa_seq<TILE>(p, w.b);
+  return true;
+}
+
+template <int TILE>
+__device__ __forceinline__ bool pa_part(const PagedAttnParams& p, PaWork& w) {
+  if (w.cur >= w.hi) return false;
+  while (w.cur >= w.base + int64_t(w.seq.tiles) * p.units) {
+    w.base += int64_t(w.seq.tiles) * p.units;
+    w.seq = pa_seq<TILE>(p, ++w.b);
+  }
+  w.unit = int((w.cur - w.base) / w.seq.tiles);
+  w.us = w.base + int64_t(w.unit) * w.seq.tiles;
+  w.ue = w.us + w.seq.tiles;
+  w.end = min(w.ue, w.hi);
+  w.t0 = int(w.cur - w.us) * TILE;
+  w.t1 = min(w.seq.n, int(w.end - w.us) * TILE);
+  return true;
 }
 
 // ---------------------------------------------------------------- rows of the pages
@@ -102,31 +167,145 @@ __device__ __forceinline__ void pa_unpack(const typename PaVec<VB>::type& raw, f
   for (int i = 0; i < VE; ++i) x[i] = static_cast<float>(e[i]);
 }
 
-// ---------------------------------------------------------------- the end of a unit
-
-// Writes the GP heads of (sequence b, unit) from their joined triples: acc(g, d) is a, m and l in smem.
-template <int GP, class F>
-__device__ __forceinline__ void pa_write(const PagedAttnParams& p, int b, int unit, const float* m, const float* l, F acc) {
-  const int kvh = unit / p.head_blocks, g0 = (unit - kvh * p.head_blocks) * GP;
-  const int live = min(GP, p.group - g0);
-  const int h0 = kvh * p.group + g0;
-  for (int i = threadIdx.x; i < live * p.kv.dh; i += PA_THREADS) {
-    const int g = i / p.kv.dh, d = i - g * p.kv.dh;
-    const float lg = l[g];
-    const float o = lg == 0.0f ? 0.0f : __fdiv_rn(acc(g, d), lg);
-    if (p.out != nullptr) dt_store(p.out, b * p.os[0] + (h0 + g) * p.os[1] + d * p.os[2], p.q_dtype, o);
-    if (p.out_i8 != nullptr)
-      p.out_i8[b * p.is[0] + (h0 + g) * p.is[1] + d * p.is[2]] = static_cast<int8_t>(quant_byte(o, p.q8) & 0xff);
-  }
-  if (p.lse != nullptr && int(threadIdx.x) < live) {
-    const float lg = l[threadIdx.x];
-    p.lse[int64_t(b) * p.heads + h0 + threadIdx.x] =
-        lg == 0.0f ? -INFINITY : fmaf(m[threadIdx.x], 0.693147180559945309f, logf(lg));
-  }
-}
+// ---------------------------------------------------------------- the end of a part
 
 __device__ __forceinline__ float pa_weight(float m, float top) {
   return m == -INFINITY ? 0.0f : exp2f(m - top);   // a part without a finite score weighs nothing
+}
+
+// Floats of a triple of `rows` heads: m [rows], l [rows], a [rows][dhp] from a multiple of four on.
+__host__ __device__ constexpr int pa_head(int rows) { return (2 * rows + 3) & ~3; }
+__host__ __device__ constexpr int pa_triple(int rows, int dhp) { return pa_head(rows) + rows * dhp; }
+// Shared memory of pa_finish in floats: a triple per warp and the joined m and l.
+__host__ __device__ constexpr int pa_finish_floats(int warps, int rows, int dhp) {
+  return warps * pa_triple(rows, dhp) + 2 * rows;
+}
+
+// Writes four values d.. of head g of the unit from its joined triple.
+__device__ __forceinline__ void pa_write4(const PagedAttnParams& p, int b, int h, int d, const float4& a, float l) {
+  const float v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (d + i >= p.kv.dh) break;
+    const float o = l == 0.0f ? 0.0f : __fdiv_rn(v[i], l);
+    if (p.out != nullptr) dt_store(p.out, b * p.os[0] + h * p.os[1] + (d + i) * p.os[2], p.q_dtype, o);
+    if (p.out_i8 != nullptr)
+      p.out_i8[b * p.is[0] + h * p.is[1] + (d + i) * p.is[2]] = static_cast<int8_t>(quant_byte(o, p.q8) & 0xff);
+  }
+}
+
+__device__ __forceinline__ void pa_write_lse(const PagedAttnParams& p, int b, int h, float m, float l) {
+  if (p.lse != nullptr)
+    p.lse[int64_t(b) * p.heads + h] = l == 0.0f ? -INFINITY : fmaf(m, 0.693147180559945309f, logf(l));
+}
+
+__device__ __forceinline__ void pa_add4(float4& a, const float4& x, float w) {
+  a.x = fmaf(x.x, w, a.x);
+  a.y = fmaf(x.y, w, a.y);
+  a.z = fmaf(x.z, w, a.z);
+  a.w = fmaf(x.w, w, a.w);
+}
+
+// Joins the warps' triples of this part (sm: one triple per warp, `rows` of them used) and either
+// writes the result, when the block had the whole unit, or leaves the joined triple in the block's
+// slot; the last block of the unit to do so joins them all.  Every thread of the block calls it.
+// h0: first of the unit's `live` heads.
+template <int DHP>
+__device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork& w, float* sm, int rows, int h0, int live) {
+  __shared__ int s_last;
+  const int warps = blockDim.x >> 5, triple = pa_triple(rows, DHP);
+  float* j_m = sm + warps * triple;
+  float* j_l = j_m + rows;
+  __syncthreads();
+  if (int(threadIdx.x) < live) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < warps; ++i) top = fmaxf(top, sm[i * triple + threadIdx.x]);
+    for (int i = 0; i < warps; ++i) {
+      float* m = sm + i * triple + threadIdx.x;
+      const float wt = pa_weight(*m, top);
+      sum += m[rows] * wt;
+      *m = wt;      // from here on the warp's weight
+    }
+    j_m[threadIdx.x] = top;
+    j_l[threadIdx.x] = sum;
+  }
+  __syncthreads();
+  const int first = pa_block_of(w.total, w.us, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
+  auto slot_of = [&](int64_t c) { return p.part + (c * 2 + (pa_lo(w.total, c, w.blocks) >= w.us ? 0 : 1)) * triple; };
+  float* mine = slot_of(blockIdx.x);
+  for (int e = threadIdx.x; e < live * (DHP / 4); e += blockDim.x) {
+    const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < warps; ++i)
+      pa_add4(a, *reinterpret_cast<const float4*>(sm + i * triple + pa_head(rows) + g * DHP + d), sm[i * triple + g]);
+    if (first == last) pa_write4(p, w.b, h0 + g, d, a, j_l[g]);
+    else *reinterpret_cast<float4*>(mine + pa_head(rows) + g * DHP + d) = a;
+  }
+  if (first == last) {
+    if (int(threadIdx.x) < live) pa_write_lse(p, w.b, h0 + threadIdx.x, j_m[threadIdx.x], j_l[threadIdx.x]);
+    __syncthreads();
+    return;
+  }
+  if (int(threadIdx.x) < live) {
+    mine[threadIdx.x] = j_m[threadIdx.x];
+    mine[rows + threadIdx.x] = j_l[threadIdx.x];
+  }
+  __threadfence();
+  __syncthreads();
+  int* counter = p.counters + int64_t(w.b) * p.units + w.unit;
+  if (threadIdx.x == 0) s_last = atomicAdd(counter, 1) == last - first;
+  __syncthreads();
+  if (s_last) {
+    __threadfence();
+    // all but the first part start at their block's first tile, so they are in slot 0
+    const float* from = slot_of(first);
+    const float* next = p.part + (int64_t(first) + 1) * 2 * triple;
+    const int n = last - first + 1;
+    auto part = [&](int i) { return i == 0 ? from : next + int64_t(i - 1) * 2 * triple; };
+    float* wts = sm;                  // [n][live] weights, if they fit where the warps' triples were
+    const bool fits = n * live <= warps * triple;
+    // a warp per head: the largest m, then the sum
+    for (int g = threadIdx.x >> 5; g < live; g += warps) {
+      const int lane = threadIdx.x & 31;
+      float top = -INFINITY, sum = 0.0f;
+      for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part(i) + g));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int i = lane; i < n; i += 32) {
+        const float wt = pa_weight(__ldcg(part(i) + g), top);
+        if (fits) wts[i * live + g] = wt;
+        sum += __ldcg(part(i) + rows + g) * wt;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) {
+        j_m[g] = top;
+        j_l[g] = sum;
+        pa_write_lse(p, w.b, h0 + g, top, sum);
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < live * (DHP / 4); e += blockDim.x) {
+      const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float top = j_m[g];
+      int i = 0;
+      for (; i + 8 <= n; i += 8) {      // eight loads in flight
+        float4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = __ldcg(reinterpret_cast<const float4*>(part(i + u) + pa_head(rows) + g * DHP + d));
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          pa_add4(a, x[u], fits ? wts[(i + u) * live + g] : pa_weight(__ldcg(part(i + u) + g), top));
+      }
+      for (; i < n; ++i)
+        pa_add4(a, __ldcg(reinterpret_cast<const float4*>(part(i) + pa_head(rows) + g * DHP + d)),
+                fits ? wts[i * live + g] : pa_weight(__ldcg(part(i) + g), top));
+      pa_write4(p, w.b, h0 + g, d, a, j_l[g]);
+    }
+    if (threadIdx.x == 0) *counter = 0;
+  }
+  __syncthreads();     // the shared triples are free again
 }
 
 // ---------------------------------------------------------------- the kernel on FMA units
@@ -135,6 +314,7 @@ __device__ __forceinline__ float pa_weight(float m, float top) {
 // share a pass over the rows; VB: bytes per access (16, or less where rows are not 16-byte aligned).
 template <typename T, int DHP, int GP, int VB>
 struct PaCfg {
+  static constexpr int WARPS = 8;
   static constexpr int VE = VB / int(sizeof(T));            // elements of an access
   static constexpr int LPR = DHP / VE < 32 ? DHP / VE : 32; // lanes of a row
   static constexpr int NV = DHP / (VE * LPR);               // accesses of a lane per row
@@ -142,69 +322,23 @@ struct PaCfg {
   static constexpr int TPS = 32 / LPR;                      // rows of a warp access
   static constexpr int U = NV > 1 ? 2 : 4;                  // rows in flight per lane
   static constexpr int ROWS = TPS * U;                      // rows of a warp step
-  static constexpr int TILE = PA_WARPS * ROWS;
-  static constexpr int SMEM = (PA_WARPS * GP * (DHP + 2) + 2 * GP) * 4;
-  static constexpr int SLOT = GP * (DHP + 2);               // floats of a partial triple
+  static constexpr int TILE = WARPS * ROWS;
+  static constexpr int SMEM = pa_finish_floats(WARPS, GP, DHP) * 4;
 };
 
 template <typename T, int DHP, int GP, int VB>
-__global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
+    paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PaCfg<T, DHP, GP, VB>;
   using V = typename PaVec<VB>::type;
   constexpr bool I8 = sizeof(T) == 1;
-  extern __shared__ __align__(16) float sm[];
-  float* s_acc = sm;                                  // [warp][GP][DHP]
-  float* s_m = s_acc + PA_WARPS * GP * DHP;           // [warp][GP]
-  float* s_l = s_m + PA_WARPS * GP;
-  float* j_m = s_l + PA_WARPS * GP;                   // [GP] the block's
-  float* j_l = j_m + GP;
-  __shared__ int64_t s_scan[PA_WARPS];
-  __shared__ int64_t s_found[2];
-  __shared__ int s_last;
+  extern __shared__ __align__(16) float pa_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % C::LPR, slot_of_lane = lane / C::LPR;
-
-  // this block's tiles
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.kv.batch; b0 += PA_THREADS) {
-    const int b = b0 + threadIdx.x;
-    int64_t before;
-    total += pa_scan(b < p.kv.batch ? pa_seq<C::TILE>(p, b).tiles : 0, before, s_scan);
-  }
-  total *= p.units;
-  const int64_t g = min(int64_t(gridDim.x), total);
-  if (blockIdx.x >= g) return;
-  const int64_t lo = pa_lo(total, blockIdx.x, g), hi = pa_lo(total, blockIdx.x + 1, g);
-  {
-    int64_t run = 0;
-    for (int b0 = 0; b0 < p.kv.batch; b0 += PA_THREADS) {
-      const int b = b0 + threadIdx.x;
-      const int64_t mine = b < p.kv.batch ? int64_t(pa_seq<C::TILE>(p, b).tiles) * p.units : 0;
-      int64_t before;
-      const int64_t sum = pa_scan(mine, before, s_scan);
-      before += run;
-      if (mine > 0 && before <= lo && lo < before + mine) {
-        s_found[0] = b;
-        s_found[1] = before;
-      }
-      run += sum;
-    }
-    __syncthreads();
-  }
-  int b = int(s_found[0]);
-  int64_t base = s_found[1];       // first tile of sequence b
-  PaSeq seq = pa_seq<C::TILE>(p, b);
-
-  for (int64_t cur = lo; cur < hi;) {
-    while (cur >= base + int64_t(seq.tiles) * p.units) {
-      base += int64_t(seq.tiles) * p.units;
-      seq = pa_seq<C::TILE>(p, ++b);
-    }
-    const int unit = int((cur - base) / seq.tiles);
-    const int64_t us = base + int64_t(unit) * seq.tiles, ue = us + seq.tiles;   // the unit's tiles
-    const int64_t end = min(ue, hi);
-    const int t0 = int(cur - us) * C::TILE, t1 = min(seq.n, int(end - us) * C::TILE);
-    const int kvh = unit / p.head_blocks, g0 = (unit - kvh * p.head_blocks) * GP;
+  PaWork w;
+  if (!pa_begin<C::TILE>(p, 1, w)) return;
+  while (pa_part<C::TILE>(p, w)) {
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
 
     // queries of the unit, scaled
     float q[GP][C::EPL];
@@ -216,7 +350,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
         for (int e = 0; e < C::VE; ++e) {
           const int d = (sub + j * C::LPR) * C::VE + e;
           q[gi][j * C::VE + e] = (g0 + gi < p.group && d < p.kv.dh)
-              ? dt_load(p.q, b * p.qs[0] + (kvh * p.group + g0 + gi) * p.qs[1] + d * p.qs[2], p.q_dtype) * p.scale_log2
+              ? dt_load(p.q, w.b * p.qs[0] + (kvh * p.group + g0 + gi) * p.qs[1] + d * p.qs[2], p.q_dtype) * p.scale_log2
               : 0.0f;
         }
     float acc[GP][C::EPL], m[GP], l[GP];
@@ -227,21 +361,31 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
 #pragma unroll
       for (int e = 0; e < C::EPL; ++e) acc[gi][e] = 0.0f;
     }
-    const int32_t* trow = p.kv.table + b * p.kv.table_ld;
+    const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
     const T* kb = static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1];
     const T* vb = static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1];
 
-    for (int w0 = t0 + warp * C::ROWS; w0 < t1; w0 += C::TILE) {
-      V kr[C::U][C::NV], vr[C::U][C::NV];
-      float ksc[C::U], vsc[C::U];
-      bool ok[C::U];
+    // where the lane's rows of a step are; looked up a step ahead of their loads
+    int page[C::U], slot[C::U];
+    bool ok[C::U];
+    auto look = [&](int w0) {
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
         const int i = w0 + u * C::TPS + slot_of_lane;
-        int page = 0, slot = 0;
-        ok[u] = i < t1 && paged_slot(p.kv, trow, i + (i < seq.sinks ? 0 : seq.skip), page, slot);
-        const T* kp = kb + page * p.kv.kst[0] + slot * p.kv.kst[2];
-        const T* vp = vb + page * p.kv.vst[0] + slot * p.kv.vst[2];
+        page[u] = slot[u] = 0;
+        ok[u] = i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page[u], slot[u]);
+      }
+    };
+    look(w.t0 + warp * C::ROWS);
+    for (int w0 = w.t0 + warp * C::ROWS; w0 < w.t1; w0 += C::TILE) {
+      V kr[C::U][C::NV], vr[C::U][C::NV];
+      float ksc[C::U], vsc[C::U];
+      bool now[C::U];
+#pragma unroll
+      for (int u = 0; u < C::U; ++u) {
+        now[u] = ok[u];
+        const T* kp = kb + page[u] * p.kv.kst[0] + slot[u] * p.kv.kst[2];
+        const T* vp = vb + page[u] * p.kv.vst[0] + slot[u] * p.kv.vst[2];
 #pragma unroll
         for (int j = 0; j < C::NV; ++j) {
           const int d = (sub + j * C::LPR) * C::VE;
@@ -250,10 +394,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
           vr[u][j] = in ? __ldg(reinterpret_cast<const V*>(vp + d)) : V{};
         }
         if (I8) {
-          ksc[u] = ok[u] ? __ldg(p.kv.ks + page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2]) : 0.0f;
-          vsc[u] = ok[u] ? __ldg(p.kv.vs + page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2]) : 0.0f;
+          ksc[u] = ok[u] ? __ldg(p.kv.ks + page[u] * p.kv.kss[0] + kvh * p.kv.kss[1] + slot[u] * p.kv.kss[2]) : 0.0f;
+          vsc[u] = ok[u] ? __ldg(p.kv.vs + page[u] * p.kv.vss[0] + kvh * p.kv.vss[1] + slot[u] * p.kv.vss[2]) : 0.0f;
         }
       }
+      look(w0 + C::TILE);
       float s[C::U][GP];
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
@@ -273,7 +418,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
 #pragma unroll
           for (int o = 1; o < C::LPR; o <<= 1) s[u][gi] += __shfl_xor_sync(0xffffffffu, s[u][gi], o);
           if (I8) s[u][gi] *= ksc[u];
-          if (!ok[u]) s[u][gi] = -INFINITY;
+          if (!now[u]) s[u][gi] = -INFINITY;
         }
       }
 #pragma unroll
@@ -308,15 +453,16 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
         }
     }
 
-    // join the warp's lane groups, then the warps
+    // join the warp's lane groups
+    float* mine = pa_smem + warp * pa_triple(GP, DHP);
 #pragma unroll
     for (int gi = 0; gi < GP; ++gi) {
 #pragma unroll
       for (int o = C::LPR; o < 32; o <<= 1) {
-        const float mo = __shfl_xor_sync(0xffffffffu, m[gi], o), lo_ = __shfl_xor_sync(0xffffffffu, l[gi], o);
+        const float mo = __shfl_xor_sync(0xffffffffu, m[gi], o), lo = __shfl_xor_sync(0xffffffffu, l[gi], o);
         const float top = fmaxf(m[gi], mo);
         const float wa = pa_weight(m[gi], top), wb = pa_weight(mo, top);
-        l[gi] = l[gi] * wa + lo_ * wb;
+        l[gi] = l[gi] * wa + lo * wb;
         m[gi] = top;
 #pragma unroll
         for (int e = 0; e < C::EPL; ++e)
@@ -326,76 +472,15 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < C::NV; ++j)
 #pragma unroll
-          for (int e = 0; e < C::VE; ++e)
-            s_acc[(warp * GP + gi) * DHP + (sub + j * C::LPR) * C::VE + e] = acc[gi][j * C::VE + e];
+          for (int e = 0; e < C::VE; ++e) mine[pa_head(GP) + gi * DHP + (sub + j * C::LPR) * C::VE + e] = acc[gi][j * C::VE + e];
       }
       if (lane == 0) {
-        s_m[warp * GP + gi] = m[gi];
-        s_l[warp * GP + gi] = l[gi];
+        mine[gi] = m[gi];
+        mine[GP + gi] = l[gi];
       }
     }
-    __syncthreads();
-    if (threadIdx.x < GP) {
-      float top = -INFINITY, sum = 0.0f;
-      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * GP + threadIdx.x]);
-      for (int w = 0; w < PA_WARPS; ++w) {
-        const float wt = pa_weight(s_m[w * GP + threadIdx.x], top);
-        sum += s_l[w * GP + threadIdx.x] * wt;
-        s_m[w * GP + threadIdx.x] = wt;      // from here on the warp's weight
-      }
-      j_m[threadIdx.x] = top;
-      j_l[threadIdx.x] = sum;
-    }
-    __syncthreads();
-    auto joined = [&](int gi, int d) {
-      float a = 0.0f;
-#pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) a = fmaf(s_acc[(w * GP + gi) * DHP + d], s_m[w * GP + gi], a);
-      return a;
-    };
-    const int first = pa_block_of(total, us, g), last = pa_block_of(total, ue - 1, g);
-    if (first == last) {
-      pa_write<GP>(p, b, unit, j_m, j_l, joined);
-    } else {
-      // a part of the unit: leave the triple in this block's slot; the last block to arrive joins all
-      float* mine = p.part + (int64_t(blockIdx.x) * 2 + (lo >= us ? 0 : 1)) * C::SLOT;
-      for (int i = threadIdx.x; i < GP * DHP; i += PA_THREADS) mine[2 * GP + i] = joined(i / DHP, i % DHP);
-      if (threadIdx.x < GP) {
-        mine[threadIdx.x] = j_m[threadIdx.x];
-        mine[GP + threadIdx.x] = j_l[threadIdx.x];
-      }
-      __threadfence();
-      __syncthreads();
-      int* counter = p.counters + int64_t(b) * p.units + unit;
-      if (threadIdx.x == 0) s_last = atomicAdd(counter, 1) == last - first;
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        auto slot_of = [&](int c) {
-          return p.part + (int64_t(c) * 2 + (pa_lo(total, c, g) >= us ? 0 : 1)) * C::SLOT;
-        };
-        if (threadIdx.x < GP) {
-          float top = -INFINITY, sum = 0.0f;
-          for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(slot_of(c) + threadIdx.x));
-          for (int c = first; c <= last; ++c)
-            sum += __ldcg(slot_of(c) + GP + threadIdx.x) * pa_weight(__ldcg(slot_of(c) + threadIdx.x), top);
-          j_m[threadIdx.x] = top;
-          j_l[threadIdx.x] = sum;
-        }
-        __syncthreads();
-        pa_write<GP>(p, b, unit, j_m, j_l, [&](int gi, int d) {
-          float a = 0.0f;
-          for (int c = first; c <= last; ++c) {
-            const float* from = slot_of(c);
-            a = fmaf(__ldcg(from + 2 * GP + gi * DHP + d), pa_weight(__ldcg(from + gi), j_m[gi]), a);
-          }
-          return a;
-        });
-        if (threadIdx.x == 0) *counter = 0;
-      }
-    }
-    cur = end;
-    __syncthreads();     // the shared triples are free again
+    pa_finish<DHP>(p, w, pa_smem, GP, kvh * p.group + g0, min(GP, p.group - g0));
+    w.cur = w.end;
   }
 }
 

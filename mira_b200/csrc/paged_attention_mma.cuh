@@ -1,0 +1,398 @@
+// Paged attention of one token per sequence on the tensor path, for 16-bit and 8-bit pages.
+//
+// Bound: the visible keys and values are read once; an SM's share of the memory bandwidth is about 23
+// bytes a clock.  The group's heads are the 16 rows of the products, so a key costs the same few
+// instructions for one head as for sixteen, and what remains is unpacking, addresses and the softmax.
+//
+// Everything stays in registers: the sums over k of a product do not care in which order k comes, so a
+// lane's 16-byte piece of a row, as it arrives from memory, is its share of a fragment.
+//   S = Q K^T: lane (g, t) holds token g's elements VE t .. VE t + VE - 1 of each run of 4 VE: four of
+//     them are the right operand of one 16x8x16 product; Q is laid out to match, once per unit.
+//   O += P V: lane (g, t) holds elements VE g .. of each run of 8 VE of the tokens 2t, 2t + 1, 2t + 8 and
+//     2t + 9; pairs of tokens of one element, one byte permutation each, are the right operand, column g
+//     of tile i being element VE g + i; P's accumulators are already the left operand's layout.
+// Exactness: q enters as one value of the pages' type where it has that type, else as three whose sum
+// it is; 8-bit codes become exact f16 values.  p is f32 and enters as PP values that agree with it to 16
+// bits or more (see PaMma), the row's sum l is of the f32 values.
+#pragma once
+#include <cstdint>
+
+#include "mma_sm80.cuh"
+#include "paged_attention.cuh"
+
+namespace mira {
+
+// T: the pages' element; DHP: head dimension rounded up to 64, 128 or 256; VB: bytes per access of a
+// key row; QP: values per query element, 1 or 3.
+template <typename T, int DHP, int VB, int QP>
+struct PaMma {
+  static constexpr bool I8 = sizeof(T) == 1;
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;      // else the products are f16
+  static constexpr int KE = VB / int(sizeof(T));                           // elements of a key access
+  static constexpr int KL = DHP / (4 * KE);                                // key accesses of a lane per token
+  static constexpr int KS = DHP / 16;                                      // products along the head dimension
+  static constexpr int VBV = VB < DHP * int(sizeof(T)) / 8 ? VB : DHP * int(sizeof(T)) / 8;
+  static constexpr int VE = VBV / int(sizeof(T));
+  static constexpr int VL = DHP / (8 * VE);                                // value accesses per token
+  static constexpr int NT = DHP / 8;                                       // tiles of O
+  static constexpr int TT = (DHP * int(sizeof(T)) <= 128) ? 2 : 1;         // runs of 16 tokens per step
+  static constexpr int TILE = 16 * TT;                                     // tokens of a warp step
+  // p: bf16 values have 8 bits, f16 ones 11.  16-bit results: 16 and 22 bits; f32 results (QP == 3): 24
+  // and 22, whose error of 2^-22 of the largest weight is that of an f32 sum of a few terms.  In f16,
+  // p is carried times 2^8: the smallest f16 is then 2^-32 of the largest weight.
+  static constexpr int PP = BF16 && QP == 3 ? 3 : 2;
+  static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
+  static constexpr int WARPS = DHP <= 64 ? 16 : DHP <= 128 ? 12 : 8;       // of an SM, by registers
+  static constexpr int Q_BYTES = QP * KS * 32 * 16;
+};
+
+// x = a + b (+ c) in 16-bit values, pairs packed.
+template <bool BF16, int N>
+__device__ __forceinline__ void pa_split2(float x, float y, uint32_t (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      out[i] = b2_bits(h);
+      if (i + 1 < N) {
+        x -= __uint_as_float(out[i] << 16);
+        y -= __uint_as_float(out[i] & 0xffff0000u);
+      }
+    } else {
+      const __half2 h = __floats2half2_rn(x, y);
+      out[i] = h2_bits(h);
+      if (i + 1 < N) {
+        const float2 f = __half22float2(h);
+        x -= f.x;
+        y -= f.y;
+      }
+    }
+  }
+}
+
+// Four 8-bit codes (as bytes + 128) -> two registers of f16 pairs (0, 1), (2, 3): the byte becomes the
+// low mantissa bits of 1024, 1152 is subtracted exactly.
+__device__ __forceinline__ uint32_t pa_codes(uint32_t biased, uint32_t sel) {
+  return h2_bits(__hsub2(bits_h2(__byte_perm(biased, 0x64646464u, sel)), bits_h2(0x64806480u)));
+}
+
+template <int WORDS> struct PaWords { uint32_t w[WORDS]; };
+
+template <int BYTES>
+__device__ __forceinline__ PaWords<BYTES / 4> pa_load(const void* p, bool ok) {
+  PaWords<BYTES / 4> r;
+  if (BYTES == 16) {
+    const uint4 v = ok ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    r.w[0] = v.x; r.w[1] = v.y; r.w[2 % (BYTES / 4)] = v.z; r.w[3 % (BYTES / 4)] = v.w;
+  } else {
+    const uint2 v = ok ? __ldg(static_cast<const uint2*>(p)) : make_uint2(0, 0);
+    r.w[0] = v.x; r.w[1] = v.y;
+  }
+  return r;
+}
+
+template <typename T, int DHP, int VB, int QP>
+__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
+    paged_attention_mma_kernel(const __grid_constant__ PagedAttnParams p) {
+  using C = PaMma<T, DHP, VB, QP>;
+  extern __shared__ __align__(16) float pa_smem[];
+  __shared__ float s_unit[16];        // per head: what turns a product into a scaled score
+  uint4* s_q = reinterpret_cast<uint4*>(pa_smem);                  // [piece][product][lane]
+  float* s_join = pa_smem + C::Q_BYTES / 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
+  const int rows = min(16, p.group);
+  PaWork w;
+  if (!pa_begin<C::TILE>(p, warps, w)) return;
+  while (pa_part<C::TILE>(p, w)) {
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * 16;
+    const int h0 = kvh * p.group + g0, live = min(16, p.group - g0);
+    const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
+    const T* kb = static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE;
+    const T* vb = static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE;
+
+    // lane i looks up token i of a step; the step's rows are shared by shuffles
+    int page = 0, slot = 0;
+    bool ok = false;
+    auto look = [&](int at) {
+      const int i = at + lane;
+      page = slot = 0;
+      ok = lane < C::TILE && i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page, slot);
+    };
+    PaWords<VB / 4> kr[C::TT][2][C::KL];
+    float kscale[C::TT][4];
+    uint32_t live_k = 0;      // tokens of the step whose keys kr holds
+    auto load_k = [&]() {
+      live_k = __ballot_sync(0xffffffffu, ok);
+      float mine = 0.0f;
+      if (C::I8 && ok) mine = __ldg(p.kv.ks + page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2]);
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int i = r * 16 + n * 8 + g;
+          const int pg = __shfl_sync(0xffffffffu, page, i), sl = __shfl_sync(0xffffffffu, slot, i);
+          const T* row = kb + pg * p.kv.kst[0] + sl * p.kv.kst[2];
+          const bool in = live_k >> i & 1;
+#pragma unroll
+          for (int j = 0; j < C::KL; ++j) {
+            const bool inside = j * 4 * C::KE + t * C::KE < p.kv.dh;
+            kr[r][n][j] = pa_load<VB>(row + j * 4 * C::KE, in && inside);
+          }
+          if (C::I8) {
+            kscale[r][2 * n] = __shfl_sync(0xffffffffu, mine, r * 16 + n * 8 + 2 * t);
+            kscale[r][2 * n + 1] = __shfl_sync(0xffffffffu, mine, r * 16 + n * 8 + 2 * t + 1);
+          }
+        }
+    };
+    const int step = warps * C::TILE;
+    int at = w.t0 + warp * C::TILE;
+    look(at);
+    load_k();        // before the queries: their latencies overlap
+
+    // queries of the unit in fragment order; a thread per (product, lane).  f16 values of a query that
+    // is not f16 itself are taken after a power of two has brought its largest element to [128, 256).
+    for (int h = warp; h < 16; h += warps) {
+      float unit = p.scale_log2;
+      if (QP == 3 && !C::BF16) {
+        float top = 0.0f;
+        if (h < live)
+          for (int d = lane; d < p.kv.dh; d += 32)
+            top = fmaxf(top, fabsf(dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + d * p.qs[2], p.q_dtype)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e = int(__float_as_uint(top) >> 23);      // 2^(e - 127) <= top
+        const int up = e == 0 || e == 255 ? 0 : min(max(134 - e, -126), 127);
+        if (lane == 0) s_unit[h] = __int_as_float((127 + up) << 23);
+      } else if (lane == 0) {
+        s_unit[h] = unit;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < C::KS * 32; i += blockDim.x) {
+      const int ks = i >> 5, l = i & 31, lg = l >> 2, lt = l & 3;
+      const int d = (ks / (C::KE / 4)) * 4 * C::KE + lt * C::KE + (ks % (C::KE / 4)) * 4;
+      float x[2][4];       // head g and g + 8, elements d .. d + 3
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = lg + 8 * hh;
+          float v = h < live && d + e < p.kv.dh
+              ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + (d + e) * p.qs[2], p.q_dtype) : 0.0f;
+          if (QP == 3 && !C::BF16) v *= s_unit[h];
+          x[hh][e] = v;
+        }
+      uint32_t f[4][QP];
+      if (C::BF16 && QP == 3) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[3], b[3];
+          split3_bf16(x[j & 1][(j >> 1) * 2], a[0], a[1], a[2]);
+          split3_bf16(x[j & 1][(j >> 1) * 2 + 1], b[0], b[1], b[2]);
+#pragma unroll
+          for (int q = 0; q < QP; ++q) f[j][q] = __byte_perm(a[q], b[q], 0x7632);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pa_split2<C::BF16, QP>(x[j & 1][(j >> 1) * 2], x[j & 1][(j >> 1) * 2 + 1], f[j]);
+      }
+#pragma unroll
+      for (int q = 0; q < QP; ++q) s_q[(q * C::KS + ks) * 32 + l] = make_uint4(f[0][q], f[1][q], f[2][q], f[3][q]);
+    }
+    __syncthreads();
+    float unit0 = s_unit[g], unit1 = s_unit[g + 8];
+    if (QP == 3 && !C::BF16) {      // powers of two: the division is exact
+      unit0 = p.scale_log2 / unit0;
+      unit1 = p.scale_log2 / unit1;
+    }
+
+    float acc[C::NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    uint32_t v_exp = 1;       // 8-bit pages: exponent of the largest value scale so far, which acc is divided by
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+
+    for (; at < w.t1; at += step) {
+      // values of this step
+      PaWords<C::VBV / 4> vr[C::TT][4][C::VL];
+      float vscale = 0.0f;
+      const uint32_t now = live_k;
+      if (C::I8 && ok) vscale = __ldg(p.kv.vs + page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2]);
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
+          const int pg = __shfl_sync(0xffffffffu, page, i), sl = __shfl_sync(0xffffffffu, slot, i);
+          const T* row = vb + pg * p.kv.vst[0] + sl * p.kv.vst[2];
+          const bool in = now >> i & 1;
+#pragma unroll
+          for (int j = 0; j < C::VL; ++j) {
+            const bool inside = j * 8 * C::VE + g * C::VE < p.kv.dh;
+            vr[r][n][j] = pa_load<C::VBV>(row + j * 8 * C::VE, in && inside);
+          }
+        }
+      look(at + step);
+
+      // scores
+      float s[C::TT][2][4];
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][n][i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < C::KL; ++j)
+#pragma unroll
+        for (int e = 0; e < C::KE / 4; ++e) {
+          uint32_t b[C::TT][2][2];
+#pragma unroll
+          for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              if (C::I8) {
+                const uint32_t x = kr[r][n][j].w[e] ^ 0x80808080u;
+                b[r][n][0] = pa_codes(x, 0x4140);
+                b[r][n][1] = pa_codes(x, 0x4342);
+              } else {
+                b[r][n][0] = kr[r][n][j].w[(2 * e) % (VB / 4)];
+                b[r][n][1] = kr[r][n][j].w[(2 * e + 1) % (VB / 4)];
+              }
+            }
+#pragma unroll
+          for (int q = QP - 1; q >= 0; --q) {
+            const uint4 a = s_q[(q * C::KS + j * (C::KE / 4) + e) * 32 + lane];
+#pragma unroll
+            for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) mma_16816<C::BF16>(s[r][n], a.x, a.y, a.z, a.w, b[r][n][0], b[r][n][1]);
+          }
+        }
+      float top0 = m0, top1 = m1;
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const bool in = now >> (r * 16 + n * 8 + 2 * t + i) & 1;
+            const float ks = C::I8 ? kscale[r][2 * n + i] : 1.0f;
+            s[r][n][i] = in ? s[r][n][i] * (C::I8 ? unit0 * ks : unit0) : -INFINITY;
+            s[r][n][2 + i] = in ? s[r][n][2 + i] * (C::I8 ? unit1 * ks : unit1) : -INFINITY;
+            top0 = fmaxf(top0, s[r][n][i]);
+            top1 = fmaxf(top1, s[r][n][2 + i]);
+          }
+      load_k();          // the next step's keys, while this one's softmax and values go on
+
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+      }
+      float grow = 1.0f;
+      if (C::I8) {
+        const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vscale))) >> 23, v_exp), 253u);
+        grow = __int_as_float((127 - min(int(e - v_exp), 126)) << 23);
+        v_exp = e;
+        vscale *= __int_as_float((254 - e) << 23);
+      }
+      const float safe0 = top0 == -INFINITY ? 0.0f : top0, safe1 = top1 == -INFINITY ? 0.0f : top1;
+      if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1 || grow != 1.0f)) {
+        const float f0 = exp2f(m0 - safe0), f1 = exp2f(m1 - safe1);
+        m0 = top0;
+        m1 = top1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) {
+          acc[n][0] *= f0 * grow;
+          acc[n][1] *= f0 * grow;
+          acc[n][2] *= f1 * grow;
+          acc[n][3] *= f1 * grow;
+        }
+      }
+      const float z0 = safe0 - C::SHIFT, z1 = safe1 - C::SHIFT;
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r) {
+        uint32_t a[4][C::PP];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float x0 = exp2f(s[r][n][0] - z0), x1 = exp2f(s[r][n][1] - z0);
+          float y0 = exp2f(s[r][n][2] - z1), y1 = exp2f(s[r][n][3] - z1);
+          l0 += x0 + x1;
+          l1 += y0 + y1;
+          if (C::I8) {
+            const float u0 = __shfl_sync(0xffffffffu, vscale, r * 16 + n * 8 + 2 * t);
+            const float u1 = __shfl_sync(0xffffffffu, vscale, r * 16 + n * 8 + 2 * t + 1);
+            x0 *= u0;
+            x1 *= u1;
+            y0 *= u0;
+            y1 *= u1;
+          }
+          pa_split2<C::BF16, C::PP>(x0, x1, a[2 * n]);
+          pa_split2<C::BF16, C::PP>(y0, y1, a[2 * n + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < C::VL; ++j)
+#pragma unroll
+          for (int e = 0; e < C::VBV / 4; ++e) {
+            constexpr int PER = 4 / int(sizeof(T));      // elements of a word
+            uint32_t b[PER][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t x = vr[r][2 * h][j].w[e], y = vr[r][2 * h + 1][j].w[e];
+              if (C::I8) {
+                const uint32_t bx = x ^ 0x80808080u, by = y ^ 0x80808080u;
+                const uint32_t low = __byte_perm(bx, by, 0x5140), high = __byte_perm(bx, by, 0x7362);
+                b[0][h] = pa_codes(low, 0x4140);
+                b[1][h] = pa_codes(low, 0x4342);
+                b[2 % PER][h] = pa_codes(high, 0x4140);
+                b[3 % PER][h] = pa_codes(high, 0x4342);
+              } else {
+                b[0][h] = __byte_perm(x, y, 0x5410);
+                b[1][h] = __byte_perm(x, y, 0x7632);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+#pragma unroll
+              for (int q = C::PP - 1; q >= 0; --q)
+                mma_16816<C::BF16>(acc[j * C::VE + e * PER + i], a[0][q], a[1][q], a[2][q], a[3][q], b[i][0], b[i][1]);
+          }
+      }
+    }
+
+    // the warp's triple
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    const float back = C::BF16 ? 1.0f : 0x1p-8f;
+    const float back_v = C::I8 ? back * __int_as_float(v_exp << 23) : back;
+    float* mine = s_join + warp * pa_triple(rows, DHP);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int h = g + 8 * hh;
+      if (h >= rows) continue;
+      if (t == 0) {
+        mine[h] = hh ? m1 : m0;
+        mine[rows + h] = (hh ? l1 : l0) * back;
+      }
+      float* to = mine + pa_head(rows) + h * DHP;
+#pragma unroll
+      for (int j = 0; j < C::VL; ++j)
+#pragma unroll
+        for (int i = 0; i < C::VE; ++i) {
+          to[(j * 8 + 2 * t) * C::VE + i] = acc[j * C::VE + i][2 * hh] * back_v;
+          to[(j * 8 + 2 * t + 1) * C::VE + i] = acc[j * C::VE + i][2 * hh + 1] * back_v;
+        }
+    }
+    pa_finish<DHP>(p, w, s_join, rows, h0, live);
+    w.cur = w.end;
+  }
+}
+
+}  // namespace mira
