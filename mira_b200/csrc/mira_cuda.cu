@@ -2087,50 +2087,71 @@ constexpr int PA_MAX_BLOCKS_PER_SM = 4;
 
 static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch * units * 4, 256); }
 
-template <typename T, int DHP, int GP, int VB>
-static int launch_paged_fma(DeviceState* dev, PagedAttnParams& p) {
-  using C = PaCfg<T, DHP, GP, VB>;
-  auto kern = paged_attention_kernel<T, DHP, GP, VB>;
-  static bool configured[kMaxDevices] = {};
-  if (!configured[dev->device]) {
-    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
-                  "cudaFuncSetAttribute(paged attention)");
-    configured[dev->device] = true;
-  }
-  p.head_blocks = (p.group + GP - 1) / GP;
+// Rows of any alignment.
+template <typename T>
+static int launch_paged_any(DeviceState* dev, PagedAttnParams& p) {
+  using C = PaCfg<T, 256, 1, int(sizeof(T))>;
+  auto kern = paged_attention_any_kernel<T, 256, 1, int(sizeof(T))>;
+  p.head_blocks = p.group;
   p.units = p.kv.kv_heads * p.head_blocks;
   kern<<<unsigned(dev->sm_count * 2), C::WARPS * 32, C::SMEM, dev->stream>>>(p);
+  return after_launch("paged_attention_any_kernel");
+}
+
+// What launch_paged_ring found out about a kernel: blocks per SM for its two block sizes.
+struct PagedRingFit {
+  int smem[2] = {0, 0}, blocks[2] = {0, 0};
+};
+
+// Launches a kernel whose blocks keep rings: `gp` heads per pass, `per_warp` and `fixed` bytes of shared
+// memory, or as much as joining `rows` heads takes where the rings were.
+template <class Ring, class Kernel>
+static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, int gp, int rows, int dhp, int fixed, int per_warp,
+                             PagedRingFit* fits) {
+  p.head_blocks = (p.group + gp - 1) / gp;
+  p.units = p.kv.kv_heads * p.head_blocks;
+  // A block of all the SM's warps where the sequences are fewer than the SMs: each is cut into parts
+  // for many SMs, and a part per SM is the least to join.  Else two blocks, one of which works while the
+  // other's warps wait for one another at the end of a part.
+  const int kind = int64_t(p.kv.batch) * p.units < dev->sm_count || Ring::WARPS <= 4 ? 0 : 1;
+  const int warps = kind == 0 ? Ring::WARPS : Ring::WARPS / 2;
+  const int join = pa_finish_floats(warps, rows, dhp) * 4;
+  const int smem = fixed + (warps * per_warp > join ? warps * per_warp : join);
+  PagedRingFit& fit = fits[dev->device];
+  if (fit.smem[kind] < smem) {
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       smem > fit.smem[1 - kind] ? smem : fit.smem[1 - kind]),
+                  "cudaFuncSetAttribute(paged attention)");
+    int blocks = 0;
+    MIRA_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kern, warps * 32, smem), "occupancy(paged attention)");
+    fit.blocks[kind] = blocks < 1 ? 1 : (blocks > PA_MAX_BLOCKS_PER_SM ? PA_MAX_BLOCKS_PER_SM : blocks);
+    fit.smem[kind] = smem;
+  }
+  kern<<<unsigned(dev->sm_count * fit.blocks[kind]), warps * 32, smem, dev->stream>>>(p);
   return after_launch("paged_attention_kernel");
 }
 
-template <typename T, int GP, int VB>
-static int launch_paged_fma_dh(DeviceState* dev, PagedAttnParams& p) {
-  if (p.kv.dh <= 32) return launch_paged_fma<T, 32, GP, VB>(dev, p);
-  if (p.kv.dh <= 64) return launch_paged_fma<T, 64, GP, VB>(dev, p);
-  if (p.kv.dh <= 128) return launch_paged_fma<T, 128, GP, VB>(dev, p);
-  return launch_paged_fma<T, 256, GP, VB>(dev, p);
+template <int DHP, int GP>
+static int launch_paged_f32(DeviceState* dev, PagedAttnParams& p) {
+  using C = PaF32<DHP, GP>;
+  static PagedRingFit fits[kMaxDevices];
+  return launch_paged_ring<typename C::Ring>(dev, p, paged_attention_f32_kernel<DHP, GP>, GP, GP, DHP, 0, C::Ring::BYTES, fits);
+}
+
+template <int GP>
+static int launch_paged_f32_dh(DeviceState* dev, PagedAttnParams& p) {
+  if (p.kv.dh <= 32) return launch_paged_f32<32, GP>(dev, p);
+  if (p.kv.dh <= 64) return launch_paged_f32<64, GP>(dev, p);
+  if (p.kv.dh <= 128) return launch_paged_f32<128, GP>(dev, p);
+  return launch_paged_f32<256, GP>(dev, p);
 }
 
 template <typename T, int DHP, int VB, int QP>
 static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
   using C = PaMma<T, DHP, VB, QP>;
-  auto kern = paged_attention_mma_kernel<T, DHP, VB, QP>;
-  const int rows = p.group < 16 ? p.group : 16;
-  p.head_blocks = (p.group + 15) / 16;
-  p.units = p.kv.kv_heads * p.head_blocks;
-  // A block of all the SM's warps where the sequences are fewer than the SMs: each is cut into parts
-  // for many SMs, and a part per SM is the least to join.  Else blocks of four warps, which wait for
-  // fewer others at the end of a part.
-  const int warps = int64_t(p.kv.batch) * p.units < dev->sm_count ? C::WARPS : 4;
-  const int smem = C::Q_BYTES + pa_finish_floats(warps, rows, DHP) * 4;
-  static int configured[kMaxDevices] = {};
-  if (configured[dev->device] < smem) {
-    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                  "cudaFuncSetAttribute(paged attention)");
-    configured[dev->device] = smem;
-  }
-  kern<<<unsigned(dev->sm_count * (C::WARPS / warps)), warps * 32, smem, dev->stream>>>(p);
-  return after_launch("paged_attention_mma_kernel");
+  static PagedRingFit fits[kMaxDevices];
+  return launch_paged_ring<typename C::Ring>(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP>, 16, p.group < 16 ? p.group : 16, DHP,
+                                             C::Q_BYTES, C::SCALES + C::Ring::BYTES, fits);
 }
 
 template <typename T, int VB, int QP>
@@ -2202,20 +2223,20 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
   const bool vec = paged_rows_aligned(a->kv, 16);
   switch (a->kv.dtype) {
     case MIRA_DT_F32:
-      if (!vec) return launch_paged_fma<float, 256, 1, 4>(dev, p);
-      if (p.group == 1) return launch_paged_fma_dh<float, 1, 16>(dev, p);
-      if (p.group == 2) return launch_paged_fma_dh<float, 2, 16>(dev, p);
-      return launch_paged_fma_dh<float, 4, 16>(dev, p);
+      if (!vec) return launch_paged_any<float>(dev, p);
+      if (p.group == 1) return launch_paged_f32_dh<1>(dev, p);
+      if (p.group == 2) return launch_paged_f32_dh<2>(dev, p);
+      return launch_paged_f32_dh<4>(dev, p);
     case MIRA_DT_F16:
-      if (!vec) return launch_paged_fma<__half, 256, 1, 2>(dev, p);
+      if (!vec) return launch_paged_any<__half>(dev, p);
       return launch_paged_mma_q<__half, 16>(dev, p, p.q_dtype == MIRA_DT_F16);
     case MIRA_DT_BF16:
-      if (!vec) return launch_paged_fma<__nv_bfloat16, 256, 1, 2>(dev, p);
+      if (!vec) return launch_paged_any<__nv_bfloat16>(dev, p);
       return launch_paged_mma_q<__nv_bfloat16, 16>(dev, p, p.q_dtype == MIRA_DT_BF16);
     default:
       if (vec) return launch_paged_mma_q<int8_t, 16>(dev, p, p.q_dtype == MIRA_DT_F16);
       if (paged_rows_aligned(a->kv, 8)) return launch_paged_mma_q<int8_t, 8>(dev, p, p.q_dtype == MIRA_DT_F16);
-      return launch_paged_fma<int8_t, 256, 1, 1>(dev, p);
+      return launch_paged_any<int8_t>(dev, p);
   }
 }
 

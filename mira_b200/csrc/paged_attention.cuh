@@ -96,7 +96,8 @@ struct PaWork {
   int t0, t1;
 };
 
-// least: tiles that a block can do at once, below which more blocks would only add joining.
+// least: tiles that a block can do at once; no unit is cut into smaller parts, which would only add
+// joining.
 template <int TILE>
 __device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, PaWork& w) {
   __shared__ int64_t s_scan[PA_MAX_WARPS];
@@ -108,7 +109,8 @@ __device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, Pa
     total += pa_scan(b < p.kv.batch ? pa_seq<TILE>(p, b).tiles : 0, before, s_scan);
   }
   w.total = total * p.units;
-  w.blocks = min(int64_t(gridDim.x), (w.total + least - 1) / least);
+  const int64_t apart = max(int64_t(p.kv.batch) * p.units, (w.total + least - 1) / least);
+  w.blocks = min(min(int64_t(gridDim.x), w.total), apart);
   if (blockIdx.x >= w.blocks) return false;
   w.lo = w.cur = pa_lo(w.total, blockIdx.x, w.blocks);
   w.hi = pa_lo(w.total, blockIdx.x + 1, w.blocks);
@@ -308,10 +310,322 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
   __syncthreads();     // the shared triples are free again
 }
 
-// ---------------------------------------------------------------- the kernel on FMA units
+// ---------------------------------------------------------------- rows in flight
 
-// T: the pages' element; DHP: head dimension rounded up to 32, 64, 128 or 256; GP: query heads that
-// share a pass over the rows; VB: bytes per access (16, or less where rows are not 16-byte aligned).
+// What hides the memory's latency is bytes in flight, about 64 KB per SM at full bandwidth: more than
+// registers can hold beside the sums.  Each lane therefore copies the 16-byte pieces it will use itself
+// to its own places in shared memory (cp.async, piece j of lane l at (32 j + l) * size), a step or two
+// ahead, and reads them back when their turn comes: no bank conflicts, and nothing but the lane's own
+// wait between the copy and the use.
+template <int STAGE_BYTES, bool WIDE>      // a warp's step; WIDE: sums that need more than 168 registers
+struct PaRing {
+  static constexpr int WARPS = STAGE_BYTES > 8192 ? 4 : WIDE ? 8 : STAGE_BYTES > 4096 ? 12 : 16;    // of an SM
+  static constexpr int STAGES = STAGE_BYTES <= 4096 ? 3 : STAGE_BYTES <= 8192 ? 2 : 3;
+  static constexpr int BYTES = STAGE_BYTES * STAGES;                                       // of a warp
+};
+
+// One token of a step, held by one lane: where its rows are.
+struct PaToken {
+  int64_t k, v;       // byte offsets in the pages
+  bool ok;
+};
+
+template <typename T>
+__device__ __forceinline__ PaToken pa_token(const PagedAttnParams& p, const PaWork& w, const int32_t* trow, int i, bool mine,
+                                            int& page, int& slot) {
+  PaToken t;
+  page = slot = 0;
+  t.ok = mine && i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page, slot);
+  t.k = (page * p.kv.kst[0] + slot * p.kv.kst[2]) * int(sizeof(T));
+  t.v = (page * p.kv.vst[0] + slot * p.kv.vst[2]) * int(sizeof(T));
+  return t;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void pa_copy(uint32_t dst, const uint8_t* src, bool ok) {
+  const uint32_t n = ok ? BYTES : 0;
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
+}
+
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------- f32 pages
+
+// DHP: head dimension rounded up to 32, 64, 128 or 256; GP: query heads that share a pass over the rows.
+// A row is spread over LPR lanes, 16 bytes each, a warp takes TPS rows at a time and U times that in a
+// step.  The LPR partial sums of the step's U GP scores are added crosswise, each exchange halving the
+// number of scores a lane carries, so that a score's softmax is worked out in few lanes, not in all.
+template <int DHP, int GP>
+struct PaF32 {
+  static constexpr int LPR = DHP / 4 < 32 ? DHP / 4 : 32;
+  static constexpr int NV = DHP / (4 * LPR);
+  static constexpr int EPL = 4 * NV;
+  static constexpr int TPS = 32 / LPR;
+  static constexpr int U = NV > 1 ? 4 : 8;
+  static constexpr int TILE = TPS * U;                      // rows of a warp step
+  static constexpr int STAGE = 2 * U * NV * 512;
+  static constexpr int N = U * GP;                          // scores of a lane group
+  static constexpr int HALVINGS = N <= LPR ? (N == 4 ? 2 : N == 8 ? 3 : N == 16 ? 4 : 5) : (LPR == 8 ? 3 : LPR == 16 ? 4 : 5);
+  static constexpr int LEFT = N >> HALVINGS;                // scores a lane ends up with
+  using Ring = PaRing<STAGE, false>;
+};
+
+template <int DHP, int GP>
+__global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
+    paged_attention_f32_kernel(const __grid_constant__ PagedAttnParams p) {
+  using C = PaF32<DHP, GP>;
+  using Ring = typename C::Ring;
+  extern __shared__ __align__(128) uint8_t pa_ring[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int sub = lane % C::LPR, group0 = lane - sub, row0 = lane / C::LPR;
+  const uint32_t ring = smem_u32(pa_ring) + warp * Ring::BYTES + lane * 16;
+  const uint8_t* held = pa_ring + warp * Ring::BYTES + lane * 16;
+  PaWork w;
+  if (!pa_begin<C::TILE>(p, warps, w)) return;
+  while (pa_part<C::TILE>(p, w)) {
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
+    const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
+    const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.k) + kvh * p.kv.kst[1] + sub * 4);
+    const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.v) + kvh * p.kv.vst[1] + sub * 4);
+
+    // lane i looks up row i of a step, a step before its copies are issued
+    PaToken tok;
+    uint32_t live[Ring::STAGES];        // rows of the steps in the ring that count
+    auto look = [&](int at) {
+      int page, slot;
+      tok = pa_token<float>(p, w, trow, at + lane, lane < C::TILE, page, slot);
+    };
+    auto issue = [&](int stage) {
+      live[Ring::STAGES - 1] = __ballot_sync(0xffffffffu, tok.ok);
+      const uint32_t dst = ring + stage * C::STAGE;
+#pragma unroll
+      for (int u = 0; u < C::U; ++u) {
+        const int i = u * C::TPS + row0;
+        const int64_t ko = __shfl_sync(0xffffffffu, tok.k, i), vo = __shfl_sync(0xffffffffu, tok.v, i);
+        const bool in = live[Ring::STAGES - 1] >> i & 1;
+#pragma unroll
+        for (int j = 0; j < C::NV; ++j) {
+          const bool inside = in && (sub + j * C::LPR) * 4 < p.kv.dh;
+          pa_copy<16>(dst + (u * C::NV + j) * 512, kb + ko + j * C::LPR * 16, inside);
+          pa_copy<16>(dst + ((C::U + u) * C::NV + j) * 512, vb + vo + j * C::LPR * 16, inside);
+        }
+      }
+      cp_async_commit();
+    };
+    const int step = warps * C::TILE;
+    int at = w.t0 + warp * C::TILE, next = at;
+    look(next);
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; ++i) {
+#pragma unroll
+      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
+      issue(i);
+      next += step;
+      look(next);
+    }
+
+    float q[GP][C::EPL], acc[GP][C::EPL], m[GP], l[C::LEFT];
+#pragma unroll
+    for (int gi = 0; gi < GP; ++gi) {
+      m[gi] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < C::EPL; ++e) {
+        const int d = (sub + (e / 4) * C::LPR) * 4 + e % 4;
+        q[gi][e] = (g0 + gi < p.group && d < p.kv.dh)
+            ? dt_load(p.q, w.b * p.qs[0] + (kvh * p.group + g0 + gi) * p.qs[1] + d * p.qs[2], p.q_dtype) * p.scale_log2
+            : 0.0f;
+        acc[gi][e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < C::LEFT; ++i) l[i] = 0.0f;
+
+    int stage = 0, into = Ring::STAGES - 1;
+    for (; at < w.t1; at += step) {
+      cp_async_wait<Ring::STAGES - 2>();
+#pragma unroll
+      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
+      issue(into);
+      next += step;
+      look(next);
+      const uint32_t now = live[0];
+      const uint8_t* rows = held + stage * C::STAGE;
+      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
+      into = into + 1 == Ring::STAGES ? 0 : into + 1;
+
+      // scores, score u GP + gi of the lane group's rows
+      float s[C::N];
+#pragma unroll
+      for (int u = 0; u < C::U; ++u) {
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi) s[u * GP + gi] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C::NV; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(rows + (u * C::NV + j) * 512);
+#pragma unroll
+          for (int gi = 0; gi < GP; ++gi) {
+            float& y = s[u * GP + gi];
+            y = fmaf(q[gi][4 * j], x.x, y);
+            y = fmaf(q[gi][4 * j + 1], x.y, y);
+            y = fmaf(q[gi][4 * j + 2], x.z, y);
+            y = fmaf(q[gi][4 * j + 3], x.w, y);
+          }
+        }
+      }
+      // halving h: the lanes of the upper half of 2^(.. - h) keep the upper half of the scores
+#pragma unroll
+      for (int h = 0; h < C::HALVINGS; ++h) {
+        const int o = C::LPR >> (h + 1), half = C::N >> (h + 1);
+        const bool upper = sub & o;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+          const float give = upper ? s[i] : s[i + half], keep = upper ? s[i + half] : s[i];
+          s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      }
+#pragma unroll
+      for (int o = C::LPR >> (C::HALVINGS + 1); o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < C::LEFT; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+      // this lane's scores are first .. first + LEFT - 1
+      const int first = (sub >> (C::LPR == 32 ? 5 - C::HALVINGS : C::LPR == 16 ? 4 - C::HALVINGS : 3 - C::HALVINGS)) * C::LEFT;
+#pragma unroll
+      for (int i = 0; i < C::LEFT; ++i) {
+        const int u = (first + i) / GP;
+        if (!(now >> (u * C::TPS + row0) & 1)) s[i] = -INFINITY;
+      }
+      // the largest of each head, in all lanes of the group
+      float top[GP];
+#pragma unroll
+      for (int gi = 0; gi < GP; ++gi) top[gi] = m[gi];
+      if (C::LEFT == 1) {
+        float x = s[0];       // lanes whose score index agrees mod GP share a head
+        constexpr int SHARE = C::LPR / C::N;
+#pragma unroll
+        for (int o = C::LPR / 2; o >= GP * SHARE; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi)
+          top[gi] = fmaxf(top[gi], GP == 1 ? x : __shfl_sync(0xffffffffu, x, group0 + gi * SHARE));
+      } else {
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < C::LEFT; ++i)
+            if ((first + i) % GP == gi) x = fmaxf(x, s[i]);
+#pragma unroll
+          for (int o = 1; o < C::LPR; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+          top[gi] = fmaxf(top[gi], x);
+        }
+      }
+      bool moved = false;
+#pragma unroll
+      for (int gi = 0; gi < GP; ++gi) moved = moved || top[gi] > m[gi];
+      if (__any_sync(0xffffffffu, moved)) {
+        float fade[GP];
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi) {
+          fade[gi] = pa_exp2(m[gi] - (top[gi] == -INFINITY ? 0.0f : top[gi]));
+          m[gi] = top[gi];
+#pragma unroll
+          for (int e = 0; e < C::EPL; ++e) acc[gi][e] *= fade[gi];
+        }
+#pragma unroll
+        for (int i = 0; i < C::LEFT; ++i) {
+          float f = fade[0];
+#pragma unroll
+          for (int gi = 1; gi < GP; ++gi) f = (first + i) % GP == gi ? fade[gi] : f;
+          l[i] *= f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::LEFT; ++i) {
+        float z = m[0];
+#pragma unroll
+        for (int gi = 1; gi < GP; ++gi) z = (first + i) % GP == gi ? m[gi] : z;
+        s[i] = pa_exp2(s[i] - (z == -INFINITY ? 0.0f : z));
+        l[i] += s[i];
+      }
+      constexpr int WIDTH = C::LPR >> C::HALVINGS;      // lanes that hold the same scores
+#pragma unroll
+      for (int u = 0; u < C::U; ++u) {
+        float pr[GP];
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi) {
+          const int n = u * GP + gi;
+          pr[gi] = __shfl_sync(0xffffffffu, s[n % C::LEFT], group0 + n / C::LEFT * WIDTH);
+        }
+#pragma unroll
+        for (int j = 0; j < C::NV; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(rows + ((C::U + u) * C::NV + j) * 512);
+#pragma unroll
+          for (int gi = 0; gi < GP; ++gi) {
+            acc[gi][4 * j] = fmaf(pr[gi], x.x, acc[gi][4 * j]);
+            acc[gi][4 * j + 1] = fmaf(pr[gi], x.y, acc[gi][4 * j + 1]);
+            acc[gi][4 * j + 2] = fmaf(pr[gi], x.z, acc[gi][4 * j + 2]);
+            acc[gi][4 * j + 3] = fmaf(pr[gi], x.w, acc[gi][4 * j + 3]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();        // the ring becomes the place of the warps' triples
+
+    // l of each head: the lanes' sums of its scores
+    float lsum[GP];
+    constexpr int WIDTH = C::LPR >> C::HALVINGS;
+    const int first = sub / WIDTH * C::LEFT;
+#pragma unroll
+    for (int gi = 0; gi < GP; ++gi) {
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < C::LEFT; ++i)
+        if ((first + i) % GP == gi) x += l[i];
+#pragma unroll
+      for (int o = WIDTH; o < C::LPR; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      lsum[gi] = x;
+    }
+    float* sm = reinterpret_cast<float*>(pa_ring);
+    float* mine = sm + warp * pa_triple(GP, DHP);
+#pragma unroll
+    for (int gi = 0; gi < GP; ++gi) {
+#pragma unroll
+      for (int o = C::LPR; o < 32; o <<= 1) {
+        const float mo = __shfl_xor_sync(0xffffffffu, m[gi], o), lo = __shfl_xor_sync(0xffffffffu, lsum[gi], o);
+        const float top = fmaxf(m[gi], mo);
+        const float wa = pa_weight(m[gi], top), wb = pa_weight(mo, top);
+        lsum[gi] = lsum[gi] * wa + lo * wb;
+        m[gi] = top;
+#pragma unroll
+        for (int e = 0; e < C::EPL; ++e)
+          acc[gi][e] = acc[gi][e] * wa + __shfl_xor_sync(0xffffffffu, acc[gi][e], o) * wb;
+      }
+      if (row0 == 0) {
+#pragma unroll
+        for (int j = 0; j < C::NV; ++j)
+          *reinterpret_cast<float4*>(mine + pa_head(GP) + gi * DHP + (sub + j * C::LPR) * 4) =
+              make_float4(acc[gi][4 * j], acc[gi][4 * j + 1], acc[gi][4 * j + 2], acc[gi][4 * j + 3]);
+      }
+      if (lane == 0) {
+        mine[gi] = m[gi];
+        mine[GP + gi] = lsum[gi];
+      }
+    }
+    pa_finish<DHP>(p, w, sm, GP, kvh * p.group + g0, min(GP, p.group - g0));
+    w.cur = w.end;
+  }
+}
+
+// ---------------------------------------------------------------- rows that are not 16-byte aligned
+
+// T: the pages' element, one per access; the head dimension is taken as 256 and each query head reads the
+// rows anew (the repeats come from the caches).  Right for every stride and size, and slow: 16-byte
+// aligned rows go to the other kernels.
 template <typename T, int DHP, int GP, int VB>
 struct PaCfg {
   static constexpr int WARPS = 8;
@@ -328,7 +642,7 @@ struct PaCfg {
 
 template <typename T, int DHP, int GP, int VB>
 __global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
-    paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
+    paged_attention_any_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PaCfg<T, DHP, GP, VB>;
   using V = typename PaVec<VB>::type;
   constexpr bool I8 = sizeof(T) == 1;

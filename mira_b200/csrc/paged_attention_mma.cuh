@@ -4,7 +4,7 @@
 // bytes a clock.  The group's heads are the 16 rows of the products, so a key costs the same few
 // instructions for one head as for sixteen, and what remains is unpacking, addresses and the softmax.
 //
-// Everything stays in registers: the sums over k of a product do not care in which order k comes, so a
+// No fragment crosses lanes: the sums over k of a product do not care in which order k comes, so a
 // lane's 16-byte piece of a row, as it arrives from memory, is its share of a fragment.
 //   S = Q K^T: lane (g, t) holds token g's elements VE t .. VE t + VE - 1 of each run of 4 VE: four of
 //     them are the right operand of one 16x8x16 product; Q is laid out to match, once per unit.
@@ -42,7 +42,10 @@ struct PaMma {
   // p is carried times 2^8: the smallest f16 is then 2^-32 of the largest weight.
   static constexpr int PP = BF16 && QP == 3 ? 3 : 2;
   static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
-  static constexpr int WARPS = DHP <= 64 ? 16 : DHP <= 128 ? 12 : 8;       // of an SM, by registers
+  static constexpr int K_BYTES = TT * 2 * KL * 32 * VB, V_BYTES = TT * 4 * VL * 32 * VBV;    // of a step
+  using Ring = PaRing<K_BYTES + V_BYTES, (DHP > 128)>;
+  static constexpr int STAGE = K_BYTES + V_BYTES;
+  static constexpr int SCALES = I8 ? 2 * 32 * 4 * Ring::STAGES : 0;        // bytes of a warp's scales
   static constexpr int Q_BYTES = QP * KS * 32 * 16;
 };
 
@@ -79,75 +82,90 @@ __device__ __forceinline__ uint32_t pa_codes(uint32_t biased, uint32_t sel) {
 template <int WORDS> struct PaWords { uint32_t w[WORDS]; };
 
 template <int BYTES>
-__device__ __forceinline__ PaWords<BYTES / 4> pa_load(const void* p, bool ok) {
+__device__ __forceinline__ PaWords<BYTES / 4> pa_held(const uint8_t* p) {
   PaWords<BYTES / 4> r;
-  if (BYTES == 16) {
-    const uint4 v = ok ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-    r.w[0] = v.x; r.w[1] = v.y; r.w[2 % (BYTES / 4)] = v.z; r.w[3 % (BYTES / 4)] = v.w;
-  } else {
-    const uint2 v = ok ? __ldg(static_cast<const uint2*>(p)) : make_uint2(0, 0);
-    r.w[0] = v.x; r.w[1] = v.y;
-  }
+  memcpy(&r, __builtin_assume_aligned(p, BYTES), BYTES);
   return r;
 }
 
 template <typename T, int DHP, int VB, int QP>
-__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
+__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
     paged_attention_mma_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PaMma<T, DHP, VB, QP>;
-  extern __shared__ __align__(16) float pa_smem[];
+  using Ring = typename C::Ring;
+  extern __shared__ __align__(128) uint8_t pa_ring[];      // queries, then per warp its scales and ring
   __shared__ float s_unit[16];        // per head: what turns a product into a scaled score
-  uint4* s_q = reinterpret_cast<uint4*>(pa_smem);                  // [piece][product][lane]
-  float* s_join = pa_smem + C::Q_BYTES / 4;
+  uint4* s_q = reinterpret_cast<uint4*>(pa_ring);                  // [piece][product][lane]
+  float* s_join = reinterpret_cast<float*>(pa_ring + C::Q_BYTES);  // the warps' triples, where the rings were
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
   const int rows = min(16, p.group);
+  float* scales = reinterpret_cast<float*>(pa_ring + C::Q_BYTES + warp * (C::SCALES + Ring::BYTES));   // [stage][k, v][token]
+  uint8_t* held = reinterpret_cast<uint8_t*>(scales) + C::SCALES;
+  const uint32_t ring = smem_u32(held);
   PaWork w;
   if (!pa_begin<C::TILE>(p, warps, w)) return;
   while (pa_part<C::TILE>(p, w)) {
     const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * 16;
-    const int h0 = kvh * p.group + g0, live = min(16, p.group - g0);
+    const int h0 = kvh * p.group + g0, live_heads = min(16, p.group - g0);
     const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
-    const T* kb = static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE;
-    const T* vb = static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE;
+    const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE);
+    const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE);
 
-    // lane i looks up token i of a step; the step's rows are shared by shuffles
-    int page = 0, slot = 0;
-    bool ok = false;
+    // lane i looks up token i of a step, a step before its copies are issued
+    PaToken tok;
+    int64_t ks_at = 0, vs_at = 0;
+    uint32_t live[Ring::STAGES];        // tokens of the steps in the ring that count
     auto look = [&](int at) {
-      const int i = at + lane;
-      page = slot = 0;
-      ok = lane < C::TILE && i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page, slot);
+      int page, slot;
+      tok = pa_token<T>(p, w, trow, at + lane, lane < C::TILE, page, slot);
+      if (C::I8) {
+        ks_at = page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2];
+        vs_at = page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2];
+      }
     };
-    PaWords<VB / 4> kr[C::TT][2][C::KL];
-    float kscale[C::TT][4];
-    uint32_t live_k = 0;      // tokens of the step whose keys kr holds
-    auto load_k = [&]() {
-      live_k = __ballot_sync(0xffffffffu, ok);
-      float mine = 0.0f;
-      if (C::I8 && ok) mine = __ldg(p.kv.ks + page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2]);
+    auto issue = [&](int stage) {
+      const uint32_t alive = __ballot_sync(0xffffffffu, tok.ok);
+      live[Ring::STAGES - 1] = alive;
+      const uint32_t kd = ring + stage * C::STAGE + lane * VB, vd = ring + stage * C::STAGE + C::K_BYTES + lane * C::VBV;
+      if (C::I8) {
+        const uint32_t sd = smem_u32(scales) + (stage * 64 + lane) * 4;
+        pa_copy<4>(sd, reinterpret_cast<const uint8_t*>(p.kv.ks + ks_at), tok.ok);
+        pa_copy<4>(sd + 128, reinterpret_cast<const uint8_t*>(p.kv.vs + vs_at), tok.ok);
+      }
 #pragma unroll
-      for (int r = 0; r < C::TT; ++r)
+      for (int r = 0; r < C::TT; ++r) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int i = r * 16 + n * 8 + g;
-          const int pg = __shfl_sync(0xffffffffu, page, i), sl = __shfl_sync(0xffffffffu, slot, i);
-          const T* row = kb + pg * p.kv.kst[0] + sl * p.kv.kst[2];
-          const bool in = live_k >> i & 1;
+          const uint8_t* row = kb + __shfl_sync(0xffffffffu, tok.k, i);
+          const bool in = alive >> i & 1;
 #pragma unroll
-          for (int j = 0; j < C::KL; ++j) {
-            const bool inside = j * 4 * C::KE + t * C::KE < p.kv.dh;
-            kr[r][n][j] = pa_load<VB>(row + j * 4 * C::KE, in && inside);
-          }
-          if (C::I8) {
-            kscale[r][2 * n] = __shfl_sync(0xffffffffu, mine, r * 16 + n * 8 + 2 * t);
-            kscale[r][2 * n + 1] = __shfl_sync(0xffffffffu, mine, r * 16 + n * 8 + 2 * t + 1);
-          }
+          for (int j = 0; j < C::KL; ++j)
+            pa_copy<VB>(kd + ((r * 2 + n) * C::KL + j) * (32 * VB), row + j * 4 * VB, in && (j * 4 + t) * C::KE < p.kv.dh);
         }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
+          const uint8_t* row = vb + __shfl_sync(0xffffffffu, tok.v, i);
+          const bool in = alive >> i & 1;
+#pragma unroll
+          for (int j = 0; j < C::VL; ++j)
+            pa_copy<C::VBV>(vd + ((r * 4 + n) * C::VL + j) * (32 * C::VBV), row + j * 8 * C::VBV, in && (j * 8 + g) * C::VE < p.kv.dh);
+        }
+      }
+      cp_async_commit();
     };
     const int step = warps * C::TILE;
-    int at = w.t0 + warp * C::TILE;
-    look(at);
-    load_k();        // before the queries: their latencies overlap
+    int at = w.t0 + warp * C::TILE, next = at;
+    look(next);
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; ++i) {       // before the queries: their latencies overlap
+#pragma unroll
+      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
+      issue(i);
+      next += step;
+      look(next);
+    }
 
     // queries of the unit in fragment order; a thread per (product, lane).  f16 values of a query that
     // is not f16 itself are taken after a power of two has brought its largest element to [128, 256).
@@ -155,7 +173,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
       float unit = p.scale_log2;
       if (QP == 3 && !C::BF16) {
         float top = 0.0f;
-        if (h < live)
+        if (h < live_heads)
           for (int d = lane; d < p.kv.dh; d += 32)
             top = fmaxf(top, fabsf(dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + d * p.qs[2], p.q_dtype)));
 #pragma unroll
@@ -177,7 +195,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int h = lg + 8 * hh;
-          float v = h < live && d + e < p.kv.dh
+          float v = h < live_heads && d + e < p.kv.dh
               ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + (d + e) * p.qs[2], p.q_dtype) : 0.0f;
           if (QP == 3 && !C::BF16) v *= s_unit[h];
           x[hh][e] = v;
@@ -213,27 +231,21 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
+    int stage = 0, into = Ring::STAGES - 1;
     for (; at < w.t1; at += step) {
-      // values of this step
-      PaWords<C::VBV / 4> vr[C::TT][4][C::VL];
-      float vscale = 0.0f;
-      const uint32_t now = live_k;
-      if (C::I8 && ok) vscale = __ldg(p.kv.vs + page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2]);
+      cp_async_wait<Ring::STAGES - 2>();
+      __syncwarp();
 #pragma unroll
-      for (int r = 0; r < C::TT; ++r)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
-          const int pg = __shfl_sync(0xffffffffu, page, i), sl = __shfl_sync(0xffffffffu, slot, i);
-          const T* row = vb + pg * p.kv.vst[0] + sl * p.kv.vst[2];
-          const bool in = now >> i & 1;
-#pragma unroll
-          for (int j = 0; j < C::VL; ++j) {
-            const bool inside = j * 8 * C::VE + g * C::VE < p.kv.dh;
-            vr[r][n][j] = pa_load<C::VBV>(row + j * 8 * C::VE, in && inside);
-          }
-        }
-      look(at + step);
+      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
+      issue(into);
+      next += step;
+      look(next);
+      const uint32_t now = live[0];
+      const uint8_t* kr = held + stage * C::STAGE + lane * VB;
+      const uint8_t* vr = held + stage * C::STAGE + C::K_BYTES + lane * C::VBV;
+      const float* sc = scales + stage * 64;
+      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
+      into = into + 1 == Ring::STAGES ? 0 : into + 1;
 
       // scores
       float s[C::TT][2][4];
@@ -244,7 +256,12 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[r][n][i] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < C::KL; ++j)
+      for (int j = 0; j < C::KL; ++j) {
+        PaWords<VB / 4> kx[C::TT][2];
+#pragma unroll
+        for (int r = 0; r < C::TT; ++r)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) kx[r][n] = pa_held<VB>(kr + ((r * 2 + n) * C::KL + j) * (32 * VB));
 #pragma unroll
         for (int e = 0; e < C::KE / 4; ++e) {
           uint32_t b[C::TT][2][2];
@@ -253,12 +270,12 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               if (C::I8) {
-                const uint32_t x = kr[r][n][j].w[e] ^ 0x80808080u;
+                const uint32_t x = kx[r][n].w[e] ^ 0x80808080u;
                 b[r][n][0] = pa_codes(x, 0x4140);
                 b[r][n][1] = pa_codes(x, 0x4342);
               } else {
-                b[r][n][0] = kr[r][n][j].w[(2 * e) % (VB / 4)];
-                b[r][n][1] = kr[r][n][j].w[(2 * e + 1) % (VB / 4)];
+                b[r][n][0] = kx[r][n].w[(2 * e) % (VB / 4)];
+                b[r][n][1] = kx[r][n].w[(2 * e + 1) % (VB / 4)];
               }
             }
 #pragma unroll
@@ -270,6 +287,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
               for (int n = 0; n < 2; ++n) mma_16816<C::BF16>(s[r][n], a.x, a.y, a.z, a.w, b[r][n][0], b[r][n][1]);
           }
         }
+      }
       float top0 = m0, top1 = m1;
 #pragma unroll
       for (int r = 0; r < C::TT; ++r)
@@ -278,29 +296,28 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const bool in = now >> (r * 16 + n * 8 + 2 * t + i) & 1;
-            const float ks = C::I8 ? kscale[r][2 * n + i] : 1.0f;
+            const float ks = C::I8 ? sc[r * 16 + n * 8 + 2 * t + i] : 1.0f;
             s[r][n][i] = in ? s[r][n][i] * (C::I8 ? unit0 * ks : unit0) : -INFINITY;
             s[r][n][2 + i] = in ? s[r][n][2 + i] * (C::I8 ? unit1 * ks : unit1) : -INFINITY;
             top0 = fmaxf(top0, s[r][n][i]);
             top1 = fmaxf(top1, s[r][n][2 + i]);
           }
-      load_k();          // the next step's keys, while this one's softmax and values go on
-
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
         top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
         top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
       }
-      float grow = 1.0f;
+      float grow = 1.0f, shrink = 1.0f;
       if (C::I8) {
+        const float vscale = lane < C::TILE && (now >> lane & 1) ? sc[32 + lane] : 0.0f;
         const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vscale))) >> 23, v_exp), 253u);
         grow = __int_as_float((127 - min(int(e - v_exp), 126)) << 23);
         v_exp = e;
-        vscale *= __int_as_float((254 - e) << 23);
+        shrink = __int_as_float((254 - e) << 23);
       }
       const float safe0 = top0 == -INFINITY ? 0.0f : top0, safe1 = top1 == -INFINITY ? 0.0f : top1;
       if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1 || grow != 1.0f)) {
-        const float f0 = exp2f(m0 - safe0), f1 = exp2f(m1 - safe1);
+        const float f0 = pa_exp2(m0 - safe0), f1 = pa_exp2(m1 - safe1);
         m0 = top0;
         m1 = top1;
         l0 *= f0;
@@ -319,13 +336,13 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
         uint32_t a[4][C::PP];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          float x0 = exp2f(s[r][n][0] - z0), x1 = exp2f(s[r][n][1] - z0);
-          float y0 = exp2f(s[r][n][2] - z1), y1 = exp2f(s[r][n][3] - z1);
+          float x0 = pa_exp2(s[r][n][0] - z0), x1 = pa_exp2(s[r][n][1] - z0);
+          float y0 = pa_exp2(s[r][n][2] - z1), y1 = pa_exp2(s[r][n][3] - z1);
           l0 += x0 + x1;
           l1 += y0 + y1;
           if (C::I8) {
-            const float u0 = __shfl_sync(0xffffffffu, vscale, r * 16 + n * 8 + 2 * t);
-            const float u1 = __shfl_sync(0xffffffffu, vscale, r * 16 + n * 8 + 2 * t + 1);
+            const int i = r * 16 + n * 8 + 2 * t;       // a token that does not count has no scale either
+            const float u0 = now >> i & 1 ? sc[32 + i] * shrink : 0.0f, u1 = now >> (i + 1) & 1 ? sc[33 + i] * shrink : 0.0f;
             x0 *= u0;
             x1 *= u1;
             y0 *= u0;
@@ -335,14 +352,17 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
           pa_split2<C::BF16, C::PP>(y0, y1, a[2 * n + 1]);
         }
 #pragma unroll
-        for (int j = 0; j < C::VL; ++j)
+        for (int j = 0; j < C::VL; ++j) {
+          PaWords<C::VBV / 4> vx[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) vx[n] = pa_held<C::VBV>(vr + ((r * 4 + n) * C::VL + j) * (32 * C::VBV));
 #pragma unroll
           for (int e = 0; e < C::VBV / 4; ++e) {
             constexpr int PER = 4 / int(sizeof(T));      // elements of a word
             uint32_t b[PER][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t x = vr[r][2 * h][j].w[e], y = vr[r][2 * h + 1][j].w[e];
+              const uint32_t x = vx[2 * h].w[e], y = vx[2 * h + 1].w[e];
               if (C::I8) {
                 const uint32_t bx = x ^ 0x80808080u, by = y ^ 0x80808080u;
                 const uint32_t low = __byte_perm(bx, by, 0x5140), high = __byte_perm(bx, by, 0x7362);
@@ -361,8 +381,11 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
               for (int q = C::PP - 1; q >= 0; --q)
                 mma_16816<C::BF16>(acc[j * C::VE + e * PER + i], a[0][q], a[1][q], a[2][q], a[3][q], b[i][0], b[i][1]);
           }
+        }
       }
     }
+    cp_async_wait<0>();
+    __syncthreads();        // the rings become the place of the warps' triples
 
     // the warp's triple
 #pragma unroll
@@ -390,7 +413,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
           to[(j * 8 + 2 * t + 1) * C::VE + i] = acc[j * C::VE + i][2 * hh + 1] * back_v;
         }
     }
-    pa_finish<DHP>(p, w, s_join, rows, h0, live);
+    pa_finish<DHP>(p, w, s_join, rows, h0, live_heads);
     w.cur = w.end;
   }
 }
