@@ -2083,7 +2083,7 @@ extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* re
 
 namespace mira {
 
-constexpr int PA_MAX_BLOCKS_PER_SM = 4;
+constexpr int PA_MAX_BLOCKS_PER_SM = 2;
 
 static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch * units * 4, 256); }
 
@@ -2098,44 +2098,41 @@ static int launch_paged_any(DeviceState* dev, PagedAttnParams& p) {
   return after_launch("paged_attention_any_kernel");
 }
 
-// What launch_paged_ring found out about a kernel: blocks per SM for its two block sizes.
-struct PagedRingFit {
-  int smem[2] = {0, 0}, blocks[2] = {0, 0};
-};
-
-// Launches a kernel whose blocks keep rings: `gp` heads per pass, `per_warp` and `fixed` bytes of shared
-// memory, or as much as joining `rows` heads takes where the rings were.
-template <class Ring, class Kernel>
-static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, int gp, int rows, int dhp, int fixed, int per_warp,
-                             PagedRingFit* fits) {
+// Launches a kernel whose blocks feed a ring: `gp` heads per pass, `rows` of them used, `sm_warps`
+// warps per SM, `fixed` bytes of shared memory beside the ring (steps of `step` bytes) and the
+// triples.
+template <class Kernel>
+static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, int sm_warps, int gp, int rows, int dhp, int step,
+                             int fixed, int* configured) {
   p.head_blocks = (p.group + gp - 1) / gp;
   p.units = p.kv.kv_heads * p.head_blocks;
-  // A block of all the SM's warps where the sequences are fewer than the SMs: each is cut into parts
-  // for many SMs, and a part per SM is the least to join.  Else two blocks, one of which works while the
-  // other's warps wait for one another at the end of a part.
-  const int kind = int64_t(p.kv.batch) * p.units < dev->sm_count || Ring::WARPS <= 4 ? 0 : 1;
-  const int warps = kind == 0 ? Ring::WARPS : Ring::WARPS / 2;
-  const int join = pa_finish_floats(warps, rows, dhp) * 4;
-  const int smem = fixed + (warps * per_warp > join ? warps * per_warp : join);
-  PagedRingFit& fit = fits[dev->device];
-  if (fit.smem[kind] < smem) {
-    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       smem > fit.smem[1 - kind] ? smem : fit.smem[1 - kind]),
+  // One block per SM where the sequences are fewer than the SMs: each is cut into parts for many SMs,
+  // and a part per SM is the least to join.  Else two, one of which works while the other's warps wait
+  // for one another at the end of a part.  Triples of many heads leave less room for the ring: then
+  // fewer warps.
+  const int blocks = int64_t(p.kv.batch) * p.units < dev->sm_count ? 1 : 2;
+  int all = sm_warps / blocks;
+  if (rows * dhp > 1024) all = all * 3 / 4;
+  const int warps = all - all / 3;        // the others copy
+  const int room = (blocks == 1 ? 225 : 111) << 10, triples = pa_finish_floats(warps, rows, dhp) * 4;
+  p.slots = (room - fixed - triples) / (warps * (step + 32));
+  if (p.slots > 4) p.slots = 4;
+  MIRA_CHECK_ARG(p.slots >= 1 && warps % (all / 3) == 0 && warps / (all / 3) <= PA_FED, "no room for the keys and values");
+  if (!configured[dev->device]) {
+    MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 << 10),
                   "cudaFuncSetAttribute(paged attention)");
-    int blocks = 0;
-    MIRA_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kern, warps * 32, smem), "occupancy(paged attention)");
-    fit.blocks[kind] = blocks < 1 ? 1 : (blocks > PA_MAX_BLOCKS_PER_SM ? PA_MAX_BLOCKS_PER_SM : blocks);
-    fit.smem[kind] = smem;
+    configured[dev->device] = 1;
   }
-  kern<<<unsigned(dev->sm_count * fit.blocks[kind]), warps * 32, smem, dev->stream>>>(p);
+  const int smem = pa_ring_bytes(warps * p.slots, step) + fixed + triples;
+  kern<<<unsigned(dev->sm_count * blocks), all * 32, smem, dev->stream>>>(p);
   return after_launch("paged_attention_kernel");
 }
 
 template <int DHP, int GP>
 static int launch_paged_f32(DeviceState* dev, PagedAttnParams& p) {
   using C = PaF32<DHP, GP>;
-  static PagedRingFit fits[kMaxDevices];
-  return launch_paged_ring<typename C::Ring>(dev, p, paged_attention_f32_kernel<DHP, GP>, GP, GP, DHP, 0, C::Ring::BYTES, fits);
+  static int configured[kMaxDevices] = {};
+  return launch_paged_ring(dev, p, paged_attention_f32_kernel<DHP, GP>, C::WARPS, GP, GP, DHP, C::STEP, 0, configured);
 }
 
 template <int GP>
@@ -2149,9 +2146,9 @@ static int launch_paged_f32_dh(DeviceState* dev, PagedAttnParams& p) {
 template <typename T, int DHP, int VB, int QP>
 static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
   using C = PaMma<T, DHP, VB, QP>;
-  static PagedRingFit fits[kMaxDevices];
-  return launch_paged_ring<typename C::Ring>(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP>, 16, p.group < 16 ? p.group : 16, DHP,
-                                             C::Q_BYTES, C::SCALES + C::Ring::BYTES, fits);
+  static int configured[kMaxDevices] = {};
+  return launch_paged_ring(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP>, C::WARPS, 16, p.group < 16 ? p.group : 16, DHP,
+                           C::STEP, C::Q_BYTES, configured);
 }
 
 template <typename T, int VB, int QP>

@@ -31,6 +31,7 @@ struct PagedAttnParams {
   float* lse;
   float* part;              // partial triples, two slots per block
   int* counters;            // [batch * units], zero between calls
+  int slots;                // steps in a warp's ring
 };
 
 // ---------------------------------------------------------------- dealing out the work
@@ -171,6 +172,9 @@ __device__ __forceinline__ void pa_unpack(const typename PaVec<VB>::type& raw, f
 
 // ---------------------------------------------------------------- the end of a part
 
+// Barrier among the first n threads of the block, those that compute and join.
+__device__ __forceinline__ void pa_sync(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
+
 __device__ __forceinline__ float pa_weight(float m, float top) {
   return m == -INFINITY ? 0.0f : exp2f(m - top);   // a part without a finite score weighs nothing
 }
@@ -210,15 +214,15 @@ __device__ __forceinline__ void pa_add4(float4& a, const float4& x, float w) {
 
 // Joins the warps' triples of this part (sm: one triple per warp, `rows` of them used) and either
 // writes the result, when the block had the whole unit, or leaves the joined triple in the block's
-// slot; the last block of the unit to do so joins them all.  Every thread of the block calls it.
+// slot; the last block of the unit to do so joins them all.  The block's first `warps` warps call it.
 // h0: first of the unit's `live` heads.
 template <int DHP>
-__device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork& w, float* sm, int rows, int h0, int live) {
+__device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork& w, float* sm, int warps, int rows, int h0, int live) {
   __shared__ int s_last;
-  const int warps = blockDim.x >> 5, triple = pa_triple(rows, DHP);
+  const int threads = warps * 32, triple = pa_triple(rows, DHP);
   float* j_m = sm + warps * triple;
   float* j_l = j_m + rows;
-  __syncthreads();
+  pa_sync(threads);
   if (int(threadIdx.x) < live) {
     float top = -INFINITY, sum = 0.0f;
     for (int i = 0; i < warps; ++i) top = fmaxf(top, sm[i * triple + threadIdx.x]);
@@ -231,11 +235,11 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     j_m[threadIdx.x] = top;
     j_l[threadIdx.x] = sum;
   }
-  __syncthreads();
+  pa_sync(threads);
   const int first = pa_block_of(w.total, w.us, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
   auto slot_of = [&](int64_t c) { return p.part + (c * 2 + (pa_lo(w.total, c, w.blocks) >= w.us ? 0 : 1)) * triple; };
   float* mine = slot_of(blockIdx.x);
-  for (int e = threadIdx.x; e < live * (DHP / 4); e += blockDim.x) {
+  for (int e = threadIdx.x; e < live * (DHP / 4); e += threads) {
     const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int i = 0; i < warps; ++i)
@@ -245,7 +249,7 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
   }
   if (first == last) {
     if (int(threadIdx.x) < live) pa_write_lse(p, w.b, h0 + threadIdx.x, j_m[threadIdx.x], j_l[threadIdx.x]);
-    __syncthreads();
+    pa_sync(threads);
     return;
   }
   if (int(threadIdx.x) < live) {
@@ -253,10 +257,10 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     mine[rows + threadIdx.x] = j_l[threadIdx.x];
   }
   __threadfence();
-  __syncthreads();
+  pa_sync(threads);
   int* counter = p.counters + int64_t(w.b) * p.units + w.unit;
   if (threadIdx.x == 0) s_last = atomicAdd(counter, 1) == last - first;
-  __syncthreads();
+  pa_sync(threads);
   if (s_last) {
     __threadfence();
     // all but the first part start at their block's first tile, so they are in slot 0
@@ -286,8 +290,8 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
         pa_write_lse(p, w.b, h0 + g, top, sum);
       }
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < live * (DHP / 4); e += blockDim.x) {
+    pa_sync(threads);
+    for (int e = threadIdx.x; e < live * (DHP / 4); e += threads) {
       const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
       float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       const float top = j_m[g];
@@ -307,21 +311,70 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     }
     if (threadIdx.x == 0) *counter = 0;
   }
-  __syncthreads();     // the shared triples are free again
+  pa_sync(threads);     // the shared triples are free again
 }
 
 // ---------------------------------------------------------------- rows in flight
 
-// What hides the memory's latency is bytes in flight, about 64 KB per SM at full bandwidth: more than
-// registers can hold beside the sums.  Each lane therefore copies the 16-byte pieces it will use itself
-// to its own places in shared memory (cp.async, piece j of lane l at (32 j + l) * size), a step or two
-// ahead, and reads them back when their turn comes: no bank conflicts, and nothing but the lane's own
-// wait between the copy and the use.
-template <int STAGE_BYTES, bool WIDE>      // a warp's step; WIDE: sums that need more than 168 registers
+// What hides the memory's latency is bytes in flight, about 64 KB per SM at full bandwidth, at all times:
+// also while a part is being joined and the next one begins.  A third of a block's warps therefore only
+// look rows up and copy them (cp.async, 16 bytes a lane) to shared memory, through all of the block's
+// parts.  Step k of a part is for computing warp k modulo their number; each of these has a ring of its
+// own, filled by one copying warp, so that both sides of a ring take its slots in the same order and a
+// barrier's parity always tells the round that is meant.  (With one ring for all, a warp could be two
+// rounds from another: the parity of the wrong one then passes for the right one.)  The pieces lie in
+// the order of the lanes that will use them (piece j of lane l at (32 j + l) * size), free of bank
+// conflicts.
 struct PaRing {
-  static constexpr int WARPS = STAGE_BYTES > 8192 ? 4 : WIDE ? 8 : STAGE_BYTES > 4096 ? 12 : 16;    // of an SM
-  static constexpr int STAGES = STAGE_BYTES <= 4096 ? 3 : STAGE_BYTES <= 8192 ? 2 : 3;
-  static constexpr int BYTES = STAGE_BYTES * STAGES;                                       // of a warp
+  uint8_t* steps;            // [computing warp][slot]
+  uint64_t* full;            // per slot: its copies and `live` are there
+  uint64_t* empty;           // per slot: its warp is done with it
+  uint32_t* live;            // per slot: tokens of the step that count
+  int slots;                 // of a warp
+  int* abort;                // a wait gave up: nothing is right any more, but every barrier is still met
+};
+
+// Slots have a head of 32 bytes: full, empty, live.
+__host__ __device__ constexpr int pa_ring_bytes(int slots, int step) { return slots * (step + 32); }
+
+constexpr uint64_t PA_WAIT_NS = 2000000000ull;
+
+// Every lane of the copying warp arrives on `full` when its copies have landed, and its lane 0 once more
+// for `live`; the warp that used a step arrives on `empty`.
+__device__ __forceinline__ PaRing pa_ring_at(uint8_t* at, int warps, int slots, int step, int* abort) {
+  PaRing r;
+  const int n = warps * slots;
+  r.steps = at;
+  r.full = reinterpret_cast<uint64_t*>(at + int64_t(n) * step);
+  r.empty = r.full + n;
+  r.live = reinterpret_cast<uint32_t*>(r.empty + n);
+  r.slots = slots;
+  r.abort = abort;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    mbar_init(r.full + i, 33);
+    mbar_init(r.empty + i, 1);
+  }
+  if (threadIdx.x == 0) *abort = 0;
+  fence_mbar_init();
+  __syncthreads();
+  return r;
+}
+
+__device__ __forceinline__ void pa_wait(const PaRing& r, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity) || *reinterpret_cast<volatile int*>(r.abort)) return;
+  mbar_wait(bar, parity, r.abort, PA_WAIT_NS);
+}
+
+// A place in a warp's ring: slot and the parity of its round.
+struct PaPlace {
+  int slot;
+  uint32_t round;
+  __device__ __forceinline__ void forward(int slots) {
+    if (++slot == slots) {
+      slot = 0;
+      round ^= 1;
+    }
+  }
 };
 
 // One token of a step, held by one lane: where its rows are.
@@ -343,7 +396,7 @@ __device__ __forceinline__ PaToken pa_token(const PagedAttnParams& p, const PaWo
 
 template <int BYTES>
 __device__ __forceinline__ void pa_copy(uint32_t dst, const uint8_t* src, bool ok) {
-  const uint32_t n = ok ? BYTES : 0;
+  const uint32_t n = ok ? BYTES : 0;      // 0: zeros, nothing is read
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
 }
@@ -352,6 +405,54 @@ __device__ __forceinline__ float pa_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Copying warp `me` of `feeders`: its steps of every part, step k going to copying warp k modulo their
+// number, i.e. to the rings of computing warps me, me + feeders, ..  look(w, at) finds the tokens at.. of
+// the part (a step ahead of their copies), copy(w, step) issues the copies of the tokens found last into
+// a slot and returns which of them count.
+constexpr int PA_FED = 3;      // most computing warps per copying warp
+
+template <int TILE, class Look, class Copy>
+__device__ __forceinline__ void pa_feed(const PagedAttnParams& p, PaWork& w, const PaRing& ring, int step_bytes, int me, int feeders,
+                                        int warps, Look look, Copy copy) {
+  const int lane = threadIdx.x & 31;
+  PaPlace places[PA_FED];
+#pragma unroll
+  for (int i = 0; i < PA_FED; ++i) places[i] = PaPlace{0, 0};
+  while (pa_part<TILE>(p, w)) {
+    look(w, w.t0 + me * TILE);
+    int fed = 0, to = me;       // the computing warp is `to`, the fed-th of this copying warp's
+    for (int t = w.t0 + me * TILE; t < w.t1; t += feeders * TILE) {
+      PaPlace mine = places[0];
+#pragma unroll
+      for (int i = 1; i < PA_FED; ++i)
+        if (fed == i) mine = places[i];
+      const int at = to * ring.slots + mine.slot;
+      pa_wait(ring, ring.empty + at, mine.round ^ 1);       // the first round finds every slot empty
+      __syncwarp();
+      const uint32_t live = copy(w, ring.steps + int64_t(at) * step_bytes);
+      cp_async_arrive_noinc(ring.full + at);
+      if (lane == 0) {
+        ring.live[at] = live;
+        mbar_arrive(ring.full + at);
+      }
+      mine.forward(ring.slots);
+#pragma unroll
+      for (int i = 0; i < PA_FED; ++i)
+        if (fed == i) places[i] = mine;
+      to += feeders;
+      ++fed;
+      if (to >= warps) {
+        to = me;
+        fed = 0;
+      }
+      look(w, t + feeders * TILE);
+    }
+    w.cur = w.end;
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
 }
 
 // ---------------------------------------------------------------- f32 pages
@@ -367,67 +468,64 @@ struct PaF32 {
   static constexpr int EPL = 4 * NV;
   static constexpr int TPS = 32 / LPR;
   static constexpr int U = NV > 1 ? 4 : 8;
-  static constexpr int TILE = TPS * U;                      // rows of a warp step
-  static constexpr int STAGE = 2 * U * NV * 512;
+  static constexpr int TILE = TPS * U;                      // rows of a step
+  static constexpr int STEP = 2 * U * NV * 512;
   static constexpr int N = U * GP;                          // scores of a lane group
   static constexpr int HALVINGS = N <= LPR ? (N == 4 ? 2 : N == 8 ? 3 : N == 16 ? 4 : 5) : (LPR == 8 ? 3 : LPR == 16 ? 4 : 5);
   static constexpr int LEFT = N >> HALVINGS;                // scores a lane ends up with
-  using Ring = PaRing<STAGE, false>;
+  static constexpr int WIDTH = LPR >> HALVINGS;             // lanes that end up with the same scores
+  static constexpr int WARPS = 12;                          // of an SM
 };
 
 template <int DHP, int GP>
-__global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
+__global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
     paged_attention_f32_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PaF32<DHP, GP>;
-  using Ring = typename C::Ring;
-  extern __shared__ __align__(128) uint8_t pa_ring[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  extern __shared__ __align__(128) uint8_t pa_smem[];       // ring, then the warps' triples
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, feeders = (blockDim.x >> 5) / 3, warps = (blockDim.x >> 5) - feeders;
   const int sub = lane % C::LPR, group0 = lane - sub, row0 = lane / C::LPR;
-  const uint32_t ring = smem_u32(pa_ring) + warp * Ring::BYTES + lane * 16;
-  const uint8_t* held = pa_ring + warp * Ring::BYTES + lane * 16;
+  float* sm = reinterpret_cast<float*>(pa_smem + pa_ring_bytes(warps * p.slots, C::STEP));
   PaWork w;
   if (!pa_begin<C::TILE>(p, warps, w)) return;
-  while (pa_part<C::TILE>(p, w)) {
-    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
-    const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
-    const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.k) + kvh * p.kv.kst[1] + sub * 4);
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.v) + kvh * p.kv.vst[1] + sub * 4);
+  const PaRing ring = pa_ring_at(pa_smem, warps, p.slots, C::STEP, &s_abort);
 
-    // lane i looks up row i of a step, a step before its copies are issued
+  if (warp >= warps) {
     PaToken tok;
-    uint32_t live[Ring::STAGES];        // rows of the steps in the ring that count
-    auto look = [&](int at) {
+    auto look = [&](const PaWork& w, int at) {
       int page, slot;
-      tok = pa_token<float>(p, w, trow, at + lane, lane < C::TILE, page, slot);
+      tok = pa_token<float>(p, w, p.kv.table + w.b * p.kv.table_ld, at + lane, lane < C::TILE, page, slot);
     };
-    auto issue = [&](int stage) {
-      live[Ring::STAGES - 1] = __ballot_sync(0xffffffffu, tok.ok);
-      const uint32_t dst = ring + stage * C::STAGE;
+    auto copy = [&](const PaWork& w, uint8_t* step) {
+      const int kvh = w.unit / p.head_blocks;
+      const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.k) + kvh * p.kv.kst[1] + sub * 4);
+      const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.v) + kvh * p.kv.vst[1] + sub * 4);
+      const uint32_t live = __ballot_sync(0xffffffffu, tok.ok);
+      const uint32_t dst = smem_u32(step) + lane * 16;
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
         const int i = u * C::TPS + row0;
-        const int64_t ko = __shfl_sync(0xffffffffu, tok.k, i), vo = __shfl_sync(0xffffffffu, tok.v, i);
-        const bool in = live[Ring::STAGES - 1] >> i & 1;
+        const uint8_t* k = kb + __shfl_sync(0xffffffffu, tok.k, i);
+        const uint8_t* v = vb + __shfl_sync(0xffffffffu, tok.v, i);
+        const bool in = live >> i & 1;
 #pragma unroll
         for (int j = 0; j < C::NV; ++j) {
           const bool inside = in && (sub + j * C::LPR) * 4 < p.kv.dh;
-          pa_copy<16>(dst + (u * C::NV + j) * 512, kb + ko + j * C::LPR * 16, inside);
-          pa_copy<16>(dst + ((C::U + u) * C::NV + j) * 512, vb + vo + j * C::LPR * 16, inside);
+          pa_copy<16>(dst + (u * C::NV + j) * 512, k + j * C::LPR * 16, inside);
+          pa_copy<16>(dst + ((C::U + u) * C::NV + j) * 512, v + j * C::LPR * 16, inside);
         }
       }
-      cp_async_commit();
+      return live;
     };
-    const int step = warps * C::TILE;
-    int at = w.t0 + warp * C::TILE, next = at;
-    look(next);
-#pragma unroll
-    for (int i = 0; i < Ring::STAGES - 1; ++i) {
-#pragma unroll
-      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
-      issue(i);
-      next += step;
-      look(next);
-    }
+    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, look, copy);
+    if (lane == 0 && s_abort) atomicExch(p.kv.err, 1);
+    return;
+  }
+
+  PaPlace mine{0, 0};
+  while (pa_part<C::TILE>(p, w)) {
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
+    const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
 
     float q[GP][C::EPL], acc[GP][C::EPL], m[GP], l[C::LEFT];
 #pragma unroll
@@ -445,20 +543,14 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
 #pragma unroll
     for (int i = 0; i < C::LEFT; ++i) l[i] = 0.0f;
 
-    int stage = 0, into = Ring::STAGES - 1;
-    for (; at < w.t1; at += step) {
-      cp_async_wait<Ring::STAGES - 2>();
-#pragma unroll
-      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
-      issue(into);
-      next += step;
-      look(next);
-      const uint32_t now = live[0];
-      const uint8_t* rows = held + stage * C::STAGE;
-      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
-      into = into + 1 == Ring::STAGES ? 0 : into + 1;
+    // this lane's scores are first .. first + LEFT - 1 of its group's rows, score u GP + gi
+    const int first = sub / C::WIDTH * C::LEFT;
+    for (int k = warp; k < steps; k += warps) {
+      const int slot = warp * ring.slots + mine.slot;
+      pa_wait(ring, ring.full + slot, mine.round);
+      const uint32_t now = ring.live[slot];
+      const uint8_t* rows = ring.steps + int64_t(slot) * C::STEP + lane * 16;
 
-      // scores, score u GP + gi of the lane group's rows
       float s[C::N];
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
@@ -477,7 +569,7 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
           }
         }
       }
-      // halving h: the lanes of the upper half of 2^(.. - h) keep the upper half of the scores
+      // exchange h: the lanes with bit LPR / 2^(h + 1) keep the upper half of the scores
 #pragma unroll
       for (int h = 0; h < C::HALVINGS; ++h) {
         const int o = C::LPR >> (h + 1), half = C::N >> (h + 1);
@@ -489,11 +581,9 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
         }
       }
 #pragma unroll
-      for (int o = C::LPR >> (C::HALVINGS + 1); o > 0; o >>= 1)
+      for (int o = C::WIDTH / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int i = 0; i < C::LEFT; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
-      // this lane's scores are first .. first + LEFT - 1
-      const int first = (sub >> (C::LPR == 32 ? 5 - C::HALVINGS : C::LPR == 16 ? 4 - C::HALVINGS : 3 - C::HALVINGS)) * C::LEFT;
 #pragma unroll
       for (int i = 0; i < C::LEFT; ++i) {
         const int u = (first + i) / GP;
@@ -505,12 +595,11 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
       for (int gi = 0; gi < GP; ++gi) top[gi] = m[gi];
       if (C::LEFT == 1) {
         float x = s[0];       // lanes whose score index agrees mod GP share a head
-        constexpr int SHARE = C::LPR / C::N;
 #pragma unroll
-        for (int o = C::LPR / 2; o >= GP * SHARE; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        for (int o = C::LPR / 2; o >= GP * C::WIDTH; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi)
-          top[gi] = fmaxf(top[gi], GP == 1 ? x : __shfl_sync(0xffffffffu, x, group0 + gi * SHARE));
+          top[gi] = fmaxf(top[gi], GP == 1 ? x : __shfl_sync(0xffffffffu, x, group0 + gi * C::WIDTH));
       } else {
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi) {
@@ -551,14 +640,13 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
         s[i] = pa_exp2(s[i] - (z == -INFINITY ? 0.0f : z));
         l[i] += s[i];
       }
-      constexpr int WIDTH = C::LPR >> C::HALVINGS;      // lanes that hold the same scores
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
         float pr[GP];
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi) {
           const int n = u * GP + gi;
-          pr[gi] = __shfl_sync(0xffffffffu, s[n % C::LEFT], group0 + n / C::LEFT * WIDTH);
+          pr[gi] = __shfl_sync(0xffffffffu, s[n % C::LEFT], group0 + n / C::LEFT * C::WIDTH);
         }
 #pragma unroll
         for (int j = 0; j < C::NV; ++j) {
@@ -572,14 +660,13 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ring.empty + slot);
+      mine.forward(ring.slots);
     }
-    cp_async_wait<0>();
-    __syncthreads();        // the ring becomes the place of the warps' triples
 
     // l of each head: the lanes' sums of its scores
     float lsum[GP];
-    constexpr int WIDTH = C::LPR >> C::HALVINGS;
-    const int first = sub / WIDTH * C::LEFT;
 #pragma unroll
     for (int gi = 0; gi < GP; ++gi) {
       float x = 0.0f;
@@ -587,11 +674,10 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
       for (int i = 0; i < C::LEFT; ++i)
         if ((first + i) % GP == gi) x += l[i];
 #pragma unroll
-      for (int o = WIDTH; o < C::LPR; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      for (int o = C::WIDTH; o < C::LPR; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
       lsum[gi] = x;
     }
-    float* sm = reinterpret_cast<float*>(pa_ring);
-    float* mine = sm + warp * pa_triple(GP, DHP);
+    float* to = sm + warp * pa_triple(GP, DHP);
 #pragma unroll
     for (int gi = 0; gi < GP; ++gi) {
 #pragma unroll
@@ -608,17 +694,18 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::Ring::WARPS * 32, 1)
       if (row0 == 0) {
 #pragma unroll
         for (int j = 0; j < C::NV; ++j)
-          *reinterpret_cast<float4*>(mine + pa_head(GP) + gi * DHP + (sub + j * C::LPR) * 4) =
+          *reinterpret_cast<float4*>(to + pa_head(GP) + gi * DHP + (sub + j * C::LPR) * 4) =
               make_float4(acc[gi][4 * j], acc[gi][4 * j + 1], acc[gi][4 * j + 2], acc[gi][4 * j + 3]);
       }
       if (lane == 0) {
-        mine[gi] = m[gi];
-        mine[GP + gi] = lsum[gi];
+        to[gi] = m[gi];
+        to[GP + gi] = lsum[gi];
       }
     }
-    pa_finish<DHP>(p, w, sm, GP, kvh * p.group + g0, min(GP, p.group - g0));
+    pa_finish<DHP>(p, w, sm, warps, GP, kvh * p.group + g0, min(GP, p.group - g0));
     w.cur = w.end;
   }
+  if (threadIdx.x == 0 && s_abort) atomicExch(p.kv.err, 1);
 }
 
 // ---------------------------------------------------------------- rows that are not 16-byte aligned
@@ -646,7 +733,7 @@ __global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
   using C = PaCfg<T, DHP, GP, VB>;
   using V = typename PaVec<VB>::type;
   constexpr bool I8 = sizeof(T) == 1;
-  extern __shared__ __align__(16) float pa_smem[];
+  extern __shared__ __align__(16) float pa_floats[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % C::LPR, slot_of_lane = lane / C::LPR;
   PaWork w;
@@ -768,7 +855,7 @@ __global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
     }
 
     // join the warp's lane groups
-    float* mine = pa_smem + warp * pa_triple(GP, DHP);
+    float* mine = pa_floats + warp * pa_triple(GP, DHP);
 #pragma unroll
     for (int gi = 0; gi < GP; ++gi) {
 #pragma unroll
@@ -793,7 +880,7 @@ __global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
         mine[GP + gi] = l[gi];
       }
     }
-    pa_finish<DHP>(p, w, pa_smem, GP, kvh * p.group + g0, min(GP, p.group - g0));
+    pa_finish<DHP>(p, w, pa_floats, C::WARPS, GP, kvh * p.group + g0, min(GP, p.group - g0));
     w.cur = w.end;
   }
 }

@@ -43,9 +43,8 @@ struct PaMma {
   static constexpr int PP = BF16 && QP == 3 ? 3 : 2;
   static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
   static constexpr int K_BYTES = TT * 2 * KL * 32 * VB, V_BYTES = TT * 4 * VL * 32 * VBV;    // of a step
-  using Ring = PaRing<K_BYTES + V_BYTES, (DHP > 128)>;
-  static constexpr int STAGE = K_BYTES + V_BYTES;
-  static constexpr int SCALES = I8 ? 2 * 32 * 4 * Ring::STAGES : 0;        // bytes of a warp's scales
+  static constexpr int STEP = K_BYTES + V_BYTES + (I8 ? 2 * 32 * 4 : 0);      // 8-bit pages: and the scales
+  static constexpr int WARPS = DHP <= 128 ? 12 : 8;                           // of an SM, by registers
   static constexpr int Q_BYTES = QP * KS * 32 * 16;
 };
 
@@ -89,46 +88,40 @@ __device__ __forceinline__ PaWords<BYTES / 4> pa_held(const uint8_t* p) {
 }
 
 template <typename T, int DHP, int VB, int QP>
-__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
+__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
     paged_attention_mma_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PaMma<T, DHP, VB, QP>;
-  using Ring = typename C::Ring;
-  extern __shared__ __align__(128) uint8_t pa_ring[];      // queries, then per warp its scales and ring
+  extern __shared__ __align__(128) uint8_t pa_smem[];       // ring, queries, the warps' triples
   __shared__ float s_unit[16];        // per head: what turns a product into a scaled score
-  uint4* s_q = reinterpret_cast<uint4*>(pa_ring);                  // [piece][product][lane]
-  float* s_join = reinterpret_cast<float*>(pa_ring + C::Q_BYTES);  // the warps' triples, where the rings were
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, feeders = (blockDim.x >> 5) / 3, warps = (blockDim.x >> 5) - feeders;
   const int rows = min(16, p.group);
-  float* scales = reinterpret_cast<float*>(pa_ring + C::Q_BYTES + warp * (C::SCALES + Ring::BYTES));   // [stage][k, v][token]
-  uint8_t* held = reinterpret_cast<uint8_t*>(scales) + C::SCALES;
-  const uint32_t ring = smem_u32(held);
+  uint4* s_q = reinterpret_cast<uint4*>(pa_smem + pa_ring_bytes(warps * p.slots, C::STEP));     // [piece][product][lane]
+  float* s_join = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + C::Q_BYTES);
   PaWork w;
   if (!pa_begin<C::TILE>(p, warps, w)) return;
-  while (pa_part<C::TILE>(p, w)) {
-    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * 16;
-    const int h0 = kvh * p.group + g0, live_heads = min(16, p.group - g0);
-    const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
-    const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE);
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE);
+  const PaRing ring = pa_ring_at(pa_smem, warps, p.slots, C::STEP, &s_abort);
 
-    // lane i looks up token i of a step, a step before its copies are issued
+  if (warp >= warps) {
     PaToken tok;
     int64_t ks_at = 0, vs_at = 0;
-    uint32_t live[Ring::STAGES];        // tokens of the steps in the ring that count
-    auto look = [&](int at) {
+    auto look = [&](const PaWork& w, int at) {
       int page, slot;
-      tok = pa_token<T>(p, w, trow, at + lane, lane < C::TILE, page, slot);
+      tok = pa_token<T>(p, w, p.kv.table + w.b * p.kv.table_ld, at + lane, lane < C::TILE, page, slot);
       if (C::I8) {
+        const int kvh = w.unit / p.head_blocks;
         ks_at = page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2];
         vs_at = page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2];
       }
     };
-    auto issue = [&](int stage) {
-      const uint32_t alive = __ballot_sync(0xffffffffu, tok.ok);
-      live[Ring::STAGES - 1] = alive;
-      const uint32_t kd = ring + stage * C::STAGE + lane * VB, vd = ring + stage * C::STAGE + C::K_BYTES + lane * C::VBV;
+    auto copy = [&](const PaWork& w, uint8_t* step) {
+      const int kvh = w.unit / p.head_blocks;
+      const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE);
+      const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE);
+      const uint32_t live = __ballot_sync(0xffffffffu, tok.ok);
+      const uint32_t kd = smem_u32(step) + lane * VB, vd = smem_u32(step) + C::K_BYTES + lane * C::VBV;
       if (C::I8) {
-        const uint32_t sd = smem_u32(scales) + (stage * 64 + lane) * 4;
+        const uint32_t sd = smem_u32(step) + C::K_BYTES + C::V_BYTES + lane * 4;
         pa_copy<4>(sd, reinterpret_cast<const uint8_t*>(p.kv.ks + ks_at), tok.ok);
         pa_copy<4>(sd + 128, reinterpret_cast<const uint8_t*>(p.kv.vs + vs_at), tok.ok);
       }
@@ -138,7 +131,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
         for (int n = 0; n < 2; ++n) {
           const int i = r * 16 + n * 8 + g;
           const uint8_t* row = kb + __shfl_sync(0xffffffffu, tok.k, i);
-          const bool in = alive >> i & 1;
+          const bool in = live >> i & 1;
 #pragma unroll
           for (int j = 0; j < C::KL; ++j)
             pa_copy<VB>(kd + ((r * 2 + n) * C::KL + j) * (32 * VB), row + j * 4 * VB, in && (j * 4 + t) * C::KE < p.kv.dh);
@@ -147,25 +140,24 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
         for (int n = 0; n < 4; ++n) {
           const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
           const uint8_t* row = vb + __shfl_sync(0xffffffffu, tok.v, i);
-          const bool in = alive >> i & 1;
+          const bool in = live >> i & 1;
 #pragma unroll
           for (int j = 0; j < C::VL; ++j)
             pa_copy<C::VBV>(vd + ((r * 4 + n) * C::VL + j) * (32 * C::VBV), row + j * 8 * C::VBV, in && (j * 8 + g) * C::VE < p.kv.dh);
         }
       }
-      cp_async_commit();
+      return live;
     };
-    const int step = warps * C::TILE;
-    int at = w.t0 + warp * C::TILE, next = at;
-    look(next);
-#pragma unroll
-    for (int i = 0; i < Ring::STAGES - 1; ++i) {       // before the queries: their latencies overlap
-#pragma unroll
-      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
-      issue(i);
-      next += step;
-      look(next);
-    }
+    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, look, copy);
+    if (lane == 0 && s_abort) atomicExch(p.kv.err, 1);
+    return;
+  }
+
+  PaPlace mine{0, 0};
+  while (pa_part<C::TILE>(p, w)) {
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * 16;
+    const int h0 = kvh * p.group + g0, live_heads = min(16, p.group - g0);
+    const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
 
     // queries of the unit in fragment order; a thread per (product, lane).  f16 values of a query that
     // is not f16 itself are taken after a power of two has brought its largest element to [128, 256).
@@ -185,8 +177,8 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
         s_unit[h] = unit;
       }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < C::KS * 32; i += blockDim.x) {
+    pa_sync(warps * 32);
+    for (int i = threadIdx.x; i < C::KS * 32; i += warps * 32) {
       const int ks = i >> 5, l = i & 31, lg = l >> 2, lt = l & 3;
       const int d = (ks / (C::KE / 4)) * 4 * C::KE + lt * C::KE + (ks % (C::KE / 4)) * 4;
       float x[2][4];       // head g and g + 8, elements d .. d + 3
@@ -217,7 +209,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
 #pragma unroll
       for (int q = 0; q < QP; ++q) s_q[(q * C::KS + ks) * 32 + l] = make_uint4(f[0][q], f[1][q], f[2][q], f[3][q]);
     }
-    __syncthreads();
+    pa_sync(warps * 32);
     float unit0 = s_unit[g], unit1 = s_unit[g + 8];
     if (QP == 3 && !C::BF16) {      // powers of two: the division is exact
       unit0 = p.scale_log2 / unit0;
@@ -231,30 +223,23 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
-    int stage = 0, into = Ring::STAGES - 1;
-    for (; at < w.t1; at += step) {
-      cp_async_wait<Ring::STAGES - 2>();
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k + 1 < Ring::STAGES; ++k) live[k] = live[k + 1];
-      issue(into);
-      next += step;
-      look(next);
-      const uint32_t now = live[0];
-      const uint8_t* kr = held + stage * C::STAGE + lane * VB;
-      const uint8_t* vr = held + stage * C::STAGE + C::K_BYTES + lane * C::VBV;
-      const float* sc = scales + stage * 64;
-      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
-      into = into + 1 == Ring::STAGES ? 0 : into + 1;
+    for (int k = warp; k < steps; k += warps) {
+      const int slot = warp * ring.slots + mine.slot;
+      pa_wait(ring, ring.full + slot, mine.round);
+      const uint32_t now = ring.live[slot];
+      const uint8_t* step = ring.steps + int64_t(slot) * C::STEP;
+      const uint8_t* kr = step + lane * VB;
+      const uint8_t* vr = step + C::K_BYTES + lane * C::VBV;
+      const float* sc = reinterpret_cast<const float*>(step + C::K_BYTES + C::V_BYTES);      // [k, v][token]
 
       // scores
-      float s[C::TT][2][4];
+      float s[C::TT][2][4], s2[C::TT][2][4];      // two sums each: half as many products wait for one another
 #pragma unroll
       for (int r = 0; r < C::TT; ++r)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][n][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) s[r][n][i] = s2[r][n][i] = 0.0f;
 #pragma unroll
       for (int j = 0; j < C::KL; ++j) {
         PaWords<VB / 4> kx[C::TT][2];
@@ -284,7 +269,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
 #pragma unroll
             for (int r = 0; r < C::TT; ++r)
 #pragma unroll
-              for (int n = 0; n < 2; ++n) mma_16816<C::BF16>(s[r][n], a.x, a.y, a.z, a.w, b[r][n][0], b[r][n][1]);
+              for (int n = 0; n < 2; ++n) mma_16816<C::BF16>(e & 1 ? s2[r][n] : s[r][n], a.x, a.y, a.z, a.w, b[r][n][0], b[r][n][1]);
           }
         }
       }
@@ -297,8 +282,8 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
           for (int i = 0; i < 2; ++i) {
             const bool in = now >> (r * 16 + n * 8 + 2 * t + i) & 1;
             const float ks = C::I8 ? sc[r * 16 + n * 8 + 2 * t + i] : 1.0f;
-            s[r][n][i] = in ? s[r][n][i] * (C::I8 ? unit0 * ks : unit0) : -INFINITY;
-            s[r][n][2 + i] = in ? s[r][n][2 + i] * (C::I8 ? unit1 * ks : unit1) : -INFINITY;
+            s[r][n][i] = in ? (s[r][n][i] + s2[r][n][i]) * (C::I8 ? unit0 * ks : unit0) : -INFINITY;
+            s[r][n][2 + i] = in ? (s[r][n][2 + i] + s2[r][n][2 + i]) * (C::I8 ? unit1 * ks : unit1) : -INFINITY;
             top0 = fmaxf(top0, s[r][n][i]);
             top1 = fmaxf(top1, s[r][n][2 + i]);
           }
@@ -383,10 +368,10 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ring.empty + slot);
+      mine.forward(ring.slots);
     }
-    cp_async_wait<0>();
-    __syncthreads();        // the rings become the place of the warps' triples
-
     // the warp's triple
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -395,27 +380,28 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::Ring::WARPS * 32, 1)
     }
     const float back = C::BF16 ? 1.0f : 0x1p-8f;
     const float back_v = C::I8 ? back * __int_as_float(v_exp << 23) : back;
-    float* mine = s_join + warp * pa_triple(rows, DHP);
+    float* to = s_join + warp * pa_triple(rows, DHP);
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int h = g + 8 * hh;
       if (h >= rows) continue;
       if (t == 0) {
-        mine[h] = hh ? m1 : m0;
-        mine[rows + h] = (hh ? l1 : l0) * back;
+        to[h] = hh ? m1 : m0;
+        to[rows + h] = (hh ? l1 : l0) * back;
       }
-      float* to = mine + pa_head(rows) + h * DHP;
+      float* a = to + pa_head(rows) + h * DHP;
 #pragma unroll
       for (int j = 0; j < C::VL; ++j)
 #pragma unroll
         for (int i = 0; i < C::VE; ++i) {
-          to[(j * 8 + 2 * t) * C::VE + i] = acc[j * C::VE + i][2 * hh] * back_v;
-          to[(j * 8 + 2 * t + 1) * C::VE + i] = acc[j * C::VE + i][2 * hh + 1] * back_v;
+          a[(j * 8 + 2 * t) * C::VE + i] = acc[j * C::VE + i][2 * hh] * back_v;
+          a[(j * 8 + 2 * t + 1) * C::VE + i] = acc[j * C::VE + i][2 * hh + 1] * back_v;
         }
     }
-    pa_finish<DHP>(p, w, s_join, rows, h0, live_heads);
+    pa_finish<DHP>(p, w, s_join, warps, rows, h0, live_heads);
     w.cur = w.end;
   }
+  if (threadIdx.x == 0 && s_abort) atomicExch(p.kv.err, 1);
 }
 
 }  // namespace mira
