@@ -2108,23 +2108,28 @@ static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, 
   p.units = p.kv.kv_heads * p.head_blocks;
   // One block per SM where the sequences are fewer than the SMs: each is cut into parts for many SMs,
   // and a part per SM is the least to join.  Else two, one of which works while the other's warps wait
-  // for one another at the end of a part.  Triples of many heads leave less room for the ring: then
-  // fewer warps.
+  // for one another at the end of a part.  The most warps that leave room for two steps each.
   const int blocks = int64_t(p.kv.batch) * p.units < dev->sm_count ? 1 : 2;
-  int all = sm_warps / blocks;
-  if (rows * dhp > 1024) all = all * 3 / 4;
-  const int warps = all - all / 3;        // the others copy
-  const int room = (blocks == 1 ? 225 : 111) << 10, triples = pa_finish_floats(warps, rows, dhp) * 4;
-  p.slots = (room - fixed - triples) / (warps * (step + 32));
+  const int room = (blocks == 1 ? 225 : 111) << 10;
+  static const int splits[][2] = {{12, 4}, {8, 4}, {6, 3}, {6, 2}, {4, 2}, {3, 1}, {2, 1}};      // computing, copying
+  int warps = 0, triples = 0;
+  for (const auto& split : splits) {
+    if (split[0] + split[1] > sm_warps / blocks) continue;
+    warps = split[0];
+    p.feeders = split[1];
+    triples = pa_finish_floats(warps, rows, dhp) * 4;
+    p.slots = (room - fixed - triples) / (warps * (step + 32));
+    if (p.slots >= 2) break;
+  }
   if (p.slots > 4) p.slots = 4;
-  MIRA_CHECK_ARG(p.slots >= 1 && warps % (all / 3) == 0 && warps / (all / 3) <= PA_FED, "no room for the keys and values");
+  MIRA_CHECK_ARG(p.slots >= 1, "no room for the keys and values");
   if (!configured[dev->device]) {
     MIRA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 << 10),
                   "cudaFuncSetAttribute(paged attention)");
     configured[dev->device] = 1;
   }
   const int smem = pa_ring_bytes(warps * p.slots, step) + fixed + triples;
-  kern<<<unsigned(dev->sm_count * blocks), all * 32, smem, dev->stream>>>(p);
+  kern<<<unsigned(dev->sm_count * blocks), (warps + p.feeders) * 32, smem, dev->stream>>>(p);
   return after_launch("paged_attention_kernel");
 }
 
@@ -2143,19 +2148,19 @@ static int launch_paged_f32_dh(DeviceState* dev, PagedAttnParams& p) {
   return launch_paged_f32<256, GP>(dev, p);
 }
 
-template <typename T, int DHP, int VB, int QP>
+template <typename T, int DHP, int VB, int QP, int NH>
 static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
-  using C = PaMma<T, DHP, VB, QP>;
+  using C = PaMma<T, DHP, VB, QP, NH>;
   static int configured[kMaxDevices] = {};
-  return launch_paged_ring(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP>, C::WARPS, 16, p.group < 16 ? p.group : 16, DHP,
-                           C::STEP, C::Q_BYTES, configured);
+  return launch_paged_ring(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP, NH>, C::WARPS, 8 * NH,
+                           p.group < 8 * NH ? p.group : 8 * NH, DHP, C::STEP, C::Q_BYTES, configured);
 }
 
 template <typename T, int VB, int QP>
 static int launch_paged_mma_dh(DeviceState* dev, PagedAttnParams& p) {
-  if (p.kv.dh <= 64) return launch_paged_mma<T, 64, VB, QP>(dev, p);
-  if (p.kv.dh <= 128) return launch_paged_mma<T, 128, VB, QP>(dev, p);
-  return launch_paged_mma<T, 256, VB, QP>(dev, p);
+  if (p.kv.dh <= 64) return p.group <= 8 ? launch_paged_mma<T, 64, VB, QP, 1>(dev, p) : launch_paged_mma<T, 64, VB, QP, 2>(dev, p);
+  if (p.kv.dh <= 128) return p.group <= 8 ? launch_paged_mma<T, 128, VB, QP, 1>(dev, p) : launch_paged_mma<T, 128, VB, QP, 2>(dev, p);
+  return p.group <= 8 ? launch_paged_mma<T, 256, VB, QP, 1>(dev, p) : launch_paged_mma<T, 256, VB, QP, 2>(dev, p);
 }
 
 template <typename T, int VB>

@@ -31,7 +31,7 @@ struct PagedAttnParams {
   float* lse;
   float* part;              // partial triples, two slots per block
   int* counters;            // [batch * units], zero between calls
-  int slots;                // steps in a warp's ring
+  int slots, feeders;       // steps in a warp's ring, copying warps of a block
 };
 
 // ---------------------------------------------------------------- dealing out the work
@@ -317,8 +317,8 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
 // ---------------------------------------------------------------- rows in flight
 
 // What hides the memory's latency is bytes in flight, about 64 KB per SM at full bandwidth, at all times:
-// also while a part is being joined and the next one begins.  A third of a block's warps therefore only
-// look rows up and copy them (cp.async, 16 bytes a lane) to shared memory, through all of the block's
+// also while a part is being joined and the next one begins.  A quarter to a third of a block's warps
+// therefore only look rows up and copy them (cp.async, 16 bytes a lane) to shared memory, through all of the block's
 // parts.  Step k of a part is for computing warp k modulo their number; each of these has a ring of its
 // own, filled by one copying warp, so that both sides of a ring take its slots in the same order and a
 // barrier's parity always tells the round that is meant.  (With one ring for all, a warp could be two
@@ -474,7 +474,7 @@ struct PaF32 {
   static constexpr int HALVINGS = N <= LPR ? (N == 4 ? 2 : N == 8 ? 3 : N == 16 ? 4 : 5) : (LPR == 8 ? 3 : LPR == 16 ? 4 : 5);
   static constexpr int LEFT = N >> HALVINGS;                // scores a lane ends up with
   static constexpr int WIDTH = LPR >> HALVINGS;             // lanes that end up with the same scores
-  static constexpr int WARPS = 12;                          // of an SM
+  static constexpr int WARPS = GP * EPL <= 8 ? 16 : 12;     // of an SM
 };
 
 template <int DHP, int GP>
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
   using C = PaF32<DHP, GP>;
   extern __shared__ __align__(128) uint8_t pa_smem[];       // ring, then the warps' triples
   __shared__ int s_abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, feeders = (blockDim.x >> 5) / 3, warps = (blockDim.x >> 5) - feeders;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, feeders = p.feeders, warps = (blockDim.x >> 5) - feeders;
   const int sub = lane % C::LPR, group0 = lane - sub, row0 = lane / C::LPR;
   float* sm = reinterpret_cast<float*>(pa_smem + pa_ring_bytes(warps * p.slots, C::STEP));
   PaWork w;

@@ -1,16 +1,17 @@
 // Paged attention of one token per sequence on the tensor path, for 16-bit and 8-bit pages.
 //
 // Bound: the visible keys and values are read once; an SM's share of the memory bandwidth is about 23
-// bytes a clock.  The group's heads are the 16 rows of the products, so a key costs the same few
-// instructions for one head as for sixteen, and what remains is unpacking, addresses and the softmax.
-//
-// No fragment crosses lanes: the sums over k of a product do not care in which order k comes, so a
-// lane's 16-byte piece of a row, as it arrives from memory, is its share of a fragment.
-//   S = Q K^T: lane (g, t) holds token g's elements VE t .. VE t + VE - 1 of each run of 4 VE: four of
-//     them are the right operand of one 16x8x16 product; Q is laid out to match, once per unit.
-//   O += P V: lane (g, t) holds elements VE g .. of each run of 8 VE of the tokens 2t, 2t + 1, 2t + 8 and
-//     2t + 9; pairs of tokens of one element, one byte permutation each, are the right operand, column g
-//     of tile i being element VE g + i; P's accumulators are already the left operand's layout.
+// bytes a clock, a step of 8 KB every 360 clocks.  The keys are the products' left operand, 16 tokens, and
+// the heads that share them its eight columns (twice eight for groups of more than 8), so that the
+// products, the softmax and the sums cost the same for one head as for eight, and little more than the
+// unpacking, the addresses and the waiting.
+//   S^T = K Q^T: lane (g, t) holds elements VE t .. VE t + VE - 1 of each run of 4 VE of tokens g and g + 8,
+//     16 bytes as they came from memory: four elements of each are a left fragment.  The sums over k do
+//     not care in which order k comes; Q is laid out to match, once per unit.
+//   O^T += V^T P^T: lane (g, t) holds elements VE g .. of each run of 8 VE of tokens 2t, 2t + 1, 2t + 8 and
+//     2t + 9; pairs of tokens of one element, a byte permutation each, are left fragments with rows
+//     (element i, g) and (element i + 1, g).  P^T is S^T's accumulators, packed and transposed in 8 x 8
+//     blocks by movmatrix.
 // Exactness: q enters as one value of the pages' type where it has that type, else as three whose sum
 // it is; 8-bit codes become exact f16 values.  p is f32 and enters as PP values that agree with it to 16
 // bits or more (see PaMma), the row's sum l is of the f32 values.
@@ -23,8 +24,8 @@
 namespace mira {
 
 // T: the pages' element; DHP: head dimension rounded up to 64, 128 or 256; VB: bytes per access of a
-// key row; QP: values per query element, 1 or 3.
-template <typename T, int DHP, int VB, int QP>
+// key row; QP: values per query element, 1 or 3; NH: blocks of eight heads.
+template <typename T, int DHP, int VB, int QP, int NH>
 struct PaMma {
   static constexpr bool I8 = sizeof(T) == 1;
   static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;      // else the products are f16
@@ -34,9 +35,9 @@ struct PaMma {
   static constexpr int VBV = VB < DHP * int(sizeof(T)) / 8 ? VB : DHP * int(sizeof(T)) / 8;
   static constexpr int VE = VBV / int(sizeof(T));
   static constexpr int VL = DHP / (8 * VE);                                // value accesses per token
-  static constexpr int NT = DHP / 8;                                       // tiles of O
+  static constexpr int NT = DHP / 16;                                      // tiles of O
   static constexpr int TT = (DHP * int(sizeof(T)) <= 128) ? 2 : 1;         // runs of 16 tokens per step
-  static constexpr int TILE = 16 * TT;                                     // tokens of a warp step
+  static constexpr int TILE = 16 * TT;                                     // tokens of a step
   // p: bf16 values have 8 bits, f16 ones 11.  16-bit results: 16 and 22 bits; f32 results (QP == 3): 24
   // and 22, whose error of 2^-22 of the largest weight is that of an f32 sum of a few terms.  In f16,
   // p is carried times 2^8: the smallest f16 is then 2^-32 of the largest weight.
@@ -44,9 +45,17 @@ struct PaMma {
   static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
   static constexpr int K_BYTES = TT * 2 * KL * 32 * VB, V_BYTES = TT * 4 * VL * 32 * VBV;    // of a step
   static constexpr int STEP = K_BYTES + V_BYTES + (I8 ? 2 * 32 * 4 : 0);      // 8-bit pages: and the scales
-  static constexpr int WARPS = DHP <= 128 ? 12 : 8;                           // of an SM, by registers
-  static constexpr int Q_BYTES = QP * KS * 32 * 16;
+  // warps of an SM, by the registers of the sums and by the ring: a computing warp wants two steps of it
+  static constexpr int WARPS = STEP > 9000 || NH * DHP > 256 ? 6 : NH * DHP <= 128 ? 16 : 12;
+  static constexpr int Q_BYTES = NH * QP * KS * 32 * 8;
 };
+
+// The 8 x 8 block of 16-bit values whose row g lane (g, t) holds columns 2t, 2t + 1 of, transposed.
+__device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
 // x = a + b (+ c) in 16-bit values, pairs packed.
 template <bool BF16, int N>
@@ -87,16 +96,16 @@ __device__ __forceinline__ PaWords<BYTES / 4> pa_held(const uint8_t* p) {
   return r;
 }
 
-template <typename T, int DHP, int VB, int QP>
-__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
+template <typename T, int DHP, int VB, int QP, int NH>
+__global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
     paged_attention_mma_kernel(const __grid_constant__ PagedAttnParams p) {
-  using C = PaMma<T, DHP, VB, QP>;
+  using C = PaMma<T, DHP, VB, QP, NH>;
   extern __shared__ __align__(128) uint8_t pa_smem[];       // ring, queries, the warps' triples
-  __shared__ float s_unit[16];        // per head: what turns a product into a scaled score
+  __shared__ float s_unit[8 * NH];        // per head: what turns a product into a scaled score
   __shared__ int s_abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, feeders = (blockDim.x >> 5) / 3, warps = (blockDim.x >> 5) - feeders;
-  const int rows = min(16, p.group);
-  uint4* s_q = reinterpret_cast<uint4*>(pa_smem + pa_ring_bytes(warps * p.slots, C::STEP));     // [piece][product][lane]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, feeders = p.feeders, warps = (blockDim.x >> 5) - feeders;
+  const int rows = min(8 * NH, p.group);
+  uint2* s_q = reinterpret_cast<uint2*>(pa_smem + pa_ring_bytes(warps * p.slots, C::STEP));     // [piece][heads][product][lane]
   float* s_join = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + C::Q_BYTES);
   PaWork w;
   if (!pa_begin<C::TILE>(p, warps, w)) return;
@@ -155,13 +164,13 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
 
   PaPlace mine{0, 0};
   while (pa_part<C::TILE>(p, w)) {
-    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * 16;
-    const int h0 = kvh * p.group + g0, live_heads = min(16, p.group - g0);
+    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * (8 * NH);
+    const int h0 = kvh * p.group + g0, live_heads = min(8 * NH, p.group - g0);
     const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
 
     // queries of the unit in fragment order; a thread per (product, lane).  f16 values of a query that
     // is not f16 itself are taken after a power of two has brought its largest element to [128, 256).
-    for (int h = warp; h < 16; h += warps) {
+    for (int h = warp; h < 8 * NH; h += warps) {
       float unit = p.scale_log2;
       if (QP == 3 && !C::BF16) {
         float top = 0.0f;
@@ -178,50 +187,52 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
       }
     }
     pa_sync(warps * 32);
-    for (int i = threadIdx.x; i < C::KS * 32; i += warps * 32) {
-      const int ks = i >> 5, l = i & 31, lg = l >> 2, lt = l & 3;
+    for (int i = threadIdx.x; i < NH * C::KS * 32; i += warps * 32) {
+      const int l = i & 31, lt = l & 3, ks = (i >> 5) % C::KS, h = (i >> 5) / C::KS * 8 + (l >> 2);
       const int d = (ks / (C::KE / 4)) * 4 * C::KE + lt * C::KE + (ks % (C::KE / 4)) * 4;
-      float x[2][4];       // head g and g + 8, elements d .. d + 3
+      float x[4];       // elements d .. d + 3 of head h
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = lg + 8 * hh;
-          float v = h < live_heads && d + e < p.kv.dh
-              ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + (d + e) * p.qs[2], p.q_dtype) : 0.0f;
-          if (QP == 3 && !C::BF16) v *= s_unit[h];
-          x[hh][e] = v;
-        }
-      uint32_t f[4][QP];
+      for (int e = 0; e < 4; ++e) {
+        x[e] = h < live_heads && d + e < p.kv.dh
+            ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + (d + e) * p.qs[2], p.q_dtype) : 0.0f;
+        if (QP == 3 && !C::BF16) x[e] *= s_unit[h];
+      }
+      uint32_t f[2][QP];
       if (C::BF16 && QP == 3) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           uint32_t a[3], b[3];
-          split3_bf16(x[j & 1][(j >> 1) * 2], a[0], a[1], a[2]);
-          split3_bf16(x[j & 1][(j >> 1) * 2 + 1], b[0], b[1], b[2]);
+          split3_bf16(x[2 * j], a[0], a[1], a[2]);
+          split3_bf16(x[2 * j + 1], b[0], b[1], b[2]);
 #pragma unroll
           for (int q = 0; q < QP; ++q) f[j][q] = __byte_perm(a[q], b[q], 0x7632);
         }
       } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pa_split2<C::BF16, QP>(x[j & 1][(j >> 1) * 2], x[j & 1][(j >> 1) * 2 + 1], f[j]);
+        pa_split2<C::BF16, QP>(x[0], x[1], f[0]);
+        pa_split2<C::BF16, QP>(x[2], x[3], f[1]);
       }
 #pragma unroll
-      for (int q = 0; q < QP; ++q) s_q[(q * C::KS + ks) * 32 + l] = make_uint4(f[0][q], f[1][q], f[2][q], f[3][q]);
+      for (int q = 0; q < QP; ++q) s_q[q * (NH * C::KS * 32) + i] = make_uint2(f[0][q], f[1][q]);
     }
     pa_sync(warps * 32);
-    float unit0 = s_unit[g], unit1 = s_unit[g + 8];
-    if (QP == 3 && !C::BF16) {      // powers of two: the division is exact
-      unit0 = p.scale_log2 / unit0;
-      unit1 = p.scale_log2 / unit1;
-    }
-
-    float acc[C::NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    // this lane's heads are 8 b + 2t + i
+    float unit[NH][2], m[NH][2], l[NH][2], acc[C::NT][NH][4];
+#pragma unroll
+    for (int b = 0; b < NH; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        unit[b][i] = s_unit[8 * b + 2 * t + i];
+        if (QP == 3 && !C::BF16) unit[b][i] = p.scale_log2 / unit[b][i];      // a power of two: exact
+        m[b][i] = -INFINITY;
+        l[b][i] = 0.0f;
+      }
     uint32_t v_exp = 1;       // 8-bit pages: exponent of the largest value scale so far, which acc is divided by
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+      for (int b = 0; b < NH; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][b][i] = 0.0f;
 
     for (int k = warp; k < steps; k += warps) {
       const int slot = warp * ring.slots + mine.slot;
@@ -232,16 +243,18 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
       const uint8_t* vr = step + C::K_BYTES + lane * C::VBV;
       const float* sc = reinterpret_cast<const float*>(step + C::K_BYTES + C::V_BYTES);      // [k, v][token]
 
-      // scores
-      float s[C::TT][2][4], s2[C::TT][2][4];      // two sums each: half as many products wait for one another
+      // scores of tokens 16 r + g (values 0, 1) and + 8 (2, 3); two sums each, so that half as many
+      // products wait for one another
+      float s[C::TT][NH][4], s2[C::TT][NH][4];
 #pragma unroll
       for (int r = 0; r < C::TT; ++r)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int b = 0; b < NH; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][n][i] = s2[r][n][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) s[r][b][i] = s2[r][b][i] = 0.0f;
 #pragma unroll
       for (int j = 0; j < C::KL; ++j) {
+        if (j * 4 * C::KE >= p.kv.dh) break;
         PaWords<VB / 4> kx[C::TT][2];
 #pragma unroll
         for (int r = 0; r < C::TT; ++r)
@@ -249,49 +262,49 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
           for (int n = 0; n < 2; ++n) kx[r][n] = pa_held<VB>(kr + ((r * 2 + n) * C::KL + j) * (32 * VB));
 #pragma unroll
         for (int e = 0; e < C::KE / 4; ++e) {
-          uint32_t b[C::TT][2][2];
+          uint32_t a[C::TT][4];
 #pragma unroll
           for (int r = 0; r < C::TT; ++r)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               if (C::I8) {
                 const uint32_t x = kx[r][n].w[e] ^ 0x80808080u;
-                b[r][n][0] = pa_codes(x, 0x4140);
-                b[r][n][1] = pa_codes(x, 0x4342);
+                a[r][n] = pa_codes(x, 0x4140);
+                a[r][2 + n] = pa_codes(x, 0x4342);
               } else {
-                b[r][n][0] = kx[r][n].w[(2 * e) % (VB / 4)];
-                b[r][n][1] = kx[r][n].w[(2 * e + 1) % (VB / 4)];
+                a[r][n] = kx[r][n].w[(2 * e) % (VB / 4)];
+                a[r][2 + n] = kx[r][n].w[(2 * e + 1) % (VB / 4)];
               }
             }
 #pragma unroll
-          for (int q = QP - 1; q >= 0; --q) {
-            const uint4 a = s_q[(q * C::KS + j * (C::KE / 4) + e) * 32 + lane];
+          for (int q = QP - 1; q >= 0; --q)
 #pragma unroll
-            for (int r = 0; r < C::TT; ++r)
+            for (int b = 0; b < NH; ++b) {
+              const uint2 y = s_q[((q * NH + b) * C::KS + j * (C::KE / 4) + e) * 32 + lane];
 #pragma unroll
-              for (int n = 0; n < 2; ++n) mma_16816<C::BF16>(e & 1 ? s2[r][n] : s[r][n], a.x, a.y, a.z, a.w, b[r][n][0], b[r][n][1]);
-          }
+              for (int r = 0; r < C::TT; ++r)
+                mma_16816<C::BF16>(e & 1 ? s2[r][b] : s[r][b], a[r][0], a[r][1], a[r][2], a[r][3], y.x, y.y);
+            }
         }
       }
-      float top0 = m0, top1 = m1;
+      float top[NH][2];
 #pragma unroll
-      for (int r = 0; r < C::TT; ++r)
+      for (int b = 0; b < NH; ++b)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int i = 0; i < 2; ++i) {
+          top[b][i] = m[b][i];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const bool in = now >> (r * 16 + n * 8 + 2 * t + i) & 1;
-            const float ks = C::I8 ? sc[r * 16 + n * 8 + 2 * t + i] : 1.0f;
-            s[r][n][i] = in ? (s[r][n][i] + s2[r][n][i]) * (C::I8 ? unit0 * ks : unit0) : -INFINITY;
-            s[r][n][2 + i] = in ? (s[r][n][2 + i] + s2[r][n][2 + i]) * (C::I8 ? unit1 * ks : unit1) : -INFINITY;
-            top0 = fmaxf(top0, s[r][n][i]);
-            top1 = fmaxf(top1, s[r][n][2 + i]);
-          }
+          for (int r = 0; r < C::TT; ++r)
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
-        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
-      }
+            for (int n = 0; n < 2; ++n) {
+              const int token = r * 16 + n * 8 + g;
+              float& x = s[r][b][2 * n + i];
+              x = now >> token & 1 ? (x + s2[r][b][2 * n + i]) * (C::I8 ? unit[b][i] * sc[token] : unit[b][i]) : -INFINITY;
+              top[b][i] = fmaxf(top[b][i], x);
+            }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top[b][i] = fmaxf(top[b][i], __shfl_xor_sync(0xffffffffu, top[b][i], o));
+        }
       float grow = 1.0f, shrink = 1.0f;
       if (C::I8) {
         const float vscale = lane < C::TILE && (now >> lane & 1) ? sc[32 + lane] : 0.0f;
@@ -300,71 +313,78 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
         v_exp = e;
         shrink = __int_as_float((254 - e) << 23);
       }
-      const float safe0 = top0 == -INFINITY ? 0.0f : top0, safe1 = top1 == -INFINITY ? 0.0f : top1;
-      if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1 || grow != 1.0f)) {
-        const float f0 = pa_exp2(m0 - safe0), f1 = pa_exp2(m1 - safe1);
-        m0 = top0;
-        m1 = top1;
-        l0 *= f0;
-        l1 *= f1;
+      bool moved = grow != 1.0f;
 #pragma unroll
-        for (int n = 0; n < C::NT; ++n) {
-          acc[n][0] *= f0 * grow;
-          acc[n][1] *= f0 * grow;
-          acc[n][2] *= f1 * grow;
-          acc[n][3] *= f1 * grow;
-        }
+      for (int b = 0; b < NH; ++b) moved = moved || top[b][0] > m[b][0] || top[b][1] > m[b][1];
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int b = 0; b < NH; ++b)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float f = pa_exp2(m[b][i] - (top[b][i] == -INFINITY ? 0.0f : top[b][i]));
+            m[b][i] = top[b][i];
+            l[b][i] *= f;
+#pragma unroll
+            for (int n = 0; n < C::NT; ++n) {
+              acc[n][b][i] *= f * grow;
+              acc[n][b][2 + i] *= f * grow;
+            }
+          }
       }
-      const float z0 = safe0 - C::SHIFT, z1 = safe1 - C::SHIFT;
 #pragma unroll
       for (int r = 0; r < C::TT; ++r) {
-        uint32_t a[4][C::PP];
+        uint32_t pt[NH][2][C::PP];       // P^T: tokens 2t, 2t + 1 (+ 8) of head g
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float x0 = pa_exp2(s[r][n][0] - z0), x1 = pa_exp2(s[r][n][1] - z0);
-          float y0 = pa_exp2(s[r][n][2] - z1), y1 = pa_exp2(s[r][n][3] - z1);
-          l0 += x0 + x1;
-          l1 += y0 + y1;
-          if (C::I8) {
-            const int i = r * 16 + n * 8 + 2 * t;       // a token that does not count has no scale either
-            const float u0 = now >> i & 1 ? sc[32 + i] * shrink : 0.0f, u1 = now >> (i + 1) & 1 ? sc[33 + i] * shrink : 0.0f;
-            x0 *= u0;
-            x1 *= u1;
-            y0 *= u0;
-            y1 *= u1;
+        for (int b = 0; b < NH; ++b)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            float x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              x[i] = pa_exp2(s[r][b][2 * n + i] - ((m[b][i] == -INFINITY ? 0.0f : m[b][i]) - C::SHIFT));
+              l[b][i] += x[i];
+              if (C::I8) {       // a token that does not count has no scale either
+                const int token = r * 16 + n * 8 + g;
+                x[i] *= now >> token & 1 ? sc[32 + token] * shrink : 0.0f;
+              }
+            }
+            pa_split2<C::BF16, C::PP>(x[0], x[1], pt[b][n]);
+#pragma unroll
+            for (int q = 0; q < C::PP; ++q) pt[b][n][q] = pa_transpose(pt[b][n][q]);
           }
-          pa_split2<C::BF16, C::PP>(x0, x1, a[2 * n]);
-          pa_split2<C::BF16, C::PP>(y0, y1, a[2 * n + 1]);
-        }
 #pragma unroll
         for (int j = 0; j < C::VL; ++j) {
+          if (j * 8 * C::VE >= p.kv.dh) break;
           PaWords<C::VBV / 4> vx[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) vx[n] = pa_held<C::VBV>(vr + ((r * 4 + n) * C::VL + j) * (32 * C::VBV));
 #pragma unroll
           for (int e = 0; e < C::VBV / 4; ++e) {
             constexpr int PER = 4 / int(sizeof(T));      // elements of a word
-            uint32_t b[PER][2];
+            uint32_t a[PER][2];                          // element, tokens 2t, 2t + 1 (+ 8)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t x = vx[2 * h].w[e], y = vx[2 * h + 1].w[e];
               if (C::I8) {
                 const uint32_t bx = x ^ 0x80808080u, by = y ^ 0x80808080u;
                 const uint32_t low = __byte_perm(bx, by, 0x5140), high = __byte_perm(bx, by, 0x7362);
-                b[0][h] = pa_codes(low, 0x4140);
-                b[1][h] = pa_codes(low, 0x4342);
-                b[2 % PER][h] = pa_codes(high, 0x4140);
-                b[3 % PER][h] = pa_codes(high, 0x4342);
+                a[0][h] = pa_codes(low, 0x4140);
+                a[1][h] = pa_codes(low, 0x4342);
+                a[2 % PER][h] = pa_codes(high, 0x4140);
+                a[3 % PER][h] = pa_codes(high, 0x4342);
               } else {
-                b[0][h] = __byte_perm(x, y, 0x5410);
-                b[1][h] = __byte_perm(x, y, 0x7632);
+                a[0][h] = __byte_perm(x, y, 0x5410);
+                a[1][h] = __byte_perm(x, y, 0x7632);
               }
             }
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
+            for (int i = 0; i < PER / 2; ++i)
 #pragma unroll
-              for (int q = C::PP - 1; q >= 0; --q)
-                mma_16816<C::BF16>(acc[j * C::VE + e * PER + i], a[0][q], a[1][q], a[2][q], a[3][q], b[i][0], b[i][1]);
+              for (int b = 0; b < NH; ++b)
+#pragma unroll
+                for (int q = C::PP - 1; q >= 0; --q)
+                  mma_16816<C::BF16>(acc[(j * C::VE + e * PER) / 2 + i][b], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1],
+                                     pt[b][0][q], pt[b][1][q]);
           }
         }
       }
@@ -372,32 +392,32 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP>::WARPS * 32, 1)
       if (lane == 0) mbar_arrive(ring.empty + slot);
       mine.forward(ring.slots);
     }
+
     // the warp's triple
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-    }
     const float back = C::BF16 ? 1.0f : 0x1p-8f;
     const float back_v = C::I8 ? back * __int_as_float(v_exp << 23) : back;
     float* to = s_join + warp * pa_triple(rows, DHP);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int h = g + 8 * hh;
-      if (h >= rows) continue;
-      if (t == 0) {
-        to[h] = hh ? m1 : m0;
-        to[rows + h] = (hh ? l1 : l0) * back;
-      }
-      float* a = to + pa_head(rows) + h * DHP;
+    for (int b = 0; b < NH; ++b)
 #pragma unroll
-      for (int j = 0; j < C::VL; ++j)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int i = 0; i < C::VE; ++i) {
-          a[(j * 8 + 2 * t) * C::VE + i] = acc[j * C::VE + i][2 * hh] * back_v;
-          a[(j * 8 + 2 * t + 1) * C::VE + i] = acc[j * C::VE + i][2 * hh + 1] * back_v;
+        for (int o = 4; o < 32; o <<= 1) l[b][i] += __shfl_xor_sync(0xffffffffu, l[b][i], o);
+        const int h = 8 * b + 2 * t + i;
+        if (h >= rows) continue;
+        if (g == 0) {
+          to[h] = m[b][i];
+          to[rows + h] = l[b][i] * back;
         }
-    }
+        // tile n: elements 2 n and 2 n + 1 of the lane's runs
+        float* a = to + pa_head(rows) + h * DHP;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) {
+          const int d = ((2 * n) / C::VE * 8 + g) * C::VE + (2 * n) % C::VE;
+          a[d] = acc[n][b][i] * back_v;
+          a[d + 1] = acc[n][b][2 + i] * back_v;
+        }
+      }
     pa_finish<DHP>(p, w, s_join, warps, rows, h0, live_heads);
     w.cur = w.end;
   }
