@@ -54,8 +54,12 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedAttnParams& p, int b) {
   return s;
 }
 
-// The tiles of all (sequence, unit) pairs form one line of `total` tiles, sequence by sequence and
-// unit by unit; block c of g takes [total c / g, total (c + 1) / g).
+// The tiles of all (sequence, unit) pairs form one line of length `total`, sequence by sequence and unit
+// by unit; block c of g takes [total c / g, total (c + 1) / g).  Before its tiles each unit has an empty
+// stretch of PA_PART_COST: a part's beginning and end take a block as long as about that many tiles, and
+// without it the blocks that get many short sequences finish last (64 sequences of 16 to 1024 tokens: the
+// last block at twice the median's time).
+constexpr int PA_PART_COST = 8;
 __device__ __forceinline__ int64_t pa_lo(int64_t total, int64_t c, int64_t g) { return total * c / g; }
 __device__ __forceinline__ int pa_block_of(int64_t total, int64_t x, int64_t g) {
   return static_cast<int>(((x + 1) * g - 1) / total);
@@ -84,16 +88,16 @@ __device__ __forceinline__ int64_t pa_scan(int64_t v, int64_t& before, int64_t* 
 
 // A block's share of the line, and the part of a unit at its front.
 struct PaWork {
-  int64_t total, blocks;       // tiles, and blocks that share them
-  int64_t lo, hi;              // this block's
-  int64_t cur;                 // first tile not done yet
-  int b;                       // its sequence
-  int64_t base;                // first tile of that sequence
+  int64_t total, blocks;       // the line, and blocks that share it
+  int64_t lo, hi;              // this block's share
+  int64_t cur;                 // what is done of it
+  int b;                       // the sequence there
+  int64_t base;                // its first place
   PaSeq seq;
-  // the part: unit and its tiles [us, ue), of which this block does those up to `end`; visible positions
-  // [t0, t1)
+  // the part: unit and its tiles' places [ts, ue), of which this block does those up to `end`; visible
+  // positions [t0, t1)
   int unit;
-  int64_t us, ue, end;
+  int64_t ts, ue, end;
   int t0, t1;
 };
 
@@ -103,28 +107,29 @@ template <int TILE>
 __device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, PaWork& w) {
   __shared__ int64_t s_scan[PA_MAX_WARPS];
   __shared__ int64_t s_found[2];
-  int64_t total = 0;
+  auto length = [&](int b) { return b < p.kv.batch ? int64_t(pa_seq<TILE>(p, b).tiles + PA_PART_COST) * p.units : 0; };
+  // where the sequence of this thread begins (of the last chunk of sequences, if there are many)
+  int64_t mine = 0, before = 0, sum = 0;
+  w.total = 0;
   for (int b0 = 0; b0 < p.kv.batch; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    int64_t before;
-    total += pa_scan(b < p.kv.batch ? pa_seq<TILE>(p, b).tiles : 0, before, s_scan);
+    mine = length(b0 + threadIdx.x);
+    sum = pa_scan(mine, before, s_scan);
+    w.total += sum;
   }
-  w.total = total * p.units;
-  const int64_t apart = max(int64_t(p.kv.batch) * p.units, (w.total + least - 1) / least);
+  const int64_t apart = max(int64_t(p.kv.batch) * p.units, w.total / least);
   w.blocks = min(min(int64_t(gridDim.x), w.total), apart);
   if (blockIdx.x >= w.blocks) return false;
   w.lo = w.cur = pa_lo(w.total, blockIdx.x, w.blocks);
   w.hi = pa_lo(w.total, blockIdx.x + 1, w.blocks);
   int64_t run = 0;
   for (int b0 = 0; b0 < p.kv.batch; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    const int64_t mine = b < p.kv.batch ? int64_t(pa_seq<TILE>(p, b).tiles) * p.units : 0;
-    int64_t before;
-    const int64_t sum = pa_scan(mine, before, s_scan);
-    before += run;
-    if (mine > 0 && before <= w.lo && w.lo < before + mine) {
-      s_found[0] = b;
-      s_found[1] = before;
+    if (p.kv.batch > int(blockDim.x)) {
+      mine = length(b0 + threadIdx.x);
+      sum = pa_scan(mine, before, s_scan);
+    }
+    if (run + before <= w.lo && w.lo < run + before + mine) {
+      s_found[0] = b0 + threadIdx.x;
+      s_found[1] = run + before;
     }
     run += sum;
   }
@@ -137,18 +142,28 @@ __device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, Pa
 
 template <int TILE>
 __device__ __forceinline__ bool pa_part(const PagedAttnParams& p, PaWork& w) {
-  if (w.cur >= w.hi) return false;
-  while (w.cur >= w.base + int64_t(w.seq.tiles) * p.units) {
-    w.base += int64_t(w.seq.tiles) * p.units;
-    w.seq = pa_seq<TILE>(p, ++w.b);
+  while (w.cur < w.hi) {
+    int64_t per = w.seq.tiles + PA_PART_COST;
+    while (w.cur >= w.base + per * p.units) {
+      w.base += per * p.units;
+      w.seq = pa_seq<TILE>(p, ++w.b);
+      per = w.seq.tiles + PA_PART_COST;
+    }
+    const int64_t in = w.cur - w.base;
+    w.unit = in <= int64_t(UINT32_MAX) ? int(uint32_t(in) / uint32_t(per)) : int(in / per);
+    const int64_t us = w.base + w.unit * per;
+    w.ts = us + PA_PART_COST;
+    w.ue = us + per;
+    w.end = min(w.ue, w.hi);
+    const int64_t from = max(w.cur, w.ts);
+    if (from < w.end) {
+      w.t0 = int(from - w.ts) * TILE;
+      w.t1 = min(w.seq.n, int(w.end - w.ts) * TILE);
+      return true;
+    }
+    w.cur = w.end;      // only the empty stretch was this block's
   }
-  w.unit = int((w.cur - w.base) / w.seq.tiles);
-  w.us = w.base + int64_t(w.unit) * w.seq.tiles;
-  w.ue = w.us + w.seq.tiles;
-  w.end = min(w.ue, w.hi);
-  w.t0 = int(w.cur - w.us) * TILE;
-  w.t1 = min(w.seq.n, int(w.end - w.us) * TILE);
-  return true;
+  return false;
 }
 
 // ---------------------------------------------------------------- rows of the pages
@@ -182,10 +197,8 @@ __device__ __forceinline__ float pa_weight(float m, float top) {
 // Floats of a triple of `rows` heads: m [rows], l [rows], a [rows][dhp] from a multiple of four on.
 __host__ __device__ constexpr int pa_head(int rows) { return (2 * rows + 3) & ~3; }
 __host__ __device__ constexpr int pa_triple(int rows, int dhp) { return pa_head(rows) + rows * dhp; }
-// Shared memory of pa_finish in floats: a triple per warp and the joined m and l.
-__host__ __device__ constexpr int pa_finish_floats(int warps, int rows, int dhp) {
-  return warps * pa_triple(rows, dhp) + 2 * rows;
-}
+// Shared memory of pa_finish in floats: a triple per warp.
+__host__ __device__ constexpr int pa_finish_floats(int warps, int rows, int dhp) { return warps * pa_triple(rows, dhp); }
 
 // Writes four values d.. of head g of the unit from its joined triple.
 __device__ __forceinline__ void pa_write4(const PagedAttnParams& p, int b, int h, int d, const float4& a, float l) {
@@ -220,42 +233,38 @@ template <int DHP>
 __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork& w, float* sm, int warps, int rows, int h0, int live) {
   __shared__ int s_last;
   const int threads = warps * 32, triple = pa_triple(rows, DHP);
-  float* j_m = sm + warps * triple;
-  float* j_l = j_m + rows;
   pa_sync(threads);
-  if (int(threadIdx.x) < live) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < warps; ++i) top = fmaxf(top, sm[i * triple + threadIdx.x]);
-    for (int i = 0; i < warps; ++i) {
-      float* m = sm + i * triple + threadIdx.x;
-      const float wt = pa_weight(*m, top);
-      sum += m[rows] * wt;
-      *m = wt;      // from here on the warp's weight
-    }
-    j_m[threadIdx.x] = top;
-    j_l[threadIdx.x] = sum;
-  }
-  pa_sync(threads);
-  const int first = pa_block_of(w.total, w.us, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
-  auto slot_of = [&](int64_t c) { return p.part + (c * 2 + (pa_lo(w.total, c, w.blocks) >= w.us ? 0 : 1)) * triple; };
-  float* mine = slot_of(blockIdx.x);
+  const bool whole = w.lo <= w.ts && w.ue <= w.hi;
+  auto slot_of = [&](int64_t c) { return p.part + (c * 2 + (pa_lo(w.total, c, w.blocks) >= w.ts ? 0 : 1)) * triple; };
+  float* mine = p.part + (int64_t(blockIdx.x) * 2 + (w.lo >= w.ts ? 0 : 1)) * triple;
   for (int e = threadIdx.x; e < live * (DHP / 4); e += threads) {
     const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < warps; ++i)
-      pa_add4(a, *reinterpret_cast<const float4*>(sm + i * triple + pa_head(rows) + g * DHP + d), sm[i * triple + g]);
-    if (first == last) pa_write4(p, w.b, h0 + g, d, a, j_l[g]);
-    else *reinterpret_cast<float4*>(mine + pa_head(rows) + g * DHP + d) = a;
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < warps; ++i) top = fmaxf(top, sm[i * triple + g]);
+#pragma unroll 4
+    for (int i = 0; i < warps; ++i) {
+      const float* from = sm + i * triple;
+      const float wt = pa_weight(from[g], top);
+      sum += from[rows + g] * wt;
+      pa_add4(a, *reinterpret_cast<const float4*>(from + pa_head(rows) + g * DHP + d), wt);
+    }
+    if (whole) {
+      pa_write4(p, w.b, h0 + g, d, a, sum);
+      if (d == 0) pa_write_lse(p, w.b, h0 + g, top, sum);
+    } else {
+      *reinterpret_cast<float4*>(mine + pa_head(rows) + g * DHP + d) = a;
+      if (d == 0) {
+        mine[g] = top;
+        mine[rows + g] = sum;
+      }
+    }
   }
-  if (first == last) {
-    if (int(threadIdx.x) < live) pa_write_lse(p, w.b, h0 + threadIdx.x, j_m[threadIdx.x], j_l[threadIdx.x]);
-    pa_sync(threads);
+  if (whole) {
+    pa_sync(threads);     // the triples are free again
     return;
   }
-  if (int(threadIdx.x) < live) {
-    mine[threadIdx.x] = j_m[threadIdx.x];
-    mine[rows + threadIdx.x] = j_l[threadIdx.x];
-  }
+  const int first = pa_block_of(w.total, w.ts, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
   __threadfence();
   pa_sync(threads);
   int* counter = p.counters + int64_t(w.b) * p.units + w.unit;
@@ -268,19 +277,26 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     const float* next = p.part + (int64_t(first) + 1) * 2 * triple;
     const int n = last - first + 1;
     auto part = [&](int i) { return i == 0 ? from : next + int64_t(i - 1) * 2 * triple; };
-    float* wts = sm;                  // [n][live] weights, if they fit where the warps' triples were
-    const bool fits = n * live <= warps * triple;
+    float* j_m = sm;
+    float* j_l = sm + rows;
+    float* wts = sm + pa_head(rows);                  // [n][live] weights, if they fit
+    const bool fits = n * live <= warps * triple - pa_head(rows);
     // a warp per head: the largest m, then the sum
     for (int g = threadIdx.x >> 5; g < live; g += warps) {
       const int lane = threadIdx.x & 31;
       float top = -INFINITY, sum = 0.0f;
-      for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part(i) + g));
+      for (int i = lane; i < n; i += 32) {
+        const float m = __ldcg(part(i) + g);
+        if (fits) wts[i * live + g] = m;
+        top = fmaxf(top, m);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       for (int i = lane; i < n; i += 32) {
-        const float wt = pa_weight(__ldcg(part(i) + g), top);
+        const float l = __ldcg(part(i) + rows + g);
+        const float wt = pa_weight(fits ? wts[i * live + g] : __ldcg(part(i) + g), top);
         if (fits) wts[i * live + g] = wt;
-        sum += __ldcg(part(i) + rows + g) * wt;
+        sum += l * wt;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -291,27 +307,26 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
       }
     }
     pa_sync(threads);
+    constexpr int FLY = 16;      // loads in flight
     for (int e = threadIdx.x; e < live * (DHP / 4); e += threads) {
       const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
       float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       const float top = j_m[g];
-      int i = 0;
-      for (; i + 8 <= n; i += 8) {      // eight loads in flight
-        float4 x[8];
+      for (int i = 0; i < n; i += FLY) {
+        float4 x[FLY];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = __ldcg(reinterpret_cast<const float4*>(part(i + u) + pa_head(rows) + g * DHP + d));
+        for (int u = 0; u < FLY; ++u)
+          x[u] = i + u < n ? __ldcg(reinterpret_cast<const float4*>(part(i + u) + pa_head(rows) + g * DHP + d))
+                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          pa_add4(a, x[u], fits ? wts[(i + u) * live + g] : pa_weight(__ldcg(part(i + u) + g), top));
+        for (int u = 0; u < FLY; ++u)
+          if (i + u < n) pa_add4(a, x[u], fits ? wts[(i + u) * live + g] : pa_weight(__ldcg(part(i + u) + g), top));
       }
-      for (; i < n; ++i)
-        pa_add4(a, __ldcg(reinterpret_cast<const float4*>(part(i) + pa_head(rows) + g * DHP + d)),
-                fits ? wts[i * live + g] : pa_weight(__ldcg(part(i) + g), top));
       pa_write4(p, w.b, h0 + g, d, a, j_l[g]);
     }
     if (threadIdx.x == 0) *counter = 0;
   }
-  pa_sync(threads);     // the shared triples are free again
+  pa_sync(threads);     // the triples are free again
 }
 
 // ---------------------------------------------------------------- rows in flight

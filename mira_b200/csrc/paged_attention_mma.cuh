@@ -168,51 +168,51 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
     const int h0 = kvh * p.group + g0, live_heads = min(8 * NH, p.group - g0);
     const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
 
-    // queries of the unit in fragment order; a thread per (product, lane).  f16 values of a query that
-    // is not f16 itself are taken after a power of two has brought its largest element to [128, 256).
+    // queries of the unit in fragment order, a warp per head, four elements of it per lane and turn.  f16
+    // values of a query that is not f16 itself are taken after a power of two has brought its largest
+    // element to [128, 256).
     for (int h = warp; h < 8 * NH; h += warps) {
-      float unit = p.scale_log2;
+      constexpr int TURNS = DHP / 128 > 1 ? DHP / 128 : 1;
+      float x[TURNS][4], top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = (i * 32 + lane) * 4 + e;
+          x[i][e] = h < live_heads && d < p.kv.dh
+              ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + d * p.qs[2], p.q_dtype) : 0.0f;
+          top = fmaxf(top, fabsf(x[i][e]));
+        }
+      float up = 1.0f;
       if (QP == 3 && !C::BF16) {
-        float top = 0.0f;
-        if (h < live_heads)
-          for (int d = lane; d < p.kv.dh; d += 32)
-            top = fmaxf(top, fabsf(dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + d * p.qs[2], p.q_dtype)));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int e = int(__float_as_uint(top) >> 23);      // 2^(e - 127) <= top
-        const int up = e == 0 || e == 255 ? 0 : min(max(134 - e, -126), 127);
-        if (lane == 0) s_unit[h] = __int_as_float((127 + up) << 23);
-      } else if (lane == 0) {
-        s_unit[h] = unit;
+        up = __int_as_float((127 + (e == 0 || e == 255 ? 0 : min(max(134 - e, -126), 127))) << 23);
       }
-    }
-    pa_sync(warps * 32);
-    for (int i = threadIdx.x; i < NH * C::KS * 32; i += warps * 32) {
-      const int l = i & 31, lt = l & 3, ks = (i >> 5) % C::KS, h = (i >> 5) / C::KS * 8 + (l >> 2);
-      const int d = (ks / (C::KE / 4)) * 4 * C::KE + lt * C::KE + (ks % (C::KE / 4)) * 4;
-      float x[4];       // elements d .. d + 3 of head h
+      if (lane == 0) s_unit[h] = p.scale_log2 / up;         // a power of two: exact
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = h < live_heads && d + e < p.kv.dh
-            ? dt_load(p.q, w.b * p.qs[0] + (h0 + h) * p.qs[1] + (d + e) * p.qs[2], p.q_dtype) : 0.0f;
-        if (QP == 3 && !C::BF16) x[e] *= s_unit[h];
-      }
-      uint32_t f[2][QP];
-      if (C::BF16 && QP == 3) {
+      for (int i = 0; i < TURNS; ++i) {
+        const int d = (i * 32 + lane) * 4;
+        if (d >= DHP) break;
+        const int lt = d % (4 * C::KE) / C::KE, ks = d / (4 * C::KE) * (C::KE / 4) + d % C::KE / 4;
+        uint32_t f[2][QP];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          uint32_t a[3], b[3];
-          split3_bf16(x[2 * j], a[0], a[1], a[2]);
-          split3_bf16(x[2 * j + 1], b[0], b[1], b[2]);
+          if (C::BF16 && QP == 3) {
+            uint32_t a[3], b[3];
+            split3_bf16(x[i][2 * j], a[0], a[1], a[2]);
+            split3_bf16(x[i][2 * j + 1], b[0], b[1], b[2]);
 #pragma unroll
-          for (int q = 0; q < QP; ++q) f[j][q] = __byte_perm(a[q], b[q], 0x7632);
+            for (int q = 0; q < QP; ++q) f[j][q] = __byte_perm(a[q], b[q], 0x7632);
+          } else {
+            pa_split2<C::BF16, QP>(x[i][2 * j] * up, x[i][2 * j + 1] * up, f[j]);
+          }
         }
-      } else {
-        pa_split2<C::BF16, QP>(x[0], x[1], f[0]);
-        pa_split2<C::BF16, QP>(x[2], x[3], f[1]);
-      }
 #pragma unroll
-      for (int q = 0; q < QP; ++q) s_q[q * (NH * C::KS * 32) + i] = make_uint2(f[0][q], f[1][q]);
+        for (int q = 0; q < QP; ++q)
+          s_q[((q * NH + h / 8) * C::KS + ks) * 32 + h % 8 * 4 + lt] = make_uint2(f[0][q], f[1][q]);
+      }
     }
     pa_sync(warps * 32);
     // this lane's heads are 8 b + 2t + i
@@ -222,7 +222,6 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         unit[b][i] = s_unit[8 * b + 2 * t + i];
-        if (QP == 3 && !C::BF16) unit[b][i] = p.scale_log2 / unit[b][i];      // a power of two: exact
         m[b][i] = -INFINITY;
         l[b][i] = 0.0f;
       }
