@@ -60,9 +60,13 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedAttnParams& p, int b) {
 // without it the blocks that get many short sequences finish last (64 sequences of 16 to 1024 tokens: the
 // last block at twice the median's time).
 constexpr int PA_PART_COST = 8;
-__device__ __forceinline__ int64_t pa_lo(int64_t total, int64_t c, int64_t g) { return total * c / g; }
+// Quotients of nonnegative numbers; nearly all fit 32 bits, where dividing takes a fraction of the time.
+__device__ __forceinline__ int64_t pa_quot(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+__device__ __forceinline__ int64_t pa_lo(int64_t total, int64_t c, int64_t g) { return pa_quot(total * c, g); }
 __device__ __forceinline__ int pa_block_of(int64_t total, int64_t x, int64_t g) {
-  return static_cast<int>(((x + 1) * g - 1) / total);
+  return static_cast<int>(pa_quot((x + 1) * g - 1, total));
 }
 
 // Sum of v over the block, and the sum over the lower-numbered threads.
@@ -116,7 +120,7 @@ __device__ __forceinline__ bool pa_begin(const PagedAttnParams& p, int least, Pa
     sum = pa_scan(mine, before, s_scan);
     w.total += sum;
   }
-  const int64_t apart = max(int64_t(p.kv.batch) * p.units, w.total / least);
+  const int64_t apart = max(int64_t(p.kv.batch) * p.units, pa_quot(w.total, least));
   w.blocks = min(min(int64_t(gridDim.x), w.total), apart);
   if (blockIdx.x >= w.blocks) return false;
   w.lo = w.cur = pa_lo(w.total, blockIdx.x, w.blocks);
@@ -150,7 +154,7 @@ __device__ __forceinline__ bool pa_part(const PagedAttnParams& p, PaWork& w) {
       per = w.seq.tiles + PA_PART_COST;
     }
     const int64_t in = w.cur - w.base;
-    w.unit = in <= int64_t(UINT32_MAX) ? int(uint32_t(in) / uint32_t(per)) : int(in / per);
+    w.unit = int(pa_quot(in, per));
     const int64_t us = w.base + w.unit * per;
     w.ts = us + PA_PART_COST;
     w.ue = us + per;
@@ -200,16 +204,22 @@ __host__ __device__ constexpr int pa_triple(int rows, int dhp) { return pa_head(
 // Shared memory of pa_finish in floats: a triple per warp.
 __host__ __device__ constexpr int pa_finish_floats(int warps, int rows, int dhp) { return warps * pa_triple(rows, dhp); }
 
-// Writes four values d.. of head g of the unit from its joined triple.
+// Writes four values d.. of head h of sequence b from its joined triple.  l is at least about 1 (the
+// largest score's weight) or 0, so its reciprocal is as good as a division to the last place or two.
 __device__ __forceinline__ void pa_write4(const PagedAttnParams& p, int b, int h, int d, const float4& a, float l) {
-  const float v[4] = {a.x, a.y, a.z, a.w};
+  const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
+  const float v[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+  if (p.out != nullptr) {
+    const int64_t at = b * p.os[0] + h * p.os[1] + d * p.os[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (d + i >= p.kv.dh) break;
-    const float o = l == 0.0f ? 0.0f : __fdiv_rn(v[i], l);
-    if (p.out != nullptr) dt_store(p.out, b * p.os[0] + h * p.os[1] + (d + i) * p.os[2], p.q_dtype, o);
-    if (p.out_i8 != nullptr)
-      p.out_i8[b * p.is[0] + h * p.is[1] + (d + i) * p.is[2]] = static_cast<int8_t>(quant_byte(o, p.q8) & 0xff);
+    for (int i = 0; i < 4; ++i)
+      if (d + i < p.kv.dh) dt_store(p.out, at + i * p.os[2], p.q_dtype, v[i]);
+  }
+  if (p.out_i8 != nullptr) {
+    const int64_t at = b * p.is[0] + h * p.is[1] + d * p.is[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < p.kv.dh) p.out_i8[at + i * p.is[2]] = static_cast<int8_t>(quant_byte(v[i], p.q8) & 0xff);
   }
 }
 
@@ -241,6 +251,7 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < warps; ++i) top = fmaxf(top, sm[i * triple + g]);
 #pragma unroll 4
     for (int i = 0; i < warps; ++i) {
@@ -265,10 +276,12 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     return;
   }
   const int first = pa_block_of(w.total, w.ts, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
-  __threadfence();
   pa_sync(threads);
   int* counter = p.counters + int64_t(w.b) * p.units + w.unit;
-  if (threadIdx.x == 0) s_last = atomicAdd(counter, 1) == last - first;
+  if (threadIdx.x == 0) {
+    __threadfence();      // the whole block's slot, by the barrier before
+    s_last = atomicAdd(counter, 1) == last - first;
+  }
   pa_sync(threads);
   if (s_last) {
     __threadfence();
@@ -285,18 +298,29 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
     for (int g = threadIdx.x >> 5; g < live; g += warps) {
       const int lane = threadIdx.x & 31;
       float top = -INFINITY, sum = 0.0f;
-      for (int i = lane; i < n; i += 32) {
-        const float m = __ldcg(part(i) + g);
-        if (fits) wts[i * live + g] = m;
-        top = fmaxf(top, m);
+      // m and l of up to 64 parts at once, the rest (if any) one by one
+      float m[2], l[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = lane + 32 * u;
+        m[u] = i < n ? __ldcg(part(i) + g) : -INFINITY;
+        l[u] = i < n ? __ldcg(part(i) + rows + g) : 0.0f;
+        top = fmaxf(top, m[u]);
       }
+      for (int i = lane + 64; i < n; i += 32) top = fmaxf(top, __ldcg(part(i) + g));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      for (int i = lane; i < n; i += 32) {
-        const float l = __ldcg(part(i) + rows + g);
-        const float wt = pa_weight(fits ? wts[i * live + g] : __ldcg(part(i) + g), top);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = lane + 32 * u;
+        const float wt = pa_weight(m[u], top);
+        if (fits && i < n) wts[i * live + g] = wt;
+        sum += l[u] * wt;
+      }
+      for (int i = lane + 64; i < n; i += 32) {
+        const float wt = pa_weight(__ldcg(part(i) + g), top);
         if (fits) wts[i * live + g] = wt;
-        sum += l * wt;
+        sum += __ldcg(part(i) + rows + g) * wt;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
