@@ -2007,6 +2007,27 @@ static bool paged_rows_aligned(const mira_paged_kv& a, int64_t bytes) {
 
 }  // namespace mira
 
+namespace mira {
+
+template <int SRC, int DST, bool VEC>
+static int launch_append(DeviceState* dev, AppendParams& p) {
+  p.per_div = make_div(p.kv.dh / (VEC ? 4 : 1));
+  kv_append_kernel<SRC, DST, VEC><<<grid_for(dev, p.rows * 32, APPEND_WARPS * 32), APPEND_WARPS * 32, 0, dev->stream>>>(p);
+  return after_launch("kv_append_kernel");
+}
+
+template <int SRC>
+static int launch_append_from(DeviceState* dev, AppendParams& p, int dtype, bool vec) {
+  switch (dtype) {
+    case MIRA_DT_F32: return vec ? launch_append<SRC, MIRA_DT_F32, true>(dev, p) : launch_append<SRC, MIRA_DT_F32, false>(dev, p);
+    case MIRA_DT_F16: return vec ? launch_append<SRC, MIRA_DT_F16, true>(dev, p) : launch_append<SRC, MIRA_DT_F16, false>(dev, p);
+    case MIRA_DT_BF16: return vec ? launch_append<SRC, MIRA_DT_BF16, true>(dev, p) : launch_append<SRC, MIRA_DT_BF16, false>(dev, p);
+    default: return launch_append<SRC, MIRA_DT_I8, false>(dev, p);
+  }
+}
+
+}  // namespace mira
+
 extern "C" int mira_cuda_kv_append(const mira_kv_append* a) {
   MIRA_GET_DEVICE(dev);
   MIRA_CHECK_ARG(a != nullptr, "null append descriptor");
@@ -2028,10 +2049,17 @@ extern "C" int mira_cuda_kv_append(const mira_kv_append* a) {
   for (int i = 0; i < 2; ++i) { p.kn[i] = a->k_new.stride[i + 1]; p.vn[i] = a->v_new.stride[i + 1]; }
   p.row_start = a->row_start;
   p.rows = a->rows;
-  p.src_dtype = a->src_dtype;
-  p.dtype = a->kv.dtype;
-  kv_append_kernel<<<grid_for(dev, a->rows * a->kv.kv_heads * 32, APPEND_WARPS * 32), APPEND_WARPS * 32, 0, dev->stream>>>(p);
-  return after_launch("kv_append_kernel");
+  // four elements at a time: rows and slots on multiples of four elements
+  const int64_t from = 4 * dt_size(a->src_dtype), to = 4 * dt_size(a->kv.dtype);
+  bool vec = a->kv.dh % 4 == 0 && aligned_to(a->k_new.ptr, from) && aligned_to(a->v_new.ptr, from) &&
+             aligned_to(a->kv.k.ptr, to) && aligned_to(a->kv.v.ptr, to);
+  for (int i = 0; i < 2; ++i) vec = vec && p.kn[i] % 4 == 0 && p.vn[i] % 4 == 0;
+  for (int i = 0; i < 3; ++i) vec = vec && p.kv.kst[i] % 4 == 0 && p.kv.vst[i] % 4 == 0;
+  switch (a->src_dtype) {
+    case MIRA_DT_F32: return launch_append_from<MIRA_DT_F32>(dev, p, a->kv.dtype, vec);
+    case MIRA_DT_F16: return launch_append_from<MIRA_DT_F16>(dev, p, a->kv.dtype, vec);
+    default: return launch_append_from<MIRA_DT_BF16>(dev, p, a->kv.dtype, vec);
+  }
 }
 
 extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* regions, int64_t num_pages, int64_t n,

@@ -85,20 +85,39 @@ struct AppendParams {
   int64_t kn[2], vn[2];       // element strides of (kv head, row)
   const int32_t* row_start;
   int64_t rows;
-  int src_dtype, dtype;
+  QgDiv per_div;              // accesses of a head
 };
 
-// One warp per (row, kv head): the row's sequence by bisection of row_start, then the head's key and
-// value converted lane by lane.
+// Bound: the new rows are read and written once (f32 into bf16: 6 bytes an element).  A warp takes one
+// row, looks its sequence and its slot up once (the sequence by bisection of row_start, one probe per
+// lane and turn) and copies all heads' keys and values: 16-byte reads where the rows allow, four in
+// flight per lane, written in the width that they convert to.
 constexpr int APPEND_WARPS = 8;
 
-__device__ __forceinline__ void append_row(const void* src, int64_t so, int src_dtype, void* dst, int64_t d0, int dtype,
-                                           float* scale, int dh, int lane) {
-  if (dtype != MIRA_DT_I8) {
-    for (int i = lane; i < dh; i += 32) dt_store(dst, d0 + i, dtype, dt_load(src, so + i, src_dtype));
-    return;
-  }
-  // scale = absmax / 127 and codes rint(x / scale), both IEEE divisions like the int8 weights
+template <int DT> struct AppendElem;
+template <> struct AppendElem<MIRA_DT_F32> { using type = float; };
+template <> struct AppendElem<MIRA_DT_F16> { using type = __half; };
+template <> struct AppendElem<MIRA_DT_BF16> { using type = __nv_bfloat16; };
+
+template <int DT>
+__device__ __forceinline__ float append_f32(typename AppendElem<DT>::type x) {
+  if constexpr (DT == MIRA_DT_F32) return x;
+  else if constexpr (DT == MIRA_DT_F16) return __half2float(x);
+  else return __bfloat162float(x);
+}
+template <int DT>
+__device__ __forceinline__ typename AppendElem<DT>::type append_to(float x) {
+  if constexpr (DT == MIRA_DT_F32) return x;
+  else if constexpr (DT == MIRA_DT_F16) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
+
+// Four elements as one access.
+template <class T> struct alignas(4 * sizeof(T)) Append4 { T v[4]; };
+
+// One head's row of 8-bit codes: scale = absmax / 127 and codes rint(x / scale), both IEEE divisions like
+// the int8 weights.
+__device__ __forceinline__ void append_codes(const void* src, int64_t so, int src_dtype, int8_t* dst, float* scale, int dh, int lane) {
   float top = 0.0f;
   for (int i = lane; i < dh; i += 32) top = np_maximum(top, fabsf(dt_load(src, so + i, src_dtype)));
 #pragma unroll
@@ -107,44 +126,102 @@ __device__ __forceinline__ void append_row(const void* src, int64_t so, int src_
   if (lane == 0) *scale = s;
   for (int i = lane; i < dh; i += 32) {
     const float z = __fdiv_rn(dt_load(src, so + i, src_dtype), s);
-    static_cast<int8_t*>(dst)[d0 + i] = static_cast<int8_t>(round_clip_i8(z) & 0xff);
+    dst[i] = static_cast<int8_t>(round_clip_i8(z) & 0xff);
   }
 }
 
+// The sequence of a row: the last b with row_start[b] <= row.  The whole warp asks.
+__device__ __forceinline__ int append_sequence(const AppendParams& p, int64_t row, int lane) {
+  int lo = 0, hi = p.kv.batch;        // row_start[lo] <= row < row_start[hi]
+  while (hi - lo > 1) {
+    const int width = (hi - lo + 31) / 32;
+    const int at = lo + lane * width;
+    const uint32_t le = __ballot_sync(0xffffffffu, at < hi && __ldg(p.row_start + at) <= row);
+    const int last = 31 - __clz(le);  // -1: row_start[0] is above the row, which the caller refuses
+    if (last < 0) return 0;
+    lo += last * width;
+    hi = min(hi, lo + width);
+  }
+  return lo;
+}
+
+// DST: MIRA_DT_I8, or the pages' type; VEC: rows and slots can be read and written four elements at a time.
+template <int SRC, int DST, bool VEC>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __grid_constant__ AppendParams p) {
   const PagedKv& kv = p.kv;
   const int lane = threadIdx.x & 31;
-  const int64_t tasks = p.rows * kv.kv_heads;
-  const int64_t step = int64_t(gridDim.x) * APPEND_WARPS;
-  for (int64_t t = blockIdx.x * int64_t(APPEND_WARPS) + (threadIdx.x >> 5); t < tasks; t += step) {
-    const int64_t row = t / kv.kv_heads;
-    const int h = int(t - row * kv.kv_heads);
+  for (int64_t row = blockIdx.x * int64_t(APPEND_WARPS) + (threadIdx.x >> 5); row < p.rows; row += int64_t(gridDim.x) * APPEND_WARPS) {
     int b = int(row), from_end = 1;
     if (p.row_start != nullptr) {
-      int lo = 0, hi = kv.batch;        // row_start[lo] <= row < row_start[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(p.row_start + mid) <= row) lo = mid;
-        else hi = mid;
-      }
-      b = lo;
-      from_end = int(__ldg(p.row_start + b + 1) - row);
+      b = append_sequence(p, row, lane);
+      from_end = int(min(int64_t(__ldg(p.row_start + b + 1)) - row, int64_t(INT32_MAX)));
+      if (__ldg(p.row_start + b) > row) from_end = 0;
     }
     const int n = paged_length(kv, b);
     if (n == 0 && p.row_start == nullptr) continue;
     const int pos = n - from_end;
+    int page, slot;
     if (from_end <= 0 || pos < 0) {
       if (lane == 0) atomicExch(kv.err, PAGED_ERR);
       continue;
     }
-    int page, slot;
     if (!paged_slot(kv, kv.table + b * kv.table_ld, pos, page, slot)) continue;
-    append_row(p.k_new, h * p.kn[0] + row * p.kn[1], p.src_dtype, kv.k,
-               page * kv.kst[0] + h * kv.kst[1] + slot * kv.kst[2], p.dtype,
-               kv.ks + (page * kv.kss[0] + h * kv.kss[1] + slot * kv.kss[2]), kv.dh, lane);
-    append_row(p.v_new, h * p.vn[0] + row * p.vn[1], p.src_dtype, kv.v,
-               page * kv.vst[0] + h * kv.vst[1] + slot * kv.vst[2], p.dtype,
-               kv.vs + (page * kv.vss[0] + h * kv.vss[1] + slot * kv.vss[2]), kv.dh, lane);
+    const int64_t ko = page * kv.kst[0] + slot * kv.kst[2], vo = page * kv.vst[0] + slot * kv.vst[2];
+    if constexpr (DST == MIRA_DT_I8) {
+      for (int h = 0; h < kv.kv_heads; ++h) {
+        append_codes(p.k_new, h * p.kn[0] + row * p.kn[1], SRC, static_cast<int8_t*>(kv.k) + ko + h * kv.kst[1],
+                     kv.ks + page * kv.kss[0] + h * kv.kss[1] + slot * kv.kss[2], kv.dh, lane);
+        append_codes(p.v_new, h * p.vn[0] + row * p.vn[1], SRC, static_cast<int8_t*>(kv.v) + vo + h * kv.vst[1],
+                     kv.vs + page * kv.vss[0] + h * kv.vss[1] + slot * kv.vss[2], kv.dh, lane);
+      }
+    } else {
+      using S = typename AppendElem<SRC>::type;
+      using D = typename AppendElem<DST>::type;
+      const S* ks = static_cast<const S*>(p.k_new) + row * p.kn[1];
+      const S* vs = static_cast<const S*>(p.v_new) + row * p.vn[1];
+      D* kd = static_cast<D*>(kv.k) + ko;
+      D* vd = static_cast<D*>(kv.v) + vo;
+      constexpr int W = VEC ? 4 : 1, U = 4;
+      const int per = kv.dh / W, total = kv.kv_heads * per;      // accesses of a head, of the row
+      for (int e0 = lane; e0 < total; e0 += 32 * U) {
+        Append4<S> k[U], v[U];
+        int64_t kt[U], vt[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int e = e0 + 32 * u;
+          if (e >= total) break;
+          const int h = qg_div(e, p.per_div), d = (e - h * per) * W;
+          kt[u] = h * kv.kst[1] + d;
+          vt[u] = h * kv.vst[1] + d;
+          const S* kf = ks + h * p.kn[0] + d;
+          const S* vf = vs + h * p.vn[0] + d;
+          if constexpr (VEC) {
+            k[u] = *reinterpret_cast<const Append4<S>*>(kf);
+            v[u] = *reinterpret_cast<const Append4<S>*>(vf);
+          } else {
+            k[u].v[0] = *kf;
+            v[u].v[0] = *vf;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (e0 + 32 * u >= total) break;
+          if constexpr (VEC) {
+            Append4<D> x, y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x.v[i] = append_to<DST>(append_f32<SRC>(k[u].v[i]));
+              y.v[i] = append_to<DST>(append_f32<SRC>(v[u].v[i]));
+            }
+            *reinterpret_cast<Append4<D>*>(kd + kt[u]) = x;
+            *reinterpret_cast<Append4<D>*>(vd + vt[u]) = y;
+          } else {
+            kd[kt[u]] = append_to<DST>(append_f32<SRC>(k[u].v[0]));
+            vd[vt[u]] = append_to<DST>(append_f32<SRC>(v[u].v[0]));
+          }
+        }
+      }
+    }
   }
 }
 
