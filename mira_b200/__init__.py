@@ -6,7 +6,7 @@ quantized matmuls and convolutions on hand-written tcgen05 kernels (libmira_cuda
 """
 from __future__ import annotations
 
-__all__ = ["install", "CudaTarget", "int8_depthwise"]
+__all__ = ["install", "CudaTarget", "int8_depthwise", "PagedCache", "PagedTransformer"]
 
 
 def install():
@@ -21,4 +21,10 @@ def __getattr__(name):
     if name == "int8_depthwise":
         from .depthwise import int8_depthwise
         return int8_depthwise
+    if name == "PagedCache":
+        from .paged import PagedCache
+        return PagedCache
+    if name == "PagedTransformer":
+        from .paged_decode import PagedTransformer
+        return PagedTransformer
     raise AttributeError(name)

@@ -2062,28 +2062,51 @@ extern "C" int mira_cuda_kv_append(const mira_kv_append* a) {
   }
 }
 
+namespace mira {
+
+template <int PAIRS>
+static int launch_page_copy(DeviceState* dev, const PageCopyRegion* r, int n_regions, int64_t tasks, int64_t n, const int32_t* src,
+                            const int32_t* dst) {
+  PageCopyParams<PAIRS> p;
+  std::memcpy(p.r, r, sizeof(p.r));
+  p.n_regions = n_regions;
+  p.tasks = tasks;
+  for (int64_t at = 0; at < n; at += PAIRS) {
+    p.n = int(n - at < PAIRS ? n - at : PAIRS);
+    std::memcpy(p.src, src + at, size_t(p.n) * 4);
+    std::memcpy(p.dst, dst + at, size_t(p.n) * 4);
+    const int64_t blocks = tasks * p.n, cap = int64_t(dev->sm_count) * 64;
+    page_copy_kernel<PAIRS><<<unsigned(blocks < cap ? blocks : cap), PAGE_COPY_THREADS, 0, dev->stream>>>(p);
+    const int rc = after_launch("page_copy_kernel");
+    if (rc != MIRA_CUDA_OK) return rc;
+  }
+  return MIRA_CUDA_OK;
+}
+
+}  // namespace mira
+
 extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* regions, int64_t num_pages, int64_t n,
                                    const int32_t* src, const int32_t* dst) {
   MIRA_GET_DEVICE(dev);
   MIRA_CHECK_ARG(n_regions > 0 && n_regions <= MIRA_PAGE_REGIONS && regions != nullptr, "1 to 4 page regions");
   MIRA_CHECK_ARG(num_pages > 0 && num_pages <= INT32_MAX && n >= 0 && n <= num_pages, "bad page counts");
   MIRA_CHECK_ARG(n == 0 || (src != nullptr && dst != nullptr), "null page lists");
-  PageCopyParams p;
-  std::memset(&p, 0, sizeof(p));
-  p.n_regions = int(n_regions);
-  for (int i = 0; i < p.n_regions; ++i) {
+  PageCopyRegion region[MIRA_PAGE_REGIONS];
+  std::memset(region, 0, sizeof(region));
+  int64_t tasks = 0;
+  for (int i = 0; i < int(n_regions); ++i) {
     const mira_page_region& r = regions[i];
     MIRA_CHECK_ARG(r.base != nullptr && r.planes > 0 && r.planes <= INT32_MAX && r.page_bytes > 0 &&
                        r.page_stride >= r.page_bytes && r.plane_stride >= 0,
                    "bad page region");
     const int64_t chunks = (r.page_bytes + PAGE_COPY_CHUNK - 1) / PAGE_COPY_CHUNK;
     MIRA_CHECK_ARG(chunks <= INT32_MAX, "pages too large");
-    p.r[i].base = static_cast<uint8_t*>(r.base);
-    p.r[i].plane_stride = r.plane_stride; p.r[i].page_stride = r.page_stride; p.r[i].page_bytes = r.page_bytes;
-    p.r[i].planes = int(r.planes); p.r[i].chunks = int(chunks);
-    p.r[i].first = p.tasks;
-    p.r[i].vec = aligned_to(r.base, 16) && r.plane_stride % 16 == 0 && r.page_stride % 16 == 0;
-    p.tasks += r.planes * chunks;
+    region[i].base = static_cast<uint8_t*>(r.base);
+    region[i].plane_stride = r.plane_stride; region[i].page_stride = r.page_stride; region[i].page_bytes = r.page_bytes;
+    region[i].planes = int(r.planes); region[i].chunks = int(chunks);
+    region[i].first = tasks;
+    region[i].vec = aligned_to(r.base, 16) && r.plane_stride % 16 == 0 && r.page_stride % 16 == 0;
+    tasks += r.planes * chunks;
   }
   // no page may be written twice, or written and read: the pairs run in any order
   try {
@@ -2097,16 +2120,8 @@ extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* re
   } catch (const std::exception&) {
     return set_error(MIRA_CUDA_EINVAL, "out of host memory while checking the page lists");
   }
-  for (int64_t at = 0; at < n; at += PAGE_COPY_PAIRS) {
-    p.n = int(n - at < PAGE_COPY_PAIRS ? n - at : PAGE_COPY_PAIRS);
-    std::memcpy(p.src, src + at, size_t(p.n) * 4);
-    std::memcpy(p.dst, dst + at, size_t(p.n) * 4);
-    const int64_t blocks = p.tasks * p.n, cap = int64_t(dev->sm_count) * 64;
-    page_copy_kernel<<<unsigned(blocks < cap ? blocks : cap), PAGE_COPY_THREADS, 0, dev->stream>>>(p);
-    const int rc = after_launch("page_copy_kernel");
-    if (rc != MIRA_CUDA_OK) return rc;
-  }
-  return MIRA_CUDA_OK;
+  return n <= PAGE_COPY_FEW ? launch_page_copy<PAGE_COPY_FEW>(dev, region, int(n_regions), tasks, n, src, dst)
+                            : launch_page_copy<PAGE_COPY_MANY>(dev, region, int(n_regions), tasks, n, src, dst);
 }
 
 namespace mira {

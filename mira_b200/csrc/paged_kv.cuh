@@ -227,32 +227,39 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __gr
 
 // ---------------------------------------------------------------- page copies
 
-constexpr int PAGE_COPY_PAIRS = 448;      // pairs per launch: the ids travel in the kernel's parameters
+// Bound: the moved pages are read and written once.  The page ids travel in the kernel's parameters, so
+// that nothing has to be copied to the device before it: few of them in a small parameter block (a launch
+// with 4 KB of parameters takes the host about 2 us longer), many in several launches.
+constexpr int PAGE_COPY_FEW = 32, PAGE_COPY_MANY = 448;     // pairs per launch
 constexpr int PAGE_COPY_CHUNK = 16384;    // bytes of one block's share of a page
 constexpr int PAGE_COPY_THREADS = 256;
 
+struct PageCopyRegion {
+  uint8_t* base;
+  int64_t plane_stride, page_stride, page_bytes;
+  int planes, chunks;      // chunks of a page
+  int64_t first;           // first task of this region
+  int vec;                 // 16-byte accesses
+};
+
+template <int PAIRS>
 struct PageCopyParams {
-  struct Region {
-    uint8_t* base;
-    int64_t plane_stride, page_stride, page_bytes;
-    int planes, chunks;      // chunks of a page
-    int64_t first;           // first task of this region
-    int vec;                 // 16-byte accesses
-  } r[MIRA_PAGE_REGIONS];
+  PageCopyRegion r[MIRA_PAGE_REGIONS];
   int n_regions, n;
   int64_t tasks;             // per pair
-  int32_t src[PAGE_COPY_PAIRS], dst[PAGE_COPY_PAIRS];
+  int32_t src[PAIRS], dst[PAIRS];
 };
 
 // One block per (pair, plane, 16 KB of the page).
-__global__ void __launch_bounds__(PAGE_COPY_THREADS) page_copy_kernel(const __grid_constant__ PageCopyParams p) {
+template <int PAIRS>
+__global__ void __launch_bounds__(PAGE_COPY_THREADS) page_copy_kernel(const __grid_constant__ PageCopyParams<PAIRS> p) {
   const int64_t total = p.tasks * p.n;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
     const int pair = int(t / p.tasks);
     int64_t in = t - pair * p.tasks;
     int ri = 0;
     while (ri + 1 < p.n_regions && in >= p.r[ri + 1].first) ++ri;
-    const PageCopyParams::Region& r = p.r[ri];
+    const PageCopyRegion& r = p.r[ri];
     in -= r.first;
     const int64_t plane = in / r.chunks;
     const int64_t at = (in - plane * r.chunks) * PAGE_COPY_CHUNK;

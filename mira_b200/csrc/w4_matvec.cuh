@@ -58,7 +58,7 @@ __device__ __forceinline__ float w4_steps(const W4Params& p, float y, int m, int
     float o = st.scalar;
     if (st.operand == MIRA_OPND_CHANNEL) o = __ldg(st.ptr + n);
     else if (st.operand == MIRA_OPND_ROW) o = __ldg(st.ptr + m);
-    else if (st.operand == MIRA_OPND_FULL) o = __ldg(st.ptr + int64_t(m) * st.ld + n);
+    else if (st.operand == MIRA_OPND_FULL) o = st.ptr[int64_t(m) * st.ld + n];      // may be the output itself
     y = st.swapped ? apply_binary(st.op, o, y) : apply_binary(st.op, y, o);
   }
   return y;
