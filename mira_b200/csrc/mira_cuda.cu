@@ -2294,43 +2294,46 @@ static int w4_nb(int x_dtype, int m) {
 static int w4_gs(int64_t group) { return group % 256 == 0 ? 8 : group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1; }
 
 // Row tiles of a block, blocks along k, and stages of the panel of x.  More row tiles share one panel
-// and need less joining, fewer divide the rows more evenly; cuts along k do both at the price of a
-// second pass over the sums.  The choice is the least of what a block brings in, in bytes per SM: its
-// weights and x, and for cut sums about what an SM could read in the time of writing, signalling and
-// adding them (1.5 us at 50 bytes a clock).  `gs` as for the kernel; 1 holds for every group.
+// and need less joining, fewer divide the rows more evenly; cuts along k do both and let x fit one panel,
+// at the price of a second pass over the sums.  The choice is the least time by a rough count in bytes
+// that an SM could bring in meanwhile (at 50 a clock, 95 KB/us): a block's weights and x, 1 us for every
+// panel after the first, 1.2 us and the reading of all parts for cut sums.  `gs` as for the kernel; 1
+// holds for every group.  (16 rows of bf16 through 4096 x 4096: 22.5 us with four panels, see below.)
 static int w4_plan(int sm_count, int gs, W4Params& p) {
   const int at_once = sm_count * W4_BLOCKS;
   const int pass = w4_rows(p.x_dtype), rows = p.m < pass ? p.m : pass, columns = rows * w4_pieces(p.x_dtype);
+  const int64_t passes = (int64_t(p.m) + pass - 1) / pass;
   const int room = W4_SMEM - w4_fixed(w4_nb(p.x_dtype, rows), gs);
   const int most = (room / columns - 64) / (W4_STAGE_K * 2);        // stages that fit the panel
   const int stages = (p.k + W4_STAGE_K - 1) / W4_STAGE_K;
   const int64_t tiles = (int64_t(p.n) + 15) / 16;
   int64_t best = INT64_MAX;
-  for (int cuts = 1; cuts <= (p.m <= pass ? 8 : 1); cuts *= 2) {
+  for (int cuts = 1; cuts <= 32; cuts *= 2) {
     const int per = (stages + cuts - 1) / cuts;
     if (cuts > 1 && (cuts - 1) * per >= stages) break;               // a cut without work
     for (int wr = W4_WARPS; wr >= 1; wr /= 2) {
       const int share = W4_WARPS / wr;
       if (share > most) break;
       const int64_t groups = (tiles + wr - 1) / wr;
-      const int64_t rounds = (groups * cuts + at_once - 1) / at_once;
-      const bool whole = most / share * share >= per;
+      const int64_t rounds = (groups * cuts * passes + at_once - 1) / at_once;
+      const int want = (per + share - 1) / share * share, fit = most / share * share;
+      const int64_t panels = (per + fit - 1) / fit;
       const int64_t weights = rounds * wr * 16 * per * (W4_STAGE_K / 2);
-      const int64_t x = int64_t(rows) * per * W4_STAGE_K * dt_size(p.x_dtype) * (whole ? 1 : rounds);
-      const int64_t cost = weights + x + (cuts > 1 ? 140000 : 0);
+      const int64_t x = (int64_t(rows) * per * W4_STAGE_K * dt_size(p.x_dtype) + (panels - 1) * 95000) * (panels == 1 ? 1 : rounds);
+      const int64_t join = cuts > 1 ? rounds * (115000 + int64_t(cuts) * rows * wr * 16 * 4) : 0;
+      const int64_t cost = weights + x + join;
       if (cost >= best) continue;
       best = cost;
       p.wr = wr;
       p.cuts = cuts;
       p.cut_stages = per;
-      const int want = (per + share - 1) / share * share, fit = most / share * share;
       p.panel = want < fit ? want : fit;
     }
   }
   return p.panel > 0 ? MIRA_CUDA_OK : set_error(MIRA_CUDA_EINVAL, "no room for the rows of x");
 }
 
-static int64_t w4_counters(int64_t n) { return round_up((n + 15) / 16 * 4, 256); }
+static int64_t w4_counters(int64_t m, int64_t n) { return round_up((m + 7) / 8 * ((n + 15) / 16) * 4, 256); }
 
 template <int XT, int NB, int GS, bool EXACT>
 static int launch_w4_kernel(DeviceState* dev, const W4Params& p) {
@@ -2345,7 +2348,7 @@ static int launch_w4_kernel(DeviceState* dev, const W4Params& p) {
   MIRA_CHECK_ARG(gy <= 65535, "matvec has too many rows");
   // as many blocks as run at once, each with the same number of row groups
   const int64_t at_once = int64_t(dev->sm_count) * W4_BLOCKS;
-  const int64_t rounds = (groups * p.cuts + at_once - 1) / at_once;
+  const int64_t rounds = (groups * p.cuts * gy + at_once - 1) / at_once;
   const dim3 grid(unsigned((groups + rounds - 1) / rounds), unsigned(gy), unsigned(p.cuts));
   kern<<<grid, W4_THREADS, w4_fixed(NB, GS) + columns * w4_pitch(p.panel), dev->stream>>>(p);
   return after_launch("w4_matvec_kernel");
@@ -2374,7 +2377,7 @@ extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k
       p.m = int(m); p.n = int(n); p.k = int(k); p.x_dtype = dtype;
       if (w4_plan(dev->sm_count, gs, p) == MIRA_CUDA_OK && p.cuts > cuts) cuts = p.cuts;
     }
-  return cuts > 1 ? w4_counters(n) + int64_t(cuts) * m * n * 4 : 0;
+  return cuts > 1 ? w4_counters(m, n) + int64_t(cuts) * m * n * 4 : 0;
 }
 
 extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
@@ -2418,10 +2421,10 @@ extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   if (rc != MIRA_CUDA_OK) return rc;
   if (p.cuts > 1) {
     MIRA_CHECK_ARG(a->workspace != nullptr && aligned_to(a->workspace, 16) &&
-                       a->workspace_bytes >= w4_counters(p.n) + int64_t(p.cuts) * p.m * p.n * 4,
+                       a->workspace_bytes >= w4_counters(p.m, p.n) + int64_t(p.cuts) * p.m * p.n * 4,
                    "workspace smaller than mira_cuda_w4_matvec_workspace()");
     p.counters = static_cast<int*>(a->workspace);
-    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + w4_counters(p.n));
+    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + w4_counters(p.m, p.n));
   }
   const int nb = w4_nb(p.x_dtype, p.m);
   switch (p.x_dtype) {

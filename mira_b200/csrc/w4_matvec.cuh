@@ -40,7 +40,7 @@ struct W4Params {
   int panel;                  // stages of x in shared memory, a multiple of 8 / wr
   int cuts, cut_stages;       // blocks along k and the stages of each
   float* part;                // [cut][m][n] sums of each cut
-  int* counters;              // [row group], zero between calls
+  int* counters;              // [pass over x][row group], zero between calls
   int x_vec;                  // rows of x can be read 16 bytes at a time
   int x_dtype, scale_dtype, out_dtype;
   int n_steps;
@@ -124,35 +124,21 @@ struct W4Unpack {
   }
 };
 
-// Eight values of a row of x from element k on (0 past the end), in the order of the fragments.
+// Eight values of a row of x from element k on (0 past the end), as they are: f32 in eight words, 16-bit
+// values in four.
 template <int XT>
-__device__ __forceinline__ void w4_stage_x(const W4Params& p, int row, int k, uint8_t* col, int pitch) {
-  if (XT == MIRA_DT_F32) {
-    const float* src = static_cast<const float*>(p.x) + row * p.ld_x + k;
-    float v[8];
+__device__ __forceinline__ void w4_load_x(const W4Params& p, int row, int k, uint32_t (&v)[XT == MIRA_DT_F32 ? 8 : 4]) {
+  if constexpr (XT == MIRA_DT_F32) {
+    const uint32_t* src = static_cast<const uint32_t*>(p.x) + row * p.ld_x + k;
     if (p.x_vec && k + 8 <= p.k) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(src)), b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? __ldg(src + i) : 0.0f;
+      for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? __ldg(src + i) : 0u;
     }
-    uint32_t c[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t h0, m0, l0, h1, m1, l1;
-      split3_bf16(v[i], h0, m0, l0);
-      split3_bf16(v[i + 4], h1, m1, l1);
-      c[0][i] = __byte_perm(h0, h1, 0x7632);
-      c[1][i] = __byte_perm(m0, m1, 0x7632);
-      c[2][i] = __byte_perm(l0, l1, 0x7632);
-    }
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      *reinterpret_cast<uint4*>(col + j * pitch) = make_uint4(c[j][0], c[j][1], c[j][2], c[j][3]);
   } else {
     const uint16_t* src = static_cast<const uint16_t*>(p.x) + row * p.ld_x + k;
-    uint32_t v[4];      // pairs (0, 1), (2, 3), ..
     if (p.x_vec && k + 8 <= p.k) {
       const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -162,6 +148,27 @@ __device__ __forceinline__ void w4_stage_x(const W4Params& p, int row, int k, ui
         v[i] = (k + 2 * i < p.k ? uint32_t(__ldg(src + 2 * i)) : 0u) |
                (k + 2 * i + 1 < p.k ? uint32_t(__ldg(src + 2 * i + 1)) << 16 : 0u);
     }
+  }
+}
+
+// The same in the order of the fragments, to a column of the panel (f32: to its three columns).
+template <int XT>
+__device__ __forceinline__ void w4_store_x(const uint32_t (&v)[XT == MIRA_DT_F32 ? 8 : 4], uint8_t* col, int piece_step) {
+  if constexpr (XT == MIRA_DT_F32) {
+    uint32_t c[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h0, m0, l0, h1, m1, l1;
+      split3_bf16(__uint_as_float(v[i]), h0, m0, l0);
+      split3_bf16(__uint_as_float(v[i + 4]), h1, m1, l1);
+      c[0][i] = __byte_perm(h0, h1, 0x7632);
+      c[1][i] = __byte_perm(m0, m1, 0x7632);
+      c[2][i] = __byte_perm(l0, l1, 0x7632);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      *reinterpret_cast<uint4*>(col + j * piece_step) = make_uint4(c[j][0], c[j][1], c[j][2], c[j][3]);
+  } else {
     *reinterpret_cast<uint4*>(col) = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632),
                                                 __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632));
   }
@@ -268,10 +275,20 @@ __global__ void __launch_bounds__(W4_THREADS, W4_BLOCKS) w4_matvec_kernel(const 
       const int in_panel = min(p.panel, stages - p0);
       if (round == 0 || p.panel < stages) {       // else all of x is there already
         __syncthreads();
-        const int words = in_panel * (W4_STAGE_K / 8);
-        for (int e = threadIdx.x; e < rows * words; e += W4_THREADS) {
-          const int r = e / words, word = e - r * words;
-          w4_stage_x<XT>(p, m0 + r, (first + p0) * W4_STAGE_K + word * 8, panel + r * row_step + word * 16, piece_step);
+        const int words = in_panel * (W4_STAGE_K / 8), total = rows * words;
+        constexpr int FLY = XT == MIRA_DT_F32 ? 2 : 4;        // loads in flight
+        for (int e0 = threadIdx.x; e0 < total; e0 += FLY * W4_THREADS) {
+          uint32_t v[FLY][XT == MIRA_DT_F32 ? 8 : 4];
+#pragma unroll
+          for (int u = 0; u < FLY; ++u) {
+            const int e = e0 + u * W4_THREADS, r = e / words;
+            if (e < total) w4_load_x<XT>(p, m0 + r, (first + p0) * W4_STAGE_K + (e - r * words) * 8, v[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < FLY; ++u) {
+            const int e = e0 + u * W4_THREADS, r = e / words;
+            if (e < total) w4_store_x<XT>(v[u], panel + r * row_step + (e - r * words) * 16, piece_step);
+          }
         }
         __syncthreads();
       }
@@ -342,25 +359,49 @@ __global__ void __launch_bounds__(W4_THREADS, W4_BLOCKS) w4_matvec_kernel(const 
       for (int q = JOIN - 1; q >= 0; --q)
         for (int j = 0; j < wk_n; ++j) y += red[((j * p.wr + w0) * OB * 8 + r * JOIN + q) * 16 + (c & 15)];
       if (p.cuts == 1) dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y, m0 + r, n));
-      else p.part[(int64_t(blockIdx.z) * p.m + r) * p.n + n] = y;
+      else p.part[(int64_t(blockIdx.z) * p.m + m0 + r) * p.n + n] = y;
     }
-    if (p.cuts > 1) {       // one pass over the rows: m <= ROWS
+    if (p.cuts > 1) {
       const int group = int(blockIdx.x) + round * int(gridDim.x);
-      __threadfence();
+      int* counter = p.counters + int64_t(blockIdx.y) * row_groups + group;
       __syncthreads();
-      if (threadIdx.x == 0) s_last = atomicAdd(p.counters + group, 1) == p.cuts - 1;
+      if (threadIdx.x == 0) {
+        __threadfence();      // the whole block's sums, by the barrier before
+        s_last = atomicAdd(counter, 1) == p.cuts - 1;
+      }
       __syncthreads();
       if (s_last) {
         __threadfence();
         const int width = p.wr * 16, at = group * width;
-        for (int e = threadIdx.x; e < rows * width; e += W4_THREADS) {
-          const int r = e / width, n = at + e - r * width;
-          if (n >= p.n) continue;
-          float y = 0.0f;
-          for (int z = 0; z < p.cuts; ++z) y += __ldcg(p.part + (int64_t(z) * p.m + r) * p.n + n);
-          dt_store(p.out, r * p.ld_out + n, p.out_dtype, w4_steps(p, y, r, n));
+        constexpr int FLY = 4;       // results at a time, as many parts of each
+        const int64_t step = int64_t(p.m) * p.n;
+        for (int e0 = threadIdx.x; e0 < rows * width; e0 += FLY * W4_THREADS) {
+          float y[FLY];
+          const float* from[FLY];
+#pragma unroll
+          for (int u = 0; u < FLY; ++u) {
+            const int e = e0 + u * W4_THREADS, r = e / width, n = at + e - r * width;
+            from[u] = e < rows * width && n < p.n ? p.part + int64_t(m0 + r) * p.n + n : nullptr;
+            y[u] = 0.0f;
+          }
+          for (int z0 = 0; z0 < p.cuts; z0 += 4) {      // added in order
+            float x[FLY][4];
+#pragma unroll
+            for (int u = 0; u < FLY; ++u)
+#pragma unroll
+              for (int z = 0; z < 4; ++z) x[u][z] = from[u] != nullptr && z0 + z < p.cuts ? __ldcg(from[u] + (z0 + z) * step) : 0.0f;
+#pragma unroll
+            for (int u = 0; u < FLY; ++u)
+#pragma unroll
+              for (int z = 0; z < 4; ++z) y[u] += x[u][z];
+          }
+#pragma unroll
+          for (int u = 0; u < FLY; ++u) {
+            const int e = e0 + u * W4_THREADS, r = e / width, n = at + e - r * width;
+            if (from[u] != nullptr) dt_store(p.out, (m0 + r) * p.ld_out + n, p.out_dtype, w4_steps(p, y[u], m0 + r, n));
+          }
         }
-        if (threadIdx.x == 0) p.counters[group] = 0;
+        if (threadIdx.x == 0) *counter = 0;
       }
     }
   }
