@@ -12,8 +12,9 @@
 //     2t + 9; pairs of tokens of one element, a byte permutation each, are left fragments with rows
 //     (element i, g) and (element i + 1, g).  P^T is S^T's accumulators, packed and transposed in 8 x 8
 //     blocks by movmatrix.
-// Exactness: q enters as one value of the pages' type where it has that type, else as three whose sum
-// it is; 8-bit codes become exact f16 values.  p is f32 and enters as PP values that agree with it to 16
+// Exactness: q enters as one value of the pages' type where it has that type, else as three bf16 values
+// whose sum it is, or as two f16 values that agree with it to 2^-22 of the head's largest element; 8-bit
+// codes become exact f16 values.  p is f32 and enters as PP values that agree with it to 16
 // bits or more (see PaMma), the row's sum l is of the f32 values.
 #pragma once
 #include <cstdint>
@@ -24,7 +25,7 @@
 namespace mira {
 
 // T: the pages' element; DHP: head dimension rounded up to 64, 128 or 256; VB: bytes per access of a
-// key row; QP: values per query element, 1 or 3; NH: blocks of eight heads.
+// key row; QP: values per query element, 1, or 3 (bf16) or 2 (f16); NH: blocks of eight heads.
 template <typename T, int DHP, int VB, int QP, int NH>
 struct PaMma {
   static constexpr bool I8 = sizeof(T) == 1;
@@ -38,10 +39,11 @@ struct PaMma {
   static constexpr int NT = DHP / 16;                                      // tiles of O
   static constexpr int TT = (DHP * int(sizeof(T)) <= 128) ? 2 : 1;         // runs of 16 tokens per step
   static constexpr int TILE = 16 * TT;                                     // tokens of a step
-  // p: bf16 values have 8 bits, f16 ones 11.  16-bit results: 16 and 22 bits; f32 results (QP == 3): 24
-  // and 22, whose error of 2^-22 of the largest weight is that of an f32 sum of a few terms.  In f16,
-  // p is carried times 2^8: the smallest f16 is then 2^-32 of the largest weight.
-  static constexpr int PP = BF16 && QP == 3 ? 3 : 2;
+  // p: bf16 values have 8 bits, f16 ones 11.  16-bit results: 16 and 22 bits; f32 results (QP > 1): 24
+  // and 22, whose error of 2^-22 of the largest weight is that of an f32 sum of a few terms; the same
+  // goes for the two f16 values of a query element.  In f16, p is carried times 2^8: the smallest f16 is
+  // then 2^-32 of the largest weight.
+  static constexpr int PP = BF16 && QP > 1 ? 3 : 2;
   static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
   static constexpr int K_BYTES = TT * 2 * KL * 32 * VB, V_BYTES = TT * 4 * VL * 32 * VBV;    // of a step
   static constexpr int STEP = K_BYTES + V_BYTES + (I8 ? 2 * 32 * 4 : 0);      // 8-bit pages: and the scales
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
           top = fmaxf(top, fabsf(x[i][e]));
         }
       float up = 1.0f;
-      if (QP == 3 && !C::BF16) {
+      if (QP > 1 && !C::BF16) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int e = int(__float_as_uint(top) >> 23);      // 2^(e - 127) <= top
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
         uint32_t f[2][QP];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (C::BF16 && QP == 3) {
+          if constexpr (C::BF16 && QP == 3) {
             uint32_t a[3], b[3];
             split3_bf16(x[i][2 * j], a[0], a[1], a[2]);
             split3_bf16(x[i][2 * j + 1], b[0], b[1], b[2]);
