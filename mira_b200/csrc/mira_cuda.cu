@@ -2022,7 +2022,7 @@ static int launch_append_from(DeviceState* dev, AppendParams& p, int dtype, bool
     case MIRA_DT_F32: return vec ? launch_append<SRC, MIRA_DT_F32, true>(dev, p) : launch_append<SRC, MIRA_DT_F32, false>(dev, p);
     case MIRA_DT_F16: return vec ? launch_append<SRC, MIRA_DT_F16, true>(dev, p) : launch_append<SRC, MIRA_DT_F16, false>(dev, p);
     case MIRA_DT_BF16: return vec ? launch_append<SRC, MIRA_DT_BF16, true>(dev, p) : launch_append<SRC, MIRA_DT_BF16, false>(dev, p);
-    default: return launch_append<SRC, MIRA_DT_I8, false>(dev, p);
+    default: return vec ? launch_append<SRC, MIRA_DT_I8, true>(dev, p) : launch_append<SRC, MIRA_DT_I8, false>(dev, p);
   }
 }
 
@@ -2120,8 +2120,9 @@ extern "C" int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* re
   } catch (const std::exception&) {
     return set_error(MIRA_CUDA_EINVAL, "out of host memory while checking the page lists");
   }
-  return n <= PAGE_COPY_FEW ? launch_page_copy<PAGE_COPY_FEW>(dev, region, int(n_regions), tasks, n, src, dst)
-                            : launch_page_copy<PAGE_COPY_MANY>(dev, region, int(n_regions), tasks, n, src, dst);
+  if (n <= PAGE_COPY_FEW) return launch_page_copy<PAGE_COPY_FEW>(dev, region, int(n_regions), tasks, n, src, dst);
+  if (n <= PAGE_COPY_SOME) return launch_page_copy<PAGE_COPY_SOME>(dev, region, int(n_regions), tasks, n, src, dst);
+  return launch_page_copy<PAGE_COPY_MANY>(dev, region, int(n_regions), tasks, n, src, dst);
 }
 
 namespace mira {
@@ -2133,11 +2134,9 @@ static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch
 // Rows of any alignment.
 template <typename T>
 static int launch_paged_any(DeviceState* dev, PagedAttnParams& p) {
-  using C = PaCfg<T, 256, 1, int(sizeof(T))>;
-  auto kern = paged_attention_any_kernel<T, 256, 1, int(sizeof(T))>;
   p.head_blocks = p.group;
   p.units = p.kv.kv_heads * p.head_blocks;
-  kern<<<unsigned(dev->sm_count * 2), C::WARPS * 32, C::SMEM, dev->stream>>>(p);
+  paged_attention_any_kernel<T><<<unsigned(dev->sm_count * 2), PaAny::WARPS * 32, PaAny::SMEM, dev->stream>>>(p);
   return after_launch("paged_attention_any_kernel");
 }
 
@@ -2301,7 +2300,8 @@ static int w4_gs(int64_t group) { return group % 256 == 0 ? 8 : group % 128 == 0
 // at the price of a second pass over the sums.  The choice is the least time by a rough count in bytes
 // that an SM could bring in meanwhile (at 50 a clock, 95 KB/us): a block's weights and x, 1 us for every
 // panel after the first, 1.2 us and the reading of all parts for cut sums.  `gs` as for the kernel; 1
-// holds for every group.  (16 rows of bf16 through 4096 x 4096: 22.5 us with four panels, see below.)
+// holds for every group.  (16 rows of bf16 through 4096 x 4096: 22.5 us in four panels without cuts, 14.4 to
+// 16.6 with them; 11 rows of f32, 75 x 11116: 59 and 22 us.)
 static int w4_plan(int sm_count, int gs, W4Params& p) {
   const int at_once = sm_count * W4_BLOCKS;
   const int pass = w4_rows(p.x_dtype), rows = p.m < pass ? p.m : pass, columns = rows * w4_pieces(p.x_dtype);
@@ -2371,7 +2371,7 @@ static int launch_w4(DeviceState* dev, const W4Params& p, int64_t group) {
 
 extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k) {
   DeviceState* dev = current_device();
-  if (dev == nullptr || m <= 0 || m > INT32_MAX || n <= 0 || n > INT32_MAX || k <= 0 || k > (1 << 30)) return 0;
+  if (dev == nullptr || m <= 0 || m > INT32_MAX || n <= 0 || n > (1 << 30) || k <= 0 || k > (1 << 30)) return 0;
   int cuts = 1;
   for (int dtype : {MIRA_DT_F32, MIRA_DT_F16, MIRA_DT_BF16})
     for (int gs = 1; gs <= 8; gs *= 2) {
@@ -2386,7 +2386,7 @@ extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k
 extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   MIRA_GET_DEVICE(dev);
   MIRA_CHECK_ARG(a != nullptr, "null matvec descriptor");
-  MIRA_CHECK_ARG(a->m >= 0 && a->m <= INT32_MAX && a->n >= 0 && a->n <= INT32_MAX && a->k > 0 && a->k <= (1 << 30),
+  MIRA_CHECK_ARG(a->m >= 0 && a->m <= INT32_MAX && a->n >= 0 && a->n <= (1 << 30) && a->k > 0 && a->k <= (1 << 30),
                  "bad matvec shape");
   MIRA_CHECK_ARG(a->group > 0 && a->group % 32 == 0, "the group must be a multiple of 32");
   MIRA_CHECK_ARG(row_dtype(a->x_dtype) && row_dtype(a->scale_dtype) && row_dtype(a->out_dtype),

@@ -171,25 +171,6 @@ __device__ __forceinline__ bool pa_part(const PagedAttnParams& p, PaWork& w) {
   return false;
 }
 
-// ---------------------------------------------------------------- rows of the pages
-
-// VB bytes of a row as one access; elements of T as f32.
-template <int VB> struct PaVec;
-template <> struct PaVec<16> { using type = uint4; };
-template <> struct PaVec<8> { using type = uint2; };
-template <> struct PaVec<4> { using type = uint32_t; };
-template <> struct PaVec<2> { using type = uint16_t; };
-template <> struct PaVec<1> { using type = uint8_t; };
-
-template <typename T, int VB>
-__device__ __forceinline__ void pa_unpack(const typename PaVec<VB>::type& raw, float (&x)[VB / sizeof(T)]) {
-  constexpr int VE = VB / int(sizeof(T));
-  T e[VE];
-  memcpy(e, &raw, VB);
-#pragma unroll
-  for (int i = 0; i < VE; ++i) x[i] = static_cast<float>(e[i]);
-}
-
 // ---------------------------------------------------------------- the end of a part
 
 // Barrier among the first n threads of the block, those that compute and join.
@@ -498,9 +479,15 @@ __device__ __forceinline__ void pa_feed(const PagedAttnParams& p, PaWork& w, con
 // ---------------------------------------------------------------- f32 pages
 
 // DHP: head dimension rounded up to 32, 64, 128 or 256; GP: query heads that share a pass over the rows.
+// Bound: the visible rows are read once, 8 dh bytes a token and head; a score and its value row take 4 dh
+// operations, which the FMA units do in the shadow of the loads for one query head per key head and
+// no longer for four.  (Products on the tensor path need three bf16 values per element of k and v: six
+// bytes for four, and six products for one.)
 // A row is spread over LPR lanes, 16 bytes each, a warp takes TPS rows at a time and U times that in a
 // step.  The LPR partial sums of the step's U GP scores are added crosswise, each exchange halving the
 // number of scores a lane carries, so that a score's softmax is worked out in few lanes, not in all.
+// 64 sequences of up to 1024 tokens, 12 heads of 64 (205 MB): 50.8 us, 4.0 TB/s; what is above the bytes' 31 us
+// is mostly the launch, the dealing out, and the beginnings and ends of the 768 units' parts.
 template <int DHP, int GP>
 struct PaF32 {
   static constexpr int LPR = DHP / 4 < 32 ? DHP / 4 : 32;
@@ -750,177 +737,91 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
 
 // ---------------------------------------------------------------- rows that are not 16-byte aligned
 
-// T: the pages' element, one per access; the head dimension is taken as 256 and each query head reads the
-// rows anew (the repeats come from the caches).  Right for every stride and size, and slow: 16-byte
-// aligned rows go to the other kernels.
-template <typename T, int DHP, int GP, int VB>
-struct PaCfg {
-  static constexpr int WARPS = 8;
-  static constexpr int VE = VB / int(sizeof(T));            // elements of an access
-  static constexpr int LPR = DHP / VE < 32 ? DHP / VE : 32; // lanes of a row
-  static constexpr int NV = DHP / (VE * LPR);               // accesses of a lane per row
-  static constexpr int EPL = VE * NV;                       // elements of a lane
-  static constexpr int TPS = 32 / LPR;                      // rows of a warp access
-  static constexpr int U = NV > 1 ? 2 : 4;                  // rows in flight per lane
-  static constexpr int ROWS = TPS * U;                      // rows of a warp step
-  static constexpr int TILE = WARPS * ROWS;
-  static constexpr int SMEM = pa_finish_floats(WARPS, GP, DHP) * 4;
+// One element per access, eight a lane (the head dimension is taken as 256), two rows of a warp in flight;
+// each query head reads the rows anew (the repeats come from the caches).  Right for every stride and
+// size, and slow, bound by its narrow loads: 16-byte aligned rows go to the other kernels.
+struct PaAny {
+  static constexpr int WARPS = 8, EPL = 8, DHP = 32 * EPL, U = 2, TILE = WARPS * U;
+  static constexpr int SMEM = pa_finish_floats(WARPS, 1, DHP) * 4;
 };
 
-template <typename T, int DHP, int GP, int VB>
-__global__ void __launch_bounds__(PaCfg<T, DHP, GP, VB>::WARPS * 32)
-    paged_attention_any_kernel(const __grid_constant__ PagedAttnParams p) {
-  using C = PaCfg<T, DHP, GP, VB>;
-  using V = typename PaVec<VB>::type;
+template <typename T>
+__global__ void __launch_bounds__(PaAny::WARPS * 32) paged_attention_any_kernel(const __grid_constant__ PagedAttnParams p) {
+  using C = PaAny;
   constexpr bool I8 = sizeof(T) == 1;
   extern __shared__ __align__(16) float pa_floats[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane % C::LPR, slot_of_lane = lane / C::LPR;
   PaWork w;
   if (!pa_begin<C::TILE>(p, 1, w)) return;
   while (pa_part<C::TILE>(p, w)) {
-    const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
-
-    // queries of the unit, scaled
-    float q[GP][C::EPL];
+    const int kvh = w.unit / p.head_blocks, h = kvh * p.group + (w.unit - kvh * p.head_blocks);
+    float q[C::EPL], acc[C::EPL], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int gi = 0; gi < GP; ++gi)
-#pragma unroll
-      for (int j = 0; j < C::NV; ++j)
-#pragma unroll
-        for (int e = 0; e < C::VE; ++e) {
-          const int d = (sub + j * C::LPR) * C::VE + e;
-          q[gi][j * C::VE + e] = (g0 + gi < p.group && d < p.kv.dh)
-              ? dt_load(p.q, w.b * p.qs[0] + (kvh * p.group + g0 + gi) * p.qs[1] + d * p.qs[2], p.q_dtype) * p.scale_log2
-              : 0.0f;
-        }
-    float acc[GP][C::EPL], m[GP], l[GP];
-#pragma unroll
-    for (int gi = 0; gi < GP; ++gi) {
-      m[gi] = -INFINITY;
-      l[gi] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < C::EPL; ++e) acc[gi][e] = 0.0f;
+    for (int e = 0; e < C::EPL; ++e) {
+      const int d = lane + 32 * e;
+      q[e] = d < p.kv.dh ? dt_load(p.q, w.b * p.qs[0] + h * p.qs[1] + d * p.qs[2], p.q_dtype) * p.scale_log2 : 0.0f;
+      acc[e] = 0.0f;
     }
     const int32_t* trow = p.kv.table + w.b * p.kv.table_ld;
     const T* kb = static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1];
     const T* vb = static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1];
-
-    // where the lane's rows of a step are; looked up a step ahead of their loads
-    int page[C::U], slot[C::U];
-    bool ok[C::U];
-    auto look = [&](int w0) {
+    for (int i0 = w.t0 + warp * C::U; i0 < w.t1; i0 += C::TILE) {
+      T k[C::U][C::EPL], v[C::U][C::EPL];
+      float ks[C::U], vs[C::U];
+      bool ok[C::U];
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
-        const int i = w0 + u * C::TPS + slot_of_lane;
-        page[u] = slot[u] = 0;
-        ok[u] = i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page[u], slot[u]);
-      }
-    };
-    look(w.t0 + warp * C::ROWS);
-    for (int w0 = w.t0 + warp * C::ROWS; w0 < w.t1; w0 += C::TILE) {
-      V kr[C::U][C::NV], vr[C::U][C::NV];
-      float ksc[C::U], vsc[C::U];
-      bool now[C::U];
+        const int i = i0 + u;
+        int page = 0, slot = 0;
+        ok[u] = i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page, slot);
+        const T* kp = kb + page * p.kv.kst[0] + slot * p.kv.kst[2];
+        const T* vp = vb + page * p.kv.vst[0] + slot * p.kv.vst[2];
 #pragma unroll
-      for (int u = 0; u < C::U; ++u) {
-        now[u] = ok[u];
-        const T* kp = kb + page[u] * p.kv.kst[0] + slot[u] * p.kv.kst[2];
-        const T* vp = vb + page[u] * p.kv.vst[0] + slot[u] * p.kv.vst[2];
-#pragma unroll
-        for (int j = 0; j < C::NV; ++j) {
-          const int d = (sub + j * C::LPR) * C::VE;
+        for (int e = 0; e < C::EPL; ++e) {
+          const int d = lane + 32 * e;
           const bool in = ok[u] && d < p.kv.dh;
-          kr[u][j] = in ? __ldg(reinterpret_cast<const V*>(kp + d)) : V{};
-          vr[u][j] = in ? __ldg(reinterpret_cast<const V*>(vp + d)) : V{};
+          k[u][e] = in ? kp[d] : T{};
+          v[u][e] = in ? vp[d] : T{};
         }
         if (I8) {
-          ksc[u] = ok[u] ? __ldg(p.kv.ks + page[u] * p.kv.kss[0] + kvh * p.kv.kss[1] + slot[u] * p.kv.kss[2]) : 0.0f;
-          vsc[u] = ok[u] ? __ldg(p.kv.vs + page[u] * p.kv.vss[0] + kvh * p.kv.vss[1] + slot[u] * p.kv.vss[2]) : 0.0f;
+          ks[u] = ok[u] ? p.kv.ks[page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2]] : 0.0f;
+          vs[u] = ok[u] ? p.kv.vs[page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2]] : 0.0f;
         }
       }
-      look(w0 + C::TILE);
-      float s[C::U][GP];
+      float s[C::U], top = m;
 #pragma unroll
       for (int u = 0; u < C::U; ++u) {
+        s[u] = 0.0f;
 #pragma unroll
-        for (int gi = 0; gi < GP; ++gi) s[u][gi] = 0.0f;
+        for (int e = 0; e < C::EPL; ++e) s[u] = fmaf(q[e], static_cast<float>(k[u][e]), s[u]);
 #pragma unroll
-        for (int j = 0; j < C::NV; ++j) {
-          float x[C::VE];
-          pa_unpack<T, VB>(kr[u][j], x);
-#pragma unroll
-          for (int gi = 0; gi < GP; ++gi)
-#pragma unroll
-            for (int e = 0; e < C::VE; ++e) s[u][gi] = fmaf(q[gi][j * C::VE + e], x[e], s[u][gi]);
-        }
-#pragma unroll
-        for (int gi = 0; gi < GP; ++gi) {
-#pragma unroll
-          for (int o = 1; o < C::LPR; o <<= 1) s[u][gi] += __shfl_xor_sync(0xffffffffu, s[u][gi], o);
-          if (I8) s[u][gi] *= ksc[u];
-          if (!now[u]) s[u][gi] = -INFINITY;
-        }
+        for (int o = 1; o < 32; o <<= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+        if (I8) s[u] *= ks[u];
+        if (!ok[u]) s[u] = -INFINITY;
+        top = fmaxf(top, s[u]);
       }
+      const float safe = top == -INFINITY ? 0.0f : top, fade = exp2f(m - safe);
+      m = top;
+      l *= fade;
 #pragma unroll
-      for (int gi = 0; gi < GP; ++gi) {
-        float top = m[gi];
+      for (int e = 0; e < C::EPL; ++e) acc[e] *= fade;
 #pragma unroll
-        for (int u = 0; u < C::U; ++u) top = fmaxf(top, s[u][gi]);
-        const float safe = top == -INFINITY ? 0.0f : top;
-        const float fade = exp2f(m[gi] - safe);
-        m[gi] = top;
-        l[gi] *= fade;
+      for (int u = 0; u < C::U; ++u) {
+        float x = exp2f(s[u] - safe);
+        l += x;
+        if (I8) x *= vs[u];
 #pragma unroll
-        for (int e = 0; e < C::EPL; ++e) acc[gi][e] *= fade;
-#pragma unroll
-        for (int u = 0; u < C::U; ++u) {
-          s[u][gi] = exp2f(s[u][gi] - safe);
-          l[gi] += s[u][gi];
-          if (I8) s[u][gi] *= vsc[u];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < C::U; ++u)
-#pragma unroll
-        for (int j = 0; j < C::NV; ++j) {
-          float x[C::VE];
-          pa_unpack<T, VB>(vr[u][j], x);
-#pragma unroll
-          for (int gi = 0; gi < GP; ++gi)
-#pragma unroll
-            for (int e = 0; e < C::VE; ++e)
-              acc[gi][j * C::VE + e] = fmaf(s[u][gi], x[e], acc[gi][j * C::VE + e]);
-        }
-    }
-
-    // join the warp's lane groups
-    float* mine = pa_floats + warp * pa_triple(GP, DHP);
-#pragma unroll
-    for (int gi = 0; gi < GP; ++gi) {
-#pragma unroll
-      for (int o = C::LPR; o < 32; o <<= 1) {
-        const float mo = __shfl_xor_sync(0xffffffffu, m[gi], o), lo = __shfl_xor_sync(0xffffffffu, l[gi], o);
-        const float top = fmaxf(m[gi], mo);
-        const float wa = pa_weight(m[gi], top), wb = pa_weight(mo, top);
-        l[gi] = l[gi] * wa + lo * wb;
-        m[gi] = top;
-#pragma unroll
-        for (int e = 0; e < C::EPL; ++e)
-          acc[gi][e] = acc[gi][e] * wa + __shfl_xor_sync(0xffffffffu, acc[gi][e], o) * wb;
-      }
-      if (slot_of_lane == 0) {
-#pragma unroll
-        for (int j = 0; j < C::NV; ++j)
-#pragma unroll
-          for (int e = 0; e < C::VE; ++e) mine[pa_head(GP) + gi * DHP + (sub + j * C::LPR) * C::VE + e] = acc[gi][j * C::VE + e];
-      }
-      if (lane == 0) {
-        mine[gi] = m[gi];
-        mine[GP + gi] = l[gi];
+        for (int e = 0; e < C::EPL; ++e) acc[e] = fmaf(x, static_cast<float>(v[u][e]), acc[e]);
       }
     }
-    pa_finish<DHP>(p, w, pa_floats, C::WARPS, GP, kvh * p.group + g0, min(GP, p.group - g0));
+    float* mine = pa_floats + warp * pa_triple(1, C::DHP);
+#pragma unroll
+    for (int e = 0; e < C::EPL; ++e) mine[pa_head(1) + lane + 32 * e] = acc[e];
+    if (lane == 0) {
+      mine[0] = m;
+      mine[1] = l;
+    }
+    pa_finish<C::DHP>(p, w, pa_floats, C::WARPS, 1, h, 1);
     w.cur = w.end;
   }
 }

@@ -91,7 +91,9 @@ struct AppendParams {
 // Bound: the new rows are read and written once (f32 into bf16: 6 bytes an element).  A warp takes one
 // row, looks its sequence and its slot up once (the sequence by bisection of row_start, one probe per
 // lane and turn) and copies all heads' keys and values: 16-byte reads where the rows allow, four in
-// flight per lane, written in the width that they convert to.
+// flight per lane, written in the width that they convert to.  24 prompts of up to 4096 tokens, 8 heads of
+// 128, f32 into bf16 (518 MB): 86 us, 6.06 TB/s, 92% of the copy rate (one thread per element and look-up:
+// 292 us).  64 rows of 12 heads of 64: 6.1 us, the time to launch it from the host.
 constexpr int APPEND_WARPS = 8;
 
 template <int DT> struct AppendElem;
@@ -115,18 +117,44 @@ __device__ __forceinline__ typename AppendElem<DT>::type append_to(float x) {
 // Four elements as one access.
 template <class T> struct alignas(4 * sizeof(T)) Append4 { T v[4]; };
 
-// One head's row of 8-bit codes: scale = absmax / 127 and codes rint(x / scale), both IEEE divisions like
-// the int8 weights.
-__device__ __forceinline__ void append_codes(const void* src, int64_t so, int src_dtype, int8_t* dst, float* scale, int dh, int lane) {
-  float top = 0.0f;
-  for (int i = lane; i < dh; i += 32) top = np_maximum(top, fabsf(dt_load(src, so + i, src_dtype)));
+// W elements of a row from `at` on as f32 (0 past its end).
+template <int SRC, int W>
+__device__ __forceinline__ void append_get(const typename AppendElem<SRC>::type* row, int at, int dh, float (&x)[W]) {
+  using S = typename AppendElem<SRC>::type;
+  if constexpr (W == 4) {
+    Append4<S> e{};
+    if (at < dh) e = *reinterpret_cast<const Append4<S>*>(row + at);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = np_maximum(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < 4; ++i) x[i] = append_f32<SRC>(e.v[i]);
+  } else {
+    x[0] = at < dh ? append_f32<SRC>(row[at]) : 0.0f;
+  }
+}
+
+// 8-bit codes of one row of keys or values, held by `lanes` lanes (lane `sub`), W elements each and turn:
+// scale = absmax / 127 and codes rint(x / scale), both IEEE divisions like the int8 weights,
+// whose instructions are the limit: 49152 rows of 8 heads of 128 from f32, 176 us (2.9 TB/s); reciprocals with
+// the divisions left to the quotients near the middle of two codes were no faster.
+template <int W, int TURNS>
+__device__ __forceinline__ void append_codes(const float (&x)[TURNS][W], int8_t* dst, float* scale, int dh, int lanes, int sub, bool mine) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j)
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = np_maximum(top, fabsf(x[j][i]));
+  for (int o = lanes >> 1; o > 0; o >>= 1) top = np_maximum(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float s = top > 0.0f ? __fdiv_rn(top, 127.0f) : 1.0f;
-  if (lane == 0) *scale = s;
-  for (int i = lane; i < dh; i += 32) {
-    const float z = __fdiv_rn(dt_load(src, so + i, src_dtype), s);
-    dst[i] = static_cast<int8_t>(round_clip_i8(z) & 0xff);
+  if (!mine) return;
+  if (sub == 0) *scale = s;
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j) {
+    const int at = (sub + 32 * j) * W;
+    if (at >= dh) break;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) codes |= uint32_t(round_clip_i8(__fdiv_rn(x[j][i], s)) & 0xff) << (8 * i);
+    if constexpr (W == 4) *reinterpret_cast<uint32_t*>(dst + at) = codes;
+    else dst[at] = static_cast<int8_t>(codes);
   }
 }
 
@@ -168,11 +196,27 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __gr
     if (!paged_slot(kv, kv.table + b * kv.table_ld, pos, page, slot)) continue;
     const int64_t ko = page * kv.kst[0] + slot * kv.kst[2], vo = page * kv.vst[0] + slot * kv.vst[2];
     if constexpr (DST == MIRA_DT_I8) {
-      for (int h = 0; h < kv.kv_heads; ++h) {
-        append_codes(p.k_new, h * p.kn[0] + row * p.kn[1], SRC, static_cast<int8_t*>(kv.k) + ko + h * kv.kst[1],
-                     kv.ks + page * kv.kss[0] + h * kv.kss[1] + slot * kv.kss[2], kv.dh, lane);
-        append_codes(p.v_new, h * p.vn[0] + row * p.vn[1], SRC, static_cast<int8_t*>(kv.v) + vo + h * kv.vst[1],
-                     kv.vs + page * kv.vss[0] + h * kv.vss[1] + slot * kv.vss[2], kv.dh, lane);
+      // as many heads at once as the warp has room for
+      using S = typename AppendElem<SRC>::type;
+      constexpr int W = VEC ? 4 : 1, TURNS = MIRA_PAGED_DH_MAX / (32 * W);
+      int lanes = 32;
+      while (lanes > 1 && lanes / 2 * W >= kv.dh) lanes >>= 1;
+      const int sub = lane & (lanes - 1);
+      for (int h0 = 0; h0 < kv.kv_heads; h0 += 32 / lanes) {
+        const int h = min(h0 + lane / lanes, kv.kv_heads - 1);
+        const bool own = h0 + lane / lanes < kv.kv_heads;
+        const S* kf = static_cast<const S*>(p.k_new) + h * p.kn[0] + row * p.kn[1];
+        const S* vf = static_cast<const S*>(p.v_new) + h * p.vn[0] + row * p.vn[1];
+        float k[TURNS][W], v[TURNS][W];
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j) {
+          append_get<SRC, W>(kf, (sub + 32 * j) * W, kv.dh, k[j]);
+          append_get<SRC, W>(vf, (sub + 32 * j) * W, kv.dh, v[j]);
+        }
+        append_codes<W, TURNS>(k, static_cast<int8_t*>(kv.k) + ko + h * kv.kst[1],
+                               kv.ks + page * kv.kss[0] + h * kv.kss[1] + slot * kv.kss[2], kv.dh, lanes, sub, own);
+        append_codes<W, TURNS>(v, static_cast<int8_t*>(kv.v) + vo + h * kv.vst[1],
+                               kv.vs + page * kv.vss[0] + h * kv.vss[1] + slot * kv.vss[2], kv.dh, lanes, sub, own);
       }
     } else {
       using S = typename AppendElem<SRC>::type;
@@ -228,9 +272,10 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __gr
 // ---------------------------------------------------------------- page copies
 
 // Bound: the moved pages are read and written once.  The page ids travel in the kernel's parameters, so
-// that nothing has to be copied to the device before it: few of them in a small parameter block (a launch
-// with 4 KB of parameters takes the host about 2 us longer), many in several launches.
-constexpr int PAGE_COPY_FEW = 32, PAGE_COPY_MANY = 448;     // pairs per launch
+// that nothing has to be copied to the device before it: few of them in a small parameter block (5 pages of
+// 24 planes: 10.0 us a call; with 4 KB of parameters 12.5), up to 1000 in one launch.  700 pages of 16 KB in
+// 32 planes (734 MB read and written): 119.8 us, 6.13 TB/s, 93% of the copy rate (in two launches 125.6).
+constexpr int PAGE_COPY_FEW = 32, PAGE_COPY_SOME = 256, PAGE_COPY_MANY = 1000;     // pairs per launch
 constexpr int PAGE_COPY_CHUNK = 16384;    // bytes of one block's share of a page
 constexpr int PAGE_COPY_THREADS = 256;
 

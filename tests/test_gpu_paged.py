@@ -507,6 +507,12 @@ def test_page_copy(cuda_device, planes, pages, page_bytes, stride, n):
     np.testing.assert_array_equal(buf.download(pool.shape, np.uint8), want)
 
 
+@pytest.mark.parametrize("n", [31, 32, 33, 255, 256, 257, 999, 1000, 1001, 2001])
+def test_page_copy_around_launch_sizes(cuda_device, n):
+    """As many pages as one launch takes, one fewer and one more, and several launches."""
+    test_page_copy(cuda_device, 2, 2 * n + 3, 48, 64, n)
+
+
 def test_page_copy_several_regions(cuda_device):
     """Keys, values and their scales in one call, regions of different sizes and alignments."""
     K, DB = _k()
