@@ -2201,6 +2201,10 @@ static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
 template <typename T, int VB, int QP>
 static int launch_paged_mma_dh(DeviceState* dev, PagedAttnParams& p) {
   if (p.kv.dh <= 64) return p.group <= 8 ? launch_paged_mma<T, 64, VB, QP, 1>(dev, p) : launch_paged_mma<T, 64, VB, QP, 2>(dev, p);
+  if (p.kv.dh <= 96) {
+    constexpr int VB96 = sizeof(T) == 1 ? 8 : VB;      // four lanes' accesses have to divide a key row
+    return p.group <= 8 ? launch_paged_mma<T, 96, VB96, QP, 1>(dev, p) : launch_paged_mma<T, 96, VB96, QP, 2>(dev, p);
+  }
   if (p.kv.dh <= 128) return p.group <= 8 ? launch_paged_mma<T, 128, VB, QP, 1>(dev, p) : launch_paged_mma<T, 128, VB, QP, 2>(dev, p);
   return p.group <= 8 ? launch_paged_mma<T, 256, VB, QP, 1>(dev, p) : launch_paged_mma<T, 256, VB, QP, 2>(dev, p);
 }

@@ -32,7 +32,7 @@
 
 namespace mira {
 
-// T: the pages' element; DHP: head dimension rounded up to 64, 128 or 256; VB: bytes per access of a
+// T: the pages' element; DHP: head dimension rounded up to 64, 96, 128 or 256; VB: bytes per access of a
 // key row; QP: values per query element, 1, or 3 (bf16) or 2 (f16); NH: blocks of eight heads.
 template <typename T, int DHP, int VB, int QP, int NH>
 struct PaMma {
@@ -41,7 +41,8 @@ struct PaMma {
   static constexpr int KE = VB / int(sizeof(T));                           // elements of a key access
   static constexpr int KL = DHP / (4 * KE);                                // key accesses of a lane per token
   static constexpr int KS = DHP / 16;                                      // products along the head dimension
-  static constexpr int VBV = VB < DHP * int(sizeof(T)) / 8 ? VB : DHP * int(sizeof(T)) / 8;
+  // bytes per access of a value row: eight lanes' accesses have to divide it
+  static constexpr int VBV = DHP == 96 ? 4 * int(sizeof(T)) : VB < DHP * int(sizeof(T)) / 8 ? VB : DHP * int(sizeof(T)) / 8;
   static constexpr int VE = VBV / int(sizeof(T));
   static constexpr int VL = DHP / (8 * VE);                                // value accesses per token
   static constexpr int NT = DHP / 16;                                      // tiles of O
