@@ -2142,10 +2142,10 @@ static int launch_paged_any(DeviceState* dev, PagedAttnParams& p) {
 
 // Launches a kernel whose blocks feed a ring: `gp` heads per pass, `rows` of them used, `sm_warps`
 // warps per SM, `fixed` bytes of shared memory beside the ring (steps of `step` bytes) and the
-// triples.
+// triples; `even`: of eight warps four copy.
 template <class Kernel>
 static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, int sm_warps, int gp, int rows, int dhp, int step,
-                             int fixed, int* configured) {
+                             int fixed, bool even, int* configured) {
   p.head_blocks = (p.group + gp - 1) / gp;
   p.units = p.kv.kv_heads * p.head_blocks;
   // One block per SM where the sequences are fewer than the SMs: each is cut into parts for many SMs,
@@ -2153,10 +2153,10 @@ static int launch_paged_ring(DeviceState* dev, PagedAttnParams& p, Kernel kern, 
   // for one another at the end of a part.  The most warps that leave room for two steps each.
   const int blocks = int64_t(p.kv.batch) * p.units < dev->sm_count ? 1 : 2;
   const int room = (blocks == 1 ? 225 : 111) << 10;
-  static const int splits[][2] = {{12, 4}, {8, 4}, {6, 3}, {6, 2}, {4, 2}, {3, 1}, {2, 1}};      // computing, copying
+  static const int splits[][2] = {{12, 4}, {8, 4}, {6, 3}, {4, 4}, {6, 2}, {4, 2}, {3, 1}, {2, 1}};      // computing, copying
   int warps = 0, triples = 0;
   for (const auto& split : splits) {
-    if (split[0] + split[1] > sm_warps / blocks) continue;
+    if (split[0] + split[1] > sm_warps / blocks || (split[0] == split[1] && !even)) continue;
     warps = split[0];
     p.feeders = split[1];
     triples = pa_finish_floats(warps, rows, dhp) * 4;
@@ -2179,7 +2179,7 @@ template <int DHP, int GP>
 static int launch_paged_f32(DeviceState* dev, PagedAttnParams& p) {
   using C = PaF32<DHP, GP>;
   static int configured[kMaxDevices] = {};
-  return launch_paged_ring(dev, p, paged_attention_f32_kernel<DHP, GP>, C::WARPS, GP, GP, DHP, C::STEP, 0, configured);
+  return launch_paged_ring(dev, p, paged_attention_f32_kernel<DHP, GP>, C::WARPS, GP, GP, DHP, C::STEP, 0, C::EVEN, configured);
 }
 
 template <int GP>
@@ -2195,7 +2195,7 @@ static int launch_paged_mma(DeviceState* dev, PagedAttnParams& p) {
   using C = PaMma<T, DHP, VB, QP, NH>;
   static int configured[kMaxDevices] = {};
   return launch_paged_ring(dev, p, paged_attention_mma_kernel<T, DHP, VB, QP, NH>, C::WARPS, 8 * NH,
-                           p.group < 8 * NH ? p.group : 8 * NH, DHP, C::STEP, C::Q_BYTES, configured);
+                           p.group < 8 * NH ? p.group : 8 * NH, DHP, C::STEP, C::Q_BYTES, false, configured);
 }
 
 template <typename T, int VB, int QP>

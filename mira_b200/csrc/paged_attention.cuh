@@ -217,6 +217,11 @@ __device__ __forceinline__ void pa_add4(float4& a, const float4& x, float w) {
   a.w = fmaf(x.w, w, a.w);
 }
 
+// Where value 4 d4 of head h is in a triple in shared memory: groups of four are permuted so that the
+// warps' stores fall on different banks.
+template <int DHP>
+__device__ __forceinline__ int pa_at(int rows, int h, int d4) { return pa_head(rows) + h * DHP + (d4 ^ (h >> 1 & 3)) * 4; }
+
 // Joins the warps' triples of this part (sm: one triple per warp, `rows` of them used) and either
 // writes the result, when the block had the whole unit, or leaves the joined triple in the block's
 // slot; the last block of the unit to do so joins them all.  The block's first `warps` warps call it.
@@ -230,7 +235,7 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
   auto slot_of = [&](int64_t c) { return p.part + (c * 2 + (pa_lo(w.total, c, w.blocks) >= w.ts ? 0 : 1)) * triple; };
   float* mine = p.part + (int64_t(blockIdx.x) * 2 + (w.lo >= w.ts ? 0 : 1)) * triple;
   for (int e = threadIdx.x; e < live * (DHP / 4); e += threads) {
-    const int g = e / (DHP / 4), d = (e - g * (DHP / 4)) * 4;
+    const int g = e / (DHP / 4), d4 = e - g * (DHP / 4), d = d4 * 4;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll 4
@@ -240,7 +245,7 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
       const float* from = sm + i * triple;
       const float wt = pa_weight(from[g], top);
       sum += from[rows + g] * wt;
-      pa_add4(a, *reinterpret_cast<const float4*>(from + pa_head(rows) + g * DHP + d), wt);
+      pa_add4(a, *reinterpret_cast<const float4*>(from + pa_at<DHP>(rows, g, d4)), wt);
     }
     if (whole) {
       pa_write4(p, w.b, h0 + g, d, a, sum);
@@ -338,14 +343,13 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
 // ---------------------------------------------------------------- rows in flight
 
 // What hides the memory's latency is bytes in flight, about 64 KB per SM at full bandwidth, at all times:
-// also while a part is being joined and the next one begins.  A quarter to a third of a block's warps
-// therefore only look rows up and copy them (cp.async, 16 bytes a lane) to shared memory, through all of the block's
-// parts.  Step k of a part is for computing warp k modulo their number; each of these has a ring of its
-// own, filled by one copying warp, so that both sides of a ring take its slots in the same order and a
-// barrier's parity always tells the round that is meant.  (With one ring for all, a warp could be two
-// rounds from another: the parity of the wrong one then passes for the right one.)  The pieces lie in
-// the order of the lanes that will use them (piece j of lane l at (32 j + l) * size), free of bank
-// conflicts.
+// also while a part is being joined and the next one begins.  A quarter to a half of a block's warps
+// therefore only look rows up and copy them (cp.async, mostly 16 bytes a lane) to shared memory, through all of
+// the block's parts.  Each computing warp has a ring of its own, filled by one copying warp, so that both
+// sides of a ring take its slots in the same order and a barrier's parity always tells the round that is
+// meant.  (With one ring for all, a warp could be two rounds from another: the parity of the wrong one then
+// passes for the right one.)  The pieces lie in the order of the lanes that will use them (piece j of lane l
+// at (32 j + l) * size), free of bank conflicts.
 struct PaRing {
   uint8_t* steps;            // [computing warp][slot]
   uint64_t* full;            // per slot: its copies and `live` are there
@@ -398,26 +402,43 @@ struct PaPlace {
   }
 };
 
-// One token of a step, held by one lane: where its rows are.
+// One token of a step, held by one lane: its page and slot.  The page id is on its way while the step before is
+// copied; nothing looks at it until then.
 struct PaToken {
-  int64_t k, v;       // byte offsets in the pages
+  int page, slot;
+  bool in;            // a visible token
+};
+
+__device__ __forceinline__ PaToken pa_token(const PagedAttnParams& p, const PaWork& w, int i, bool mine) {
+  PaToken t;
+  t.in = mine && i < w.t1;
+  const int pos = i + (i < w.seq.sinks ? 0 : w.seq.skip), at = qg_div(pos, p.kv.page_div);
+  t.slot = pos - at * p.kv.page_size;
+  t.page = 0;
+  if (t.in) t.page = __ldg(p.kv.table + w.b * p.kv.table_ld + at);
+  return t;
+}
+
+// Where its rows are, as byte offsets in the pages; not ok if it is none or the table names no page of the pool.
+struct PaRows {
+  int64_t k, v;
   bool ok;
 };
 
 template <typename T>
-__device__ __forceinline__ PaToken pa_token(const PagedAttnParams& p, const PaWork& w, const int32_t* trow, int i, bool mine,
-                                            int& page, int& slot) {
-  PaToken t;
-  page = slot = 0;
-  t.ok = mine && i < w.t1 && paged_slot(p.kv, trow, i + (i < w.seq.sinks ? 0 : w.seq.skip), page, slot);
-  t.k = (page * p.kv.kst[0] + slot * p.kv.kst[2]) * int(sizeof(T));
-  t.v = (page * p.kv.vst[0] + slot * p.kv.vst[2]) * int(sizeof(T));
-  return t;
+__device__ __forceinline__ PaRows pa_rows(const PagedAttnParams& p, PaToken& t) {
+  PaRows r;
+  r.ok = t.in && static_cast<uint32_t>(t.page) < static_cast<uint32_t>(p.kv.num_pages);
+  if (t.in && !r.ok) atomicExch(p.kv.err, PAGED_ERR);
+  if (!r.ok) t.page = t.slot = 0;
+  r.k = (t.page * p.kv.kst[0] + t.slot * p.kv.kst[2]) * int(sizeof(T));
+  r.v = (t.page * p.kv.vst[0] + t.slot * p.kv.vst[2]) * int(sizeof(T));
+  return r;
 }
 
+// n: BYTES, or 0 for zeros, when nothing is read.
 template <int BYTES>
-__device__ __forceinline__ void pa_copy(uint32_t dst, const uint8_t* src, bool ok) {
-  const uint32_t n = ok ? BYTES : 0;      // 0: zeros, nothing is read
+__device__ __forceinline__ void pa_copy(uint32_t dst, const uint8_t* src, uint32_t n) {
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
 }
@@ -428,48 +449,43 @@ __device__ __forceinline__ float pa_exp2(float x) {
   return y;
 }
 
-// Copying warp `me` of `feeders`: its steps of every part, step k going to copying warp k modulo their
-// number, i.e. to the rings of computing warps me, me + feeders, ..  look(w, at) finds the tokens at.. of
-// the part (a step ahead of their copies), copy(w, step) issues the copies of the tokens found last into
-// a slot and returns which of them count.
-constexpr int PA_FED = 3;      // most computing warps per copying warp
+// The steps of all of a block's parts are numbered through; step n is for computing warp n modulo their number.
+// Copying warp `me` of `feeders`, which divide the computing warps, does steps me, me + feeders, .., i.e. fills
+// the rings of computing warps me, me + feeders, ..  copy(w, tokens, step) issues the copies of the tokens into
+// a slot and returns which of them count.  A step has to be copied in about 1000 clocks for the memory to stay
+// busy (one copying warp of eight: twice the time), so that little may be worked out per step: the page ids
+// come a step ahead, and full steps are copied without a look at each token (48 x 20/4 heads of 80 up to 8000,
+// bf16: 72.2 -> 68.1 us).
+__device__ __forceinline__ int pa_steps(const PaWork& w, int tile) { return w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / tile + 1 : 0; }
 
-template <int TILE, class Look, class Copy>
+template <int TILE, class Copy>
 __device__ __forceinline__ void pa_feed(const PagedAttnParams& p, PaWork& w, const PaRing& ring, int step_bytes, int me, int feeders,
-                                        int warps, Look look, Copy copy) {
+                                        int warps, Copy copy) {
   const int lane = threadIdx.x & 31;
-  PaPlace places[PA_FED];
-#pragma unroll
-  for (int i = 0; i < PA_FED; ++i) places[i] = PaPlace{0, 0};
+  PaPlace place{0, 0};
+  int to = me, mine = me;      // the next computing warp; this warp's next step, from the part's first
   while (pa_part<TILE>(p, w)) {
-    look(w, w.t0 + me * TILE);
-    int fed = 0, to = me;       // the computing warp is `to`, the fed-th of this copying warp's
-    for (int t = w.t0 + me * TILE; t < w.t1; t += feeders * TILE) {
-      PaPlace mine = places[0];
-#pragma unroll
-      for (int i = 1; i < PA_FED; ++i)
-        if (fed == i) mine = places[i];
-      const int at = to * ring.slots + mine.slot;
-      pa_wait(ring, ring.empty + at, mine.round ^ 1);       // the first round finds every slot empty
+    const int steps = pa_steps(w, TILE);
+    PaToken next = pa_token(p, w, w.t0 + mine * TILE + lane, lane < TILE);
+    for (; mine < steps; mine += feeders) {
+      const PaToken tokens = next;
+      next = pa_token(p, w, w.t0 + (mine + feeders) * TILE + lane, lane < TILE);
+      const int at = to * ring.slots + place.slot;
+      pa_wait(ring, ring.empty + at, place.round ^ 1);       // the first round finds every slot empty
       __syncwarp();
-      const uint32_t live = copy(w, ring.steps + int64_t(at) * step_bytes);
+      const uint32_t live = copy(w, tokens, ring.steps + int64_t(at) * step_bytes);
       cp_async_arrive_noinc(ring.full + at);
       if (lane == 0) {
         ring.live[at] = live;
         mbar_arrive(ring.full + at);
       }
-      mine.forward(ring.slots);
-#pragma unroll
-      for (int i = 0; i < PA_FED; ++i)
-        if (fed == i) places[i] = mine;
       to += feeders;
-      ++fed;
       if (to >= warps) {
         to = me;
-        fed = 0;
+        place.forward(ring.slots);
       }
-      look(w, t + feeders * TILE);
     }
+    mine -= steps;
     w.cur = w.end;
   }
   cp_async_commit();
@@ -486,7 +502,7 @@ __device__ __forceinline__ void pa_feed(const PagedAttnParams& p, PaWork& w, con
 // A row is spread over LPR lanes, 16 bytes each, a warp takes TPS rows at a time and U times that in a
 // step.  The LPR partial sums of the step's U GP scores are added crosswise, each exchange halving the
 // number of scores a lane carries, so that a score's softmax is worked out in few lanes, not in all.
-// 64 sequences of up to 1024 tokens, 12 heads of 64 (205 MB): 50.8 us, 4.0 TB/s; what is above the bytes' 31 us
+// 64 sequences of up to 1024 tokens, 12 heads of 64 (205 MB): 44.3 us, 4.6 TB/s; what is above the bytes' 31 us
 // is mostly the launch, the dealing out, and the beginnings and ends of the 768 units' parts.
 template <int DHP, int GP>
 struct PaF32 {
@@ -502,6 +518,9 @@ struct PaF32 {
   static constexpr int LEFT = N >> HALVINGS;                // scores a lane ends up with
   static constexpr int WIDTH = LPR >> HALVINGS;             // lanes that end up with the same scores
   static constexpr int WARPS = GP * EPL <= 8 ? 16 : 12;     // of an SM
+  // as many copying as computing warps: with one query head a step is copied about as fast as it is used (64 x 12
+  // heads of 64 up to 1024 tokens: 44.3 us, with six computing and two copying warps 47.3)
+  static constexpr bool EVEN = GP == 1;
 };
 
 template <int DHP, int GP>
@@ -518,41 +537,44 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
   const PaRing ring = pa_ring_at(pa_smem, warps, p.slots, C::STEP, &s_abort);
 
   if (warp >= warps) {
-    PaToken tok;
-    auto look = [&](const PaWork& w, int at) {
-      int page, slot;
-      tok = pa_token<float>(p, w, p.kv.table + w.b * p.kv.table_ld, at + lane, lane < C::TILE, page, slot);
-    };
-    auto copy = [&](const PaWork& w, uint8_t* step) {
+    uint32_t size[C::NV];        // of this lane's accesses of a row
+#pragma unroll
+    for (int j = 0; j < C::NV; ++j) size[j] = (sub + j * C::LPR) * 4 < p.kv.dh ? 16 : 0;
+    auto copy = [&](const PaWork& w, PaToken tokens, uint8_t* step) {
+      const PaRows tok = pa_rows<float>(p, tokens);
       const int kvh = w.unit / p.head_blocks;
       const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.k) + kvh * p.kv.kst[1] + sub * 4);
       const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const float*>(p.kv.v) + kvh * p.kv.vst[1] + sub * 4);
       const uint32_t live = __ballot_sync(0xffffffffu, tok.ok);
       const uint32_t dst = smem_u32(step) + lane * 16;
+      auto rows = [&](auto full) {
 #pragma unroll
-      for (int u = 0; u < C::U; ++u) {
-        const int i = u * C::TPS + row0;
-        const uint8_t* k = kb + __shfl_sync(0xffffffffu, tok.k, i);
-        const uint8_t* v = vb + __shfl_sync(0xffffffffu, tok.v, i);
-        const bool in = live >> i & 1;
+        for (int u = 0; u < C::U; ++u) {
+          const int i = u * C::TPS + row0;
+          const uint8_t* k = kb + __shfl_sync(0xffffffffu, tok.k, i);
+          const uint8_t* v = vb + __shfl_sync(0xffffffffu, tok.v, i);
+          const bool in = decltype(full)::value || (live >> i & 1);
 #pragma unroll
-        for (int j = 0; j < C::NV; ++j) {
-          const bool inside = in && (sub + j * C::LPR) * 4 < p.kv.dh;
-          pa_copy<16>(dst + (u * C::NV + j) * 512, k + j * C::LPR * 16, inside);
-          pa_copy<16>(dst + ((C::U + u) * C::NV + j) * 512, v + j * C::LPR * 16, inside);
+          for (int j = 0; j < C::NV; ++j) {
+            pa_copy<16>(dst + (u * C::NV + j) * 512, k + j * C::LPR * 16, in ? size[j] : 0);
+            pa_copy<16>(dst + ((C::U + u) * C::NV + j) * 512, v + j * C::LPR * 16, in ? size[j] : 0);
+          }
         }
-      }
+      };
+      if (live == uint32_t((uint64_t(1) << C::TILE) - 1)) rows(std::true_type{});
+      else rows(std::false_type{});
       return live;
     };
-    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, look, copy);
+    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, copy);
     if (lane == 0 && s_abort) atomicExch(p.kv.err, 1);
     return;
   }
 
   PaPlace mine{0, 0};
+  int next = warp;      // this warp's next step, from the part's first
   while (pa_part<C::TILE>(p, w)) {
     const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * GP;
-    const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
+    const int steps = pa_steps(w, C::TILE);
 
     float q[GP][C::EPL], acc[GP][C::EPL], m[GP], l[C::LEFT];
 #pragma unroll
@@ -572,7 +594,7 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
 
     // this lane's scores are first .. first + LEFT - 1 of its group's rows, score u GP + gi
     const int first = sub / C::WIDTH * C::LEFT;
-    for (int k = warp; k < steps; k += warps) {
+    for (; next < steps; next += warps) {
       const int slot = warp * ring.slots + mine.slot;
       pa_wait(ring, ring.full + slot, mine.round);
       const uint32_t now = ring.live[slot];
@@ -691,6 +713,7 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
       if (lane == 0) mbar_arrive(ring.empty + slot);
       mine.forward(ring.slots);
     }
+    next -= steps;
 
     // l of each head: the lanes' sums of its scores
     float lsum[GP];
@@ -721,7 +744,7 @@ __global__ void __launch_bounds__(PaF32<DHP, GP>::WARPS * 32, 1)
       if (row0 == 0) {
 #pragma unroll
         for (int j = 0; j < C::NV; ++j)
-          *reinterpret_cast<float4*>(to + pa_head(GP) + gi * DHP + (sub + j * C::LPR) * 4) =
+          *reinterpret_cast<float4*>(to + pa_at<DHP>(GP, gi, sub + j * C::LPR)) =
               make_float4(acc[gi][4 * j], acc[gi][4 * j + 1], acc[gi][4 * j + 2], acc[gi][4 * j + 3]);
       }
       if (lane == 0) {

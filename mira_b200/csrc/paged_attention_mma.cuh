@@ -7,12 +7,12 @@
 // unpacking, the addresses and the waiting.  (Products of 64 or 128 tokens at a time out of shared memory
 // would leave the heads' columns as empty, and hand P back through memory; the operands here never leave
 // the registers, and the bytes, not the products, set the pace.)
-// Measured: 32 sequences of up to 8192 tokens, 32 heads over 8 of 128, bf16 (553 MB): 128 us, 4.3 TB/s, where
-// the steps alone run at 91% of the copy rate and 35 us go to the launch and the ends of the 256 units and their
-// parts.  One sequence of 131071 tokens, 32 heads over 4, f16 (268 MB): 71.7 us; its steps take 47 us, joining
+// Measured: 32 sequences of up to 8192 tokens, 32 heads over 8 of 128, bf16 (553 MB): 124 us, 4.5 TB/s, where
+// the steps alone run at 91% of the copy rate and some 30 us go to the launch and the ends of the 256 units and their
+// parts.  One sequence of 131071 tokens, 32 heads over 4, f16 (268 MB): 72 us; its steps take 47 us, joining
 // the 37 parts of each unit 10.  48 sequences, window 4095, 20 heads over 4 of 80, codes under f32 queries
-// (121 MB): 62.4 us; here the unpacking and products of the computing warps are the limit (issue slots 43%
-// busy, four to six warps of an SM).
+// (121 MB): 56 to 61 us; here the unpacking and products of the computing warps are the limit (issue slots 45%
+// busy by eight to twelve warps of an SM).  Head sizes up to 96 have a class of their own: in that of 128 it took 62.7.
 //   S^T = K Q^T: lane (g, t) holds elements VE t .. VE t + VE - 1 of each run of 4 VE of tokens g and g + 8,
 //     16 bytes as they came from memory: four elements of each are a left fragment.  The sums over k do
 //     not care in which order k comes; Q is laid out to match, once per unit.
@@ -123,18 +123,13 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
   const PaRing ring = pa_ring_at(pa_smem, warps, p.slots, C::STEP, &s_abort);
 
   if (warp >= warps) {
-    PaToken tok;
-    int64_t ks_at = 0, vs_at = 0;
-    auto look = [&](const PaWork& w, int at) {
-      int page, slot;
-      tok = pa_token<T>(p, w, p.kv.table + w.b * p.kv.table_ld, at + lane, lane < C::TILE, page, slot);
-      if (C::I8) {
-        const int kvh = w.unit / p.head_blocks;
-        ks_at = page * p.kv.kss[0] + kvh * p.kv.kss[1] + slot * p.kv.kss[2];
-        vs_at = page * p.kv.vss[0] + kvh * p.kv.vss[1] + slot * p.kv.vss[2];
-      }
-    };
-    auto copy = [&](const PaWork& w, uint8_t* step) {
+    uint32_t ksize[C::KL], vsize[C::VL];       // of this lane's accesses of a row
+#pragma unroll
+    for (int j = 0; j < C::KL; ++j) ksize[j] = (j * 4 + t) * C::KE < p.kv.dh ? VB : 0;
+#pragma unroll
+    for (int j = 0; j < C::VL; ++j) vsize[j] = (j * 8 + g) * C::VE < p.kv.dh ? C::VBV : 0;
+    auto copy = [&](const PaWork& w, PaToken tokens, uint8_t* step) {
+      const PaRows tok = pa_rows<T>(p, tokens);
       const int kvh = w.unit / p.head_blocks;
       const uint8_t* kb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.k) + kvh * p.kv.kst[1] + t * C::KE);
       const uint8_t* vb = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.kv.v) + kvh * p.kv.vst[1] + g * C::VE);
@@ -142,42 +137,49 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
       const uint32_t kd = smem_u32(step) + lane * VB, vd = smem_u32(step) + C::K_BYTES + lane * C::VBV;
       if (C::I8) {
         const uint32_t sd = smem_u32(step) + C::K_BYTES + C::V_BYTES + lane * 4;
-        pa_copy<4>(sd, reinterpret_cast<const uint8_t*>(p.kv.ks + ks_at), tok.ok);
-        pa_copy<4>(sd + 128, reinterpret_cast<const uint8_t*>(p.kv.vs + vs_at), tok.ok);
+        const float* ks = p.kv.ks + tokens.page * p.kv.kss[0] + kvh * p.kv.kss[1] + tokens.slot * p.kv.kss[2];
+        const float* vs = p.kv.vs + tokens.page * p.kv.vss[0] + kvh * p.kv.vss[1] + tokens.slot * p.kv.vss[2];
+        pa_copy<4>(sd, reinterpret_cast<const uint8_t*>(ks), tok.ok ? 4 : 0);
+        pa_copy<4>(sd + 128, reinterpret_cast<const uint8_t*>(vs), tok.ok ? 4 : 0);
       }
+      auto rows = [&](auto full) {
 #pragma unroll
-      for (int r = 0; r < C::TT; ++r) {
+        for (int r = 0; r < C::TT; ++r) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int i = r * 16 + n * 8 + g;
-          const uint8_t* row = kb + __shfl_sync(0xffffffffu, tok.k, i);
-          const bool in = live >> i & 1;
+          for (int n = 0; n < 2; ++n) {
+            const int i = r * 16 + n * 8 + g;
+            const uint8_t* row = kb + __shfl_sync(0xffffffffu, tok.k, i);
+            const bool in = decltype(full)::value || (live >> i & 1);
 #pragma unroll
-          for (int j = 0; j < C::KL; ++j)
-            pa_copy<VB>(kd + ((r * 2 + n) * C::KL + j) * (32 * VB), row + j * 4 * VB, in && (j * 4 + t) * C::KE < p.kv.dh);
+            for (int j = 0; j < C::KL; ++j)
+              pa_copy<VB>(kd + ((r * 2 + n) * C::KL + j) * (32 * VB), row + j * 4 * VB, in ? ksize[j] : 0);
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
+            const uint8_t* row = vb + __shfl_sync(0xffffffffu, tok.v, i);
+            const bool in = decltype(full)::value || (live >> i & 1);
+#pragma unroll
+            for (int j = 0; j < C::VL; ++j)
+              pa_copy<C::VBV>(vd + ((r * 4 + n) * C::VL + j) * (32 * C::VBV), row + j * 8 * C::VBV, in ? vsize[j] : 0);
+          }
         }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int i = r * 16 + (n >> 1) * 8 + 2 * t + (n & 1);
-          const uint8_t* row = vb + __shfl_sync(0xffffffffu, tok.v, i);
-          const bool in = live >> i & 1;
-#pragma unroll
-          for (int j = 0; j < C::VL; ++j)
-            pa_copy<C::VBV>(vd + ((r * 4 + n) * C::VL + j) * (32 * C::VBV), row + j * 8 * C::VBV, in && (j * 8 + g) * C::VE < p.kv.dh);
-        }
-      }
+      };
+      if (live == uint32_t((uint64_t(1) << C::TILE) - 1)) rows(std::true_type{});
+      else rows(std::false_type{});
       return live;
     };
-    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, look, copy);
+    pa_feed<C::TILE>(p, w, ring, C::STEP, warp - warps, feeders, warps, copy);
     if (lane == 0 && s_abort) atomicExch(p.kv.err, 1);
     return;
   }
 
   PaPlace mine{0, 0};
+  int next = warp;      // this warp's next step, from the part's first
   while (pa_part<C::TILE>(p, w)) {
     const int kvh = w.unit / p.head_blocks, g0 = (w.unit - kvh * p.head_blocks) * (8 * NH);
     const int h0 = kvh * p.group + g0, live_heads = min(8 * NH, p.group - g0);
-    const int steps = w.t1 > w.t0 ? (w.t1 - w.t0 - 1) / C::TILE + 1 : 0;
+    const int steps = pa_steps(w, C::TILE);
 
     // queries of the unit in fragment order, a warp per head, four elements of it per lane and turn.  f16
     // values of a query that is not f16 itself are taken after a power of two has brought its largest
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[n][b][i] = 0.0f;
 
-    for (int k = warp; k < steps; k += warps) {
+    for (; next < steps; next += warps) {
       const int slot = warp * ring.slots + mine.slot;
       pa_wait(ring, ring.full + slot, mine.round);
       const uint32_t now = ring.live[slot];
@@ -402,6 +404,7 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
       if (lane == 0) mbar_arrive(ring.empty + slot);
       mine.forward(ring.slots);
     }
+    next -= steps;
 
     // the warp's triple
     const float back = C::BF16 ? 1.0f : 0x1p-8f;
@@ -420,12 +423,10 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
           to[rows + h] = l[b][i] * back;
         }
         // tile n: elements 2 n and 2 n + 1 of the lane's runs
-        float* a = to + pa_head(rows) + h * DHP;
 #pragma unroll
         for (int n = 0; n < C::NT; ++n) {
           const int d = ((2 * n) / C::VE * 8 + g) * C::VE + (2 * n) % C::VE;
-          a[d] = acc[n][b][i] * back_v;
-          a[d + 1] = acc[n][b][2 + i] * back_v;
+          *reinterpret_cast<float2*>(to + pa_at<DHP>(rows, h, d / 4) + d % 4) = make_float2(acc[n][b][i] * back_v, acc[n][b][2 + i] * back_v);
         }
       }
     pa_finish<DHP>(p, w, s_join, warps, rows, h0, live_heads);

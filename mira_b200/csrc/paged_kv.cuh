@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __gr
 // Bound: the moved pages are read and written once.  The page ids travel in the kernel's parameters, so
 // that nothing has to be copied to the device before it: few of them in a small parameter block (5 pages of
 // 24 planes: 10.0 us a call; with 4 KB of parameters 12.5), up to 1000 in one launch.  700 pages of 16 KB in
-// 32 planes (734 MB read and written): 119.8 us, 6.13 TB/s, 93% of the copy rate (in two launches 125.6).
+// 32 planes (734 MB read and written): 120 us, 6.1 TB/s, 93% of the copy rate (in two launches 125.6).
 constexpr int PAGE_COPY_FEW = 32, PAGE_COPY_SOME = 256, PAGE_COPY_MANY = 1000;     // pairs per launch
 constexpr int PAGE_COPY_CHUNK = 16384;    // bytes of one block's share of a page
 constexpr int PAGE_COPY_THREADS = 256;

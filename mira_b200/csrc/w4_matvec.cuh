@@ -19,9 +19,9 @@
 // row groups with the ring running ahead over their ends.  Where the rows alone would leave SMs idle,
 // or x is wide, k is also cut over blocks (blockIdx.z); the parts are joined in order by the block
 // that finishes last.
-// Measured: one f16 row through 32768 x 8192, groups of 64 (143 MB): 43.0 us, 3.3 TB/s; 360 instructions per
+// Measured: one f16 row through 32768 x 8192, groups of 64 (143 MB): 43 to 47 us, 3.3 TB/s; 360 instructions per
 // 2 KB of weights keep 59% of the issue slots busy, and that, not the bytes, is the limit.  16 bf16 rows through
-// 4096 x 4096, groups of 128, GELU: 14.4 us.  768 x 768: 6.1 us, the time to launch it from the host.  Three
+// 4096 x 4096, groups of 128, GELU: 14.4 to 16.6 us.  768 x 768: 6.1 us, the time to launch it from the host.  Three
 // blocks per SM, stages of 512 k and any fixed wr were no faster.
 #pragma once
 #include <cstdint>

@@ -212,7 +212,7 @@ def _ring_run(seed, feeders, warps, slots, steps):
     raise AssertionError("the ring stands still")
 
 
-@pytest.mark.parametrize("feeders,warps", [(4, 12), (4, 8), (3, 6), (2, 6), (2, 4), (1, 3), (1, 2)])
+@pytest.mark.parametrize("feeders,warps", [(4, 12), (4, 8), (4, 4), (3, 6), (2, 6), (2, 4), (1, 3), (1, 2)])
 @pytest.mark.parametrize("slots", [1, 2, 3, 4])
 def test_every_warp_reads_its_own_steps_in_order(feeders, warps, slots):
     steps = 15 * warps + 1
