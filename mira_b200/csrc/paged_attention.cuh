@@ -58,9 +58,10 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedAttnParams& p, int b) {
 // by unit; block c of g takes [total c / g, total (c + 1) / g).  Before its tiles each unit has an empty
 // stretch of PA_PART_COST: a part's beginning and end take a block as long as about that many tiles, and
 // without it the blocks that get many short sequences finish last (64 sequences of 16 to 1024 tokens: the
-// last block at twice the median's time).  Of 4, 8, 14 and 24 tiles, 14 is the best or within 3% of it on
-// two dozen shapes; 4 and 24 lose up to 40%.
-constexpr int PA_PART_COST = 14;
+// last block at twice the median's time).  Of 10, 14, 20 and 28 tiles on 32 shapes, 20 is the best or within 4%
+// of it on 28 (32 sequences of 32/8 heads up to 8192, bf16: 128 us, with 14 122; 80 x 96/12 heads, f32: 121 us, with
+// 14 145; 48 x 20/4 heads of 80, bf16: 68 us, with 14 73); 4 loses up to 40%.
+constexpr int PA_PART_COST = 20;
 // Quotients of nonnegative numbers; nearly all fit 32 bits, where dividing takes a fraction of the time.
 __device__ __forceinline__ int64_t pa_quot(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
