@@ -505,8 +505,9 @@ int mira_cuda_kv_append(const mira_kv_append* a);
  * tokens of all sequences are dealt out evenly over the GPU's SMs; the parts of one (sequence, head)
  * are joined in a fixed order by whichever block finishes last, so equal inputs give equal bits.
  * workspace: device memory of mira_cuda_paged_attention_workspace() bytes, 16-byte aligned, ZEROED
- * ONCE by the caller before its first use; every call leaves it ready for the next.  Calls sharing a
- * workspace must not overlap. */
+ * ONCE by the caller before its first use; every call leaves it ready for the next, which may have
+ * other sizes or be a mira_cuda_w4_matvec: one buffer of the largest size serves them all.  Calls
+ * sharing a workspace must not overlap. */
 typedef struct mira_paged_attention {
   mira_paged_kv kv;
   int64_t heads;

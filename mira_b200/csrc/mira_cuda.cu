@@ -2129,8 +2129,6 @@ namespace mira {
 
 constexpr int PA_MAX_BLOCKS_PER_SM = 2;
 
-static int64_t pa_counters(int64_t batch, int64_t units) { return round_up(batch * units * 4, 256); }
-
 // Rows of any alignment.
 template <typename T>
 static int launch_paged_any(DeviceState* dev, PagedAttnParams& p) {
@@ -2227,7 +2225,7 @@ extern "C" int64_t mira_cuda_paged_attention_workspace(int64_t batch, int64_t he
   int dhp = 64;
   while (dhp < dh) dhp *= 2;
   const int64_t triple = pa_triple(int(rows), dhp) > pa_triple(1, 256) ? pa_triple(int(rows), dhp) : pa_triple(1, 256);
-  return pa_counters(batch, heads) + int64_t(dev->sm_count) * PA_MAX_BLOCKS_PER_SM * 2 * triple * 4;
+  return WORK_COUNTER_BYTES + int64_t(dev->sm_count) * PA_MAX_BLOCKS_PER_SM * 2 * triple * 4;
 }
 
 extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
@@ -2268,7 +2266,7 @@ extern "C" int mira_cuda_paged_attention(const mira_paged_attention* a) {
   p.q8 = make_qscale(p.out_i8 != nullptr ? a->out_scale : 1.0f);
   p.lse = a->lse;
   p.counters = static_cast<int*>(a->workspace);
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pa_counters(a->kv.batch, a->heads));
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + WORK_COUNTER_BYTES);
   const bool vec = paged_rows_aligned(a->kv, 16);
   switch (a->kv.dtype) {
     case MIRA_DT_F32:
@@ -2322,6 +2320,7 @@ static int w4_plan(int sm_count, int gs, W4Params& p) {
       const int share = W4_WARPS / wr;
       if (share > most) break;
       const int64_t groups = (tiles + wr - 1) / wr;
+      if (cuts > 1 && groups * passes > WORK_COUNTERS) continue;     // without cuts there are blocks enough then
       const int64_t rounds = (groups * cuts * passes + at_once - 1) / at_once;
       const int want = (per + share - 1) / share * share, fit = most / share * share;
       const int64_t panels = (per + fit - 1) / fit;
@@ -2339,8 +2338,6 @@ static int w4_plan(int sm_count, int gs, W4Params& p) {
   }
   return p.panel > 0 ? MIRA_CUDA_OK : set_error(MIRA_CUDA_EINVAL, "no room for the rows of x");
 }
-
-static int64_t w4_counters(int64_t m, int64_t n) { return round_up((m + 7) / 8 * ((n + 15) / 16) * 4, 256); }
 
 template <int XT, int NB, int GS, bool EXACT>
 static int launch_w4_kernel(DeviceState* dev, const W4Params& p) {
@@ -2384,7 +2381,7 @@ extern "C" int64_t mira_cuda_w4_matvec_workspace(int64_t m, int64_t n, int64_t k
       p.m = int(m); p.n = int(n); p.k = int(k); p.x_dtype = dtype;
       if (w4_plan(dev->sm_count, gs, p) == MIRA_CUDA_OK && p.cuts > cuts) cuts = p.cuts;
     }
-  return cuts > 1 ? w4_counters(m, n) + int64_t(cuts) * m * n * 4 : 0;
+  return cuts > 1 ? WORK_COUNTER_BYTES + int64_t(cuts) * m * n * 4 : 0;
 }
 
 extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
@@ -2428,10 +2425,10 @@ extern "C" int mira_cuda_w4_matvec(const mira_w4_matvec* a) {
   if (rc != MIRA_CUDA_OK) return rc;
   if (p.cuts > 1) {
     MIRA_CHECK_ARG(a->workspace != nullptr && aligned_to(a->workspace, 16) &&
-                       a->workspace_bytes >= w4_counters(p.m, p.n) + int64_t(p.cuts) * p.m * p.n * 4,
+                       a->workspace_bytes >= WORK_COUNTER_BYTES + int64_t(p.cuts) * p.m * p.n * 4,
                    "workspace smaller than mira_cuda_w4_matvec_workspace()");
     p.counters = static_cast<int*>(a->workspace);
-    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + w4_counters(p.m, p.n));
+    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + WORK_COUNTER_BYTES);
   }
   const int nb = w4_nb(p.x_dtype, p.m);
   switch (p.x_dtype) {

@@ -30,7 +30,7 @@ struct PagedAttnParams {
   QuantScale q8;
   float* lse;
   float* part;              // partial triples, two slots per block
-  int* counters;            // [batch * units], zero between calls
+  int* counters;            // [blocks], zero between calls
   int slots, feeders;       // steps in a warp's ring, copying warps of a block
 };
 
@@ -265,7 +265,7 @@ __device__ __forceinline__ void pa_finish(const PagedAttnParams& p, const PaWork
   }
   const int first = pa_block_of(w.total, w.ts, w.blocks), last = pa_block_of(w.total, w.ue - 1, w.blocks);
   pa_sync(threads);
-  int* counter = p.counters + int64_t(w.b) * p.units + w.unit;
+  int* counter = p.counters + first;      // of the units that a block begins only its last goes on in the next
   if (threadIdx.x == 0) {
     __threadfence();      // the whole block's slot, by the barrier before
     s_last = atomicAdd(counter, 1) == last - first;

@@ -13,6 +13,11 @@
 
 namespace mira {
 
+// A workspace begins with this many counters, whatever the operator and its sizes, and the sums of parts come
+// after them: the counters, zero between calls, are then where no call of any size leaves a sum.
+constexpr int64_t WORK_COUNTERS = 16384;
+constexpr int64_t WORK_COUNTER_BYTES = WORK_COUNTERS * 4;
+
 constexpr int PAGED_ERR = 4;   // error record: a page id, length or row range outside its bounds
 
 struct PagedKv {
