@@ -452,7 +452,8 @@ int mira_cuda_dynamic_update_slice(const mira_view4* x, const int64_t* x_dims, c
  * ops.py:310-313 and ops.py:217-219.  Lengths and tables are device memory, read by the kernels, so
  * a captured graph stays valid while they change.  A negative length or one beyond the table's
  * max_pages * page_size, or a page id outside [0, num_pages), touches no memory outside the pool:
- * the kernel leaves those tokens out and the next mira_cuda_sync fails with MIRA_CUDA_EKERNEL. */
+ * the kernel leaves those tokens out (an append: every row of a sequence with such a length) and the
+ * next mira_cuda_sync fails with MIRA_CUDA_EKERNEL. */
 
 /* element types */
 #define MIRA_DT_F32 0

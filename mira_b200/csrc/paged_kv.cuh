@@ -34,15 +34,18 @@ struct PagedKv {
   int* err;
 };
 
-// Tokens of sequence b, clamped to what its table row can hold (positions are below 2^31).
-__device__ __forceinline__ int paged_length(const PagedKv& p, int b) {
+// Tokens of sequence b (positions are below 2^31), negative when its table row cannot hold them, which is recorded.
+__device__ __forceinline__ int paged_count(const PagedKv& p, int b) {
   const int n = __ldg(p.lengths + b);
-  const int cap = p.max_pages * p.page_size;
-  if (n < 0 || n > cap) {
-    atomicExch(p.err, PAGED_ERR);
-    return n < 0 ? 0 : cap;
-  }
-  return n;
+  if (n >= 0 && n <= p.max_pages * p.page_size) return n;
+  atomicExch(p.err, PAGED_ERR);
+  return -1;
+}
+
+// Tokens to be read of sequence b: those that its table row can hold.
+__device__ __forceinline__ int paged_length(const PagedKv& p, int b) {
+  const int n = paged_count(p, b);
+  return n >= 0 ? n : __ldg(p.lengths + b) < 0 ? 0 : p.max_pages * p.page_size;
 }
 
 // Page and slot of a position; false (and an error record) when the table names no page of the pool.
@@ -190,8 +193,8 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const __gr
       from_end = int(min(int64_t(__ldg(p.row_start + b + 1)) - row, int64_t(INT32_MAX)));
       if (__ldg(p.row_start + b) > row) from_end = 0;
     }
-    const int n = paged_length(kv, b);
-    if (n == 0 && p.row_start == nullptr) continue;
+    const int n = paged_count(kv, b);
+    if (n < 0 || (n == 0 && p.row_start == nullptr)) continue;      // where the rows belong is not known, or none is wanted
     const int pos = n - from_end;
     int page, slot;
     if (from_end <= 0 || pos < 0) {
