@@ -480,8 +480,9 @@ typedef struct mira_paged_kv {
  * one row per sequence, row b; rows == batch) as its LAST positions, i.e. lengths[b] already counts
  * them and row row_start[b] + i goes to position lengths[b] - n_b + i.  A sequence of length 0 takes
  * no row.  Values are rounded once to the pages' type (nearest even); MIRA_DT_I8 rows get
- * scale = absmax / 127 (1 for a row of zeros) and codes clip(rint(x / scale), -127, 127).  Every
- * position must be in a page that no other sequence holds; pages shared after a fork are only read. */
+ * scale = absmax / 127 (1 for a row of zeros) and codes clip(rint(x / scale), -127, 127); a NaN or
+ * infinity in a row makes its scale one, and what the row stands for NaN.  Every position must be in a
+ * page that no other sequence holds; pages shared after a fork are only read. */
 typedef struct mira_kv_append {
   mira_paged_kv kv;
   int64_t rows;

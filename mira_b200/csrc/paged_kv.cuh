@@ -151,7 +151,7 @@ __device__ __forceinline__ void append_codes(const float (&x)[TURNS][W], int8_t*
 #pragma unroll
     for (int i = 0; i < W; ++i) top = np_maximum(top, fabsf(x[j][i]));
   for (int o = lanes >> 1; o > 0; o >>= 1) top = np_maximum(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float s = top > 0.0f ? __fdiv_rn(top, 127.0f) : 1.0f;
+  const float s = top == 0.0f ? 1.0f : __fdiv_rn(top, 127.0f);      // NaN if the row has one, so that it shows
   if (!mine) return;
   if (sub == 0) *scale = s;
 #pragma unroll
