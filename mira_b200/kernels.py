@@ -719,7 +719,7 @@ def page_copy(regions, num_pages: int, src, dst) -> None:
 
 def w4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
     """Symmetric 4-bit codes int8 [n, k] in [-7, 7] and f32 scales [n, ceil(k / group)] of f32 weights
-    [n, k]: scale = absmax / 7 of each group (1 for a group of zeros)."""
+    [n, k]: scale = absmax / 7 of each group (1 for a group of zeros, not finite for one that is not)."""
     w = np.asarray(w, np.float32)
     n, k = w.shape
     groups = -(-k // group)
@@ -727,8 +727,10 @@ def w4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
     padded[:, :k] = w
     blocks = padded.reshape(n, groups, group)
     top = np.abs(blocks).max(axis=2)
-    scales = np.where(top > 0, top / np.float32(7), np.float32(1)).astype(np.float32)
-    q = np.clip(np.round(blocks / scales[:, :, None]), -7, 7).astype(np.int8)
+    with np.errstate(all="ignore"):
+        scales = np.where(top == 0, np.float32(1), top / np.float32(7)).astype(np.float32)
+        ratio = np.nan_to_num(blocks / scales[:, :, None], nan=0.0)
+    q = np.clip(np.round(ratio), -7, 7).astype(np.int8)
     return q.reshape(n, -1)[:, :k].copy(), scales
 
 
