@@ -705,13 +705,21 @@ def page_regions(regions: Sequence[PageRegion]):
     return (_lib.PageRegion * len(regions))(*[r.struct() for r in regions])
 
 
+def _page_ids(ids) -> np.ndarray:
+    """Whole numbers as a C array of 32 bits; what 32 bits do not hold is no page."""
+    if not (isinstance(ids, np.ndarray) and ids.dtype == np.int32):
+        ids = np.asarray(ids)
+        if ids.size and (ids.dtype.kind not in "iu" or ids.min() < -2 ** 31 or ids.max() >= 2 ** 31):
+            raise ValueError("page ids are 32-bit integers")
+    return np.ascontiguousarray(ids, np.int32)
+
+
 def page_copy(regions, num_pages: int, src, dst) -> None:
     """Page dst[i] becomes a copy of page src[i] in every plane of every region (a sequence of
     PageRegion, or page_regions() of it); src and dst are host integers."""
     if not isinstance(regions, C.Array):
         regions = page_regions(regions)
-    src = np.ascontiguousarray(src, np.int32)
-    dst = np.ascontiguousarray(dst, np.int32)
+    src, dst = _page_ids(src), _page_ids(dst)
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError("src and dst are lists of the same length")
     _lib.call("mira_cuda_page_copy", len(regions), regions, num_pages, len(src), src.ctypes.data, dst.ctypes.data)

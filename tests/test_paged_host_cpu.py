@@ -36,3 +36,34 @@ def test_w4_quantize_of_the_smallest_weights():
         warnings.simplefilter("error")
         q, s = K.w4_quantize(w, 32)
     assert (q * s == 0).all() and np.abs(q).max() <= 7
+
+
+@pytest.mark.parametrize("src,dst", [([2 ** 32], [1]), ([0], [2 ** 32 + 1]), ([-2 ** 32], [1]), ([0.7], [1]), ([0], [1.5]),
+                                     ([float("nan")], [1]), ([True], [False]), (["0"], ["1"])])
+@pytest.mark.parametrize("array", [True, False])
+def test_page_copy_takes_page_ids_only(monkeypatch, src, dst, array):
+    """Ids that 32 bits do not hold, and what is no whole number, are refused, not cut to some page's id."""
+    calls = []
+    monkeypatch.setattr(K._lib, "call", lambda *a: calls.append(a))
+    region = [K.PageRegion(1 << 20, page_bytes=16, page_stride=16)]
+    if array:
+        src, dst = np.array(src), np.array(dst)
+    with pytest.raises(ValueError):
+        K.page_copy(region, 4, src, dst)
+    assert not calls
+
+
+@pytest.mark.parametrize("kind", [list, tuple, np.array, lambda x: np.array(x, np.int64), lambda x: np.array(x, np.uint8)])
+def test_page_copy_passes_page_ids(monkeypatch, kind):
+    calls = []
+
+    def call(name, n_regions, regions, num_pages, n, src, dst):
+        import ctypes
+        read = lambda at: list((ctypes.c_int32 * n).from_address(at)) if n else []
+        calls.append((name, num_pages, n, read(src), read(dst)))
+
+    monkeypatch.setattr(K._lib, "call", call)
+    region = [K.PageRegion(1 << 20, page_bytes=16, page_stride=16)]
+    K.page_copy(region, 9, kind([3, 3]), kind([5, 8]))
+    K.page_copy(region, 9, [], [])
+    assert calls == [("mira_cuda_page_copy", 9, 2, [3, 3], [5, 8]), ("mira_cuda_page_copy", 9, 0, [], [])]
