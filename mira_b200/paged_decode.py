@@ -171,17 +171,24 @@ class PagedTransformer:
 
     def generate(self, prompt, new_tokens: int, slot: Optional[int] = None) -> tuple[int, list]:
         """Feeds a prompt to a new sequence (or to `slot`) and appends `new_tokens` greedy ones; returns
-        (slot, the new tokens)."""
+        (slot, the new tokens).  If it raises, a sequence that it opened is closed again; one that was
+        there keeps the tokens that it was fed."""
         if not len(prompt):
             raise ValueError("an empty prompt")
-        slot = self.cache.open() if slot is None else slot
+        opened = slot is None
+        slot = self.cache.open() if opened else slot
         out, logits = [], None
-        for t in prompt:
-            logits = self.step({slot: int(t)})[slot]
-        for i in range(new_tokens):
-            out.append(int(np.argmax(logits)))
-            if i + 1 < new_tokens:
-                logits = self.step({slot: out[-1]})[slot]
+        try:
+            for t in prompt:
+                logits = self.step({slot: int(t)})[slot]
+            for i in range(new_tokens):
+                out.append(int(np.argmax(logits)))
+                if i + 1 < new_tokens:
+                    logits = self.step({slot: out[-1]})[slot]
+        except Exception:
+            if opened:      # the caller does not know the slot
+                self.cache.close(slot)
+            raise
         return slot, out
 
     def close(self) -> None:
