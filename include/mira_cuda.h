@@ -502,8 +502,11 @@ int mira_cuda_kv_append(const mira_kv_append* a);
  * sequence of length 0 gives o = 0 and lse = -inf.  lse[b * heads + h] = log sum_t exp(scale q . k_t)
  * (natural logarithm), which joins this result with another over other keys.
  * Scores, softmax statistics and sums are f32; k and v enter the products exactly, and so does q, or (f32
- * q with f16 or 8-bit pages) to 2^-22 of its head's largest element.  An infinite element of a visible
- * row makes the results that it enters infinite or NaN.  The visible
+ * q with f16 or 8-bit pages) to 2^-22 of its head's largest element.  With 16- and 8-bit pages a weight
+ * enters the sums to 2^-16 (bf16 q over bf16 pages) or 2^-22 of it, but f16 and 8-bit pages hold it no finer
+ * than 2^-31 of the largest weight (8-bit pages: of the largest weight times its scale, whatever scales
+ * the other rows have).  An infinite element or scale of a visible row makes the results that it enters
+ * infinite or NaN.  The visible
  * tokens of all sequences are dealt out evenly over the GPU's SMs; the parts of one (sequence, head)
  * are joined in a fixed order by whichever block finishes last, so equal inputs give equal bits.
  * workspace: device memory of mira_cuda_paged_attention_workspace() bytes, 16-byte aligned, ZEROED

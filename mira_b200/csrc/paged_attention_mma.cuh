@@ -22,8 +22,8 @@
 //     blocks by movmatrix.
 // Exactness: q enters as one value of the pages' type where it has that type, else as three bf16 values
 // whose sum it is, or as two f16 values that agree with it to 2^-22 of the head's largest element; 8-bit
-// codes become exact f16 values.  p is f32 and enters as PP values that agree with it to 16
-// bits or more (see PaMma), the row's sum l is of the f32 values.
+// codes become exact f16 (or bf16) values.  p is f32, with 8-bit pages times the value's scale, and enters as PP
+// values that agree with it to 16 bits or more (see PaMma); the row's sum l is of the f32 values.
 #pragma once
 #include <cstdint>
 
@@ -52,8 +52,14 @@ struct PaMma {
   // and 22, whose error of 2^-22 of the largest weight is that of an f32 sum of a few terms; the same
   // goes for the two f16 values of a query element.  In f16, p is carried times 2^8: the smallest f16 is
   // then 2^-32 of the largest weight.
+  // 8-bit pages: what enters is p times the value's scale, of sizes that nothing limits (an append gives a row
+  // of zeros the scale 1, whatever its neighbours have).  It is taken relative to the largest scale so far and
+  // times 2^V_SHIFT, as two f16 values as long as all scales so far are within 2^-V_NEAR of that one, so that an f16
+  // rounds to 2^-31 of the largest weight times its own scale or less; then as three bf16 values, which have f32's
+  // range (48 x 20/4 heads of 80, window: 57.4 us; with bf16 values for every step 66.1).
   static constexpr int PP = BF16 && QP > 1 ? 3 : 2;
-  static constexpr float SHIFT = BF16 ? 0.0f : 8.0f;
+  static constexpr float SHIFT = BF16 || I8 ? 0.0f : 8.0f;
+  static constexpr int V_SHIFT = 14, V_NEAR = 8;
   static constexpr int K_BYTES = TT * 2 * KL * 32 * VB, V_BYTES = TT * 4 * VL * 32 * VBV;    // of a step
   static constexpr int STEP = K_BYTES + V_BYTES + (I8 ? 2 * 32 * 4 : 0);      // 8-bit pages: and the scales
   // warps of an SM, by the registers of the sums and by the ring: a computing warp wants two steps of it
@@ -96,6 +102,12 @@ __device__ __forceinline__ void pa_split2(float x, float y, uint32_t (&out)[N]) 
 // low mantissa bits of 1024, 1152 is subtracted exactly.
 __device__ __forceinline__ uint32_t pa_codes(uint32_t biased, uint32_t sel) {
   return h2_bits(__hsub2(bits_h2(__byte_perm(biased, 0x64646464u, sel)), bits_h2(0x64806480u)));
+}
+
+// The codes in the low bytes of both halves as a bf16 pair: the seven low bits under the exponent of 128, less 128,
+// or 256 for the sign bit, which under the same exponent is the next one.
+__device__ __forceinline__ uint32_t pa_codes_bf16(uint32_t x) {
+  return b2_bits(__hsub2(bits_b2((x & 0x007f007fu) | 0x43004300u), bits_b2((x & 0x00800080u) | 0x43004300u)));
 }
 
 template <int WORDS> struct PaWords { uint32_t w[WORDS]; };
@@ -238,7 +250,8 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
         m[b][i] = -INFINITY;
         l[b][i] = 0.0f;
       }
-    uint32_t v_exp = 1;       // 8-bit pages: exponent of the largest value scale so far, which acc is divided by
+    // 8-bit pages: exponents of the largest value scale so far, which acc is divided by, and of the smallest but 0
+    uint32_t v_exp = C::V_SHIFT + 1, v_low = 255;
 #pragma unroll
     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
@@ -318,12 +331,15 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
           for (int o = 4; o < 32; o <<= 1) top[b][i] = fmaxf(top[b][i], __shfl_xor_sync(0xffffffffu, top[b][i], o));
         }
       float grow = 1.0f, shrink = 1.0f;
-      if (C::I8) {
-        const float vscale = lane < C::TILE && (now >> lane & 1) ? sc[32 + lane] : 0.0f;
-        const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vscale))) >> 23, v_exp), 253u);
-        grow = __int_as_float((127 - min(int(e - v_exp), 126)) << 23);
+      bool spread = false;
+      if (C::I8) {       // tokens that do not count have the scale 0
+        const uint32_t bits = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
+        const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, bits) >> 23, v_exp), 254u);
+        v_low = min(v_low, __reduce_min_sync(0xffffffffu, bits - 1) >> 23);      // 0 is left out as the largest
+        spread = e > v_low + C::V_NEAR;
+        grow = e - v_exp > 126 ? 0.0f : __int_as_float((127 - (e - v_exp)) << 23);
         v_exp = e;
-        shrink = __int_as_float((254 - e) << 23);
+        shrink = __int_as_float((254 + C::V_SHIFT - e) << 23);
       }
       bool moved = grow != 1.0f;
 #pragma unroll
@@ -343,9 +359,11 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
             }
           }
       }
-#pragma unroll
-      for (int r = 0; r < C::TT; ++r) {
-        uint32_t pt[NH][2][C::PP];       // P^T: tokens 2t, 2t + 1 (+ 8) of head g
+      // the weights as PC values of bf16 (PBF16) or f16, times the values
+      auto values = [&](int r, auto bf16, auto pieces) {
+        constexpr bool PBF16 = decltype(bf16)::value;
+        constexpr int PC = decltype(pieces)::value;
+        uint32_t pt[NH][2][PC];          // P^T: tokens 2t, 2t + 1 (+ 8) of head g
 #pragma unroll
         for (int b = 0; b < NH; ++b)
 #pragma unroll
@@ -355,14 +373,11 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
             for (int i = 0; i < 2; ++i) {
               x[i] = pa_exp2(s[r][b][2 * n + i] - ((m[b][i] == -INFINITY ? 0.0f : m[b][i]) - C::SHIFT));
               l[b][i] += x[i];
-              if (C::I8) {       // a token that does not count has no scale either
-                const int token = r * 16 + n * 8 + g;
-                x[i] *= now >> token & 1 ? sc[32 + token] * shrink : 0.0f;
-              }
+              if (C::I8) x[i] *= sc[32 + r * 16 + n * 8 + g] * shrink;
             }
-            pa_split2<C::BF16, C::PP>(x[0], x[1], pt[b][n]);
+            pa_split2<PBF16, PC>(x[0], x[1], pt[b][n]);
 #pragma unroll
-            for (int q = 0; q < C::PP; ++q) pt[b][n][q] = pa_transpose(pt[b][n][q]);
+            for (int q = 0; q < PC; ++q) pt[b][n][q] = pa_transpose(pt[b][n][q]);
           }
 #pragma unroll
         for (int j = 0; j < C::VL; ++j) {
@@ -377,7 +392,13 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t x = vx[2 * h].w[e], y = vx[2 * h + 1].w[e];
-              if (C::I8) {
+              if (C::I8 && PBF16) {
+                const uint32_t low = __byte_perm(x, y, 0x5410), high = __byte_perm(x, y, 0x7632);
+                a[0][h] = pa_codes_bf16(low);
+                a[1][h] = pa_codes_bf16(low >> 8);
+                a[2 % PER][h] = pa_codes_bf16(high);
+                a[3 % PER][h] = pa_codes_bf16(high >> 8);
+              } else if (C::I8) {
                 const uint32_t bx = x ^ 0x80808080u, by = y ^ 0x80808080u;
                 const uint32_t low = __byte_perm(bx, by, 0x5140), high = __byte_perm(bx, by, 0x7362);
                 a[0][h] = pa_codes(low, 0x4140);
@@ -394,11 +415,16 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
 #pragma unroll
               for (int b = 0; b < NH; ++b)
 #pragma unroll
-                for (int q = C::PP - 1; q >= 0; --q)
-                  mma_16816<C::BF16>(acc[(j * C::VE + e * PER) / 2 + i][b], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1],
-                                     pt[b][0][q], pt[b][1][q]);
+                for (int q = PC - 1; q >= 0; --q)
+                  mma_16816<PBF16>(acc[(j * C::VE + e * PER) / 2 + i][b], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1],
+                                   pt[b][0][q], pt[b][1][q]);
           }
         }
+      };
+#pragma unroll
+      for (int r = 0; r < C::TT; ++r) {
+        if (C::I8 && spread) values(r, std::true_type{}, std::integral_constant<int, 3>{});
+        else values(r, std::integral_constant<bool, C::BF16>{}, std::integral_constant<int, C::PP>{});
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(ring.empty + slot);
@@ -407,8 +433,8 @@ __global__ void __launch_bounds__(PaMma<T, DHP, VB, QP, NH>::WARPS * 32, 1)
     next -= steps;
 
     // the warp's triple
-    const float back = C::BF16 ? 1.0f : 0x1p-8f;
-    const float back_v = C::I8 ? back * __int_as_float(v_exp << 23) : back;
+    const float back = C::BF16 || C::I8 ? 1.0f : 0x1p-8f;
+    const float back_v = C::I8 ? __int_as_float((v_exp - C::V_SHIFT) << 23) : back;
     float* to = s_join + warp * pa_triple(rows, DHP);
 #pragma unroll
     for (int b = 0; b < NH; ++b)

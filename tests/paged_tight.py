@@ -4,9 +4,11 @@ For one (sequence, head) and element d let A_d = sum_t p_t |v_td| with p the sof
 the error of its score, relatively, and by the rounding of the exponential; the sums over t round each term
 independently, so that their errors add like sqrt(n), to A_d and to the sum of the weights alike:
 
-  |o_d - exact| <= 2 A_d (score + piece + (sqrt(n) + 8) eps) + |o_d| unit
+  |o_d - exact| <= 2 A_d (score + piece + (sqrt(n) + 8) eps) + |o_d| unit + n 2^-126 (max_t |v_td| + 128)
   score = (dh + 8) eps max_t sum_d |scale q_d k_td|  (+ what splitting q leaves, 2^-22 of its largest element)
   piece = what the values that a weight enters the products as leave of it, relatively
+the last term is for weights below 2^-126 of the largest, which are 0, and 8-bit codes times what f32 holds of a
+weight times a scale.
 
 It shrinks with the outputs, which are averages over n tokens, so that a missing or misweighted part shows."""
 import numpy as np
@@ -15,8 +17,8 @@ import paged_ref as R
 
 
 def piece(q, kv):
-    """What the weights' 16-bit values leave: none on the f32 path; two bf16 values 2^-16, three 2^-24; two f16
-    values 2^-22, each of the last twice over for the rounding of the largest."""
+    """What the weights' 16-bit values leave, twice over for the rounding of the largest: nothing on the f32 path;
+    two bf16 values 2^-16, three 2^-24; two f16 values 2^-22."""
     if kv == "f32":
         return 0.0
     if kv == "bf16":
@@ -51,7 +53,7 @@ def attention(q, k, v, table, lengths, page_size, scale, q_dtype, kv, window=0, 
             o[b, h], size[b, h] = p @ vv / total, p @ np.abs(vv) / total
             lse[b, h] = m + np.log(total)
             off = score + (np.sqrt(len(t)) + 8) * R.EPS
-            bound[b, h] = 2 * size[b, h] * (off + piece(q_dtype, kv))
+            bound[b, h] = 2 * size[b, h] * (off + piece(q_dtype, kv)) + len(t) * 2.0 ** -126 * (np.abs(vv).max(0) + 128)
             lse_bound[b, h] = off + 8 * R.EPS * abs(lse[b, h])
     bound += np.abs(o) * R.UNIT[q_dtype] * 1.01 + (2.0 ** -25 if q_dtype == "f16" else 0)
     return o, bound, size, lse, lse_bound

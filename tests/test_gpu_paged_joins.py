@@ -19,7 +19,7 @@ def _holds(c, got, lse, window=0, sinks=0):
     off = np.abs(got - o)
     assert (off <= bound).all(), float((off / np.maximum(bound, 1e-300)).max())
     live = np.isfinite(want_lse)
-    assert (lse[~live] == -np.inf).all() and (np.abs(lse - want_lse)[live] <= lse_bound[live]).all()
+    assert (lse[~live] == -np.inf).all() and (np.abs(lse[live] - want_lse[live]) <= lse_bound[live]).all()
     return o, bound
 
 
