@@ -13,7 +13,8 @@ A step is one forward pass of a batch through the compiled MIRA program.  `value
 on device-resident inputs (CUDA events on the library stream, max over ranks); `e2e` times the
 same K steps through the public API (`CompiledProgram.run` with pinned host inputs: host->device
 copy of the batch, the kernels, device->host copy of the logits).  `--impl reference` times the
-reference's own cpu W8A8 path (MIRA's NumPy golden model) on a bounded sample.
+reference's own cpu W8A8 path (MIRA's NumPy golden model) on a bounded sample; where the package
+`mira` is not installed it prints {"impl": "reference", "unavailable": why}.
 """
 from __future__ import annotations
 
@@ -735,6 +736,12 @@ def reference_decode_sample(steps: int, warmup: int, max_seconds: float = 60.0) 
 def run_reference(args) -> None:
     rank, world, _ = _env_rank()
     if rank != 0:
+        return
+    from mira_b200.hostfw import import_mira
+    try:
+        import_mira()
+    except ImportError as e:
+        print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
         return
     if args.workload == "decode":
         res = reference_decode_sample(args.steps, args.warmup)
