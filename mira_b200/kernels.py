@@ -746,6 +746,8 @@ def w4_weight(q: np.ndarray) -> np.ndarray:
     """4-bit codes int8 [n, k] in [-8, 7] -> uint8 [n, ld], ld = round_up(ceil(k / 2), 16): byte j
     holds q[2 j] + 8 in its low and q[2 j + 1] + 8 in its high four bits."""
     n, k = q.shape
+    if q.size and (q.min() < -8 or q.max() > 7):
+        raise ValueError("4-bit codes are in [-8, 7]")
     ld = round_up(-(-k // 2), 16)
     u = np.full((n, 2 * ld), 8, np.uint8)
     u[:, :k] = (q.astype(np.int16) + 8).astype(np.uint8)

@@ -67,3 +67,18 @@ def test_page_copy_passes_page_ids(monkeypatch, kind):
     K.page_copy(region, 9, kind([3, 3]), kind([5, 8]))
     K.page_copy(region, 9, [], [])
     assert calls == [("mira_cuda_page_copy", 9, 2, [3, 3], [5, 8]), ("mira_cuda_page_copy", 9, 0, [], [])]
+
+
+@pytest.mark.parametrize("bad", [8, -9, 127, -128])
+@pytest.mark.parametrize("dtype", [np.int8, np.int32])
+def test_w4_weight_takes_4_bit_codes_only(bad, dtype):
+    """A code that four bits do not hold would change its neighbour's."""
+    q = np.zeros((2, 5), dtype)
+    q[1, 2] = bad
+    with pytest.raises(ValueError):
+        K.w4_weight(q)
+    q[1, 2] = 7
+    q[0, 3] = -8
+    packed = K.w4_weight(q)
+    assert packed[1, 1] == 0x8f and packed[0, 1] == 0x08
+    assert K.w4_weight(np.zeros((0, 5), dtype)).shape == (0, 16)
