@@ -557,8 +557,8 @@ int mira_cuda_page_copy(int64_t n_regions, const mira_page_region* regions, int6
  * element k is not used.  scales: [n][ld_scales] of scale_dtype, ceil(k / group) used; group a
  * multiple of 32.  x, the weights and the scales enter the products exactly; sums are f32.  steps: the
  * epilogue steps of mira_epilogue on the f32 result (CHANNEL operands need n entries here, FULL
- * operands ptr[m * ld + n]); then one rounding to out_dtype.  Any m is taken; the weights are read
- * once per 16 rows (8 rows of f32).  workspace: as for mira_cuda_paged_attention, of
+ * operands ptr[m * ld + n]); then one rounding to out_dtype.  The weights are read once per 16 rows (8
+ * rows of f32), in at most 65535 such passes.  workspace: as for mira_cuda_paged_attention, of
  * mira_cuda_w4_matvec_workspace() bytes (0: none needed, workspace may be NULL). */
 typedef struct mira_w4_matvec {
   int64_t m, n, k, group;

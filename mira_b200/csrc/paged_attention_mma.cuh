@@ -11,7 +11,7 @@
 // the steps alone run at 91% of the copy rate and some 30 us go to the launch and the ends of the 256 units and their
 // parts.  One sequence of 131071 tokens, 32 heads over 4, f16 (268 MB): 72 us; its steps take 47 us, joining
 // the 37 parts of each unit 10.  48 sequences, window 4095, 20 heads over 4 of 80, codes under f32 queries
-// (121 MB): 57.6 us; here the unpacking and products of the computing warps are the limit (issue slots 45%
+// (121 MB): 57.4 us; here the unpacking and products of the computing warps are the limit (issue slots 45%
 // busy by eight to twelve warps of an SM).  Head sizes up to 96 have a class of their own: in that of 128 it took 62.7.
 //   S^T = K Q^T: lane (g, t) holds elements VE t .. VE t + VE - 1 of each run of 4 VE of tokens g and g + 8,
 //     16 bytes as they came from memory: four elements of each are a left fragment.  The sums over k do

@@ -141,7 +141,7 @@ __device__ __forceinline__ void append_get(const typename AppendElem<SRC>::type*
 
 // 8-bit codes of one row of keys or values, held by `lanes` lanes (lane `sub`), W elements each and turn:
 // scale = absmax / 127 and codes rint(x / scale), both IEEE divisions like the int8 weights,
-// whose instructions are the limit: 49152 rows of 8 heads of 128 from f32, 176 us (2.9 TB/s); reciprocals with
+// whose instructions are the limit: 42156 rows of 8 heads of 128 from f32, 155 us (2.8 TB/s); reciprocals with
 // the divisions left to the quotients near the middle of two codes were no faster.
 template <int W, int TURNS>
 __device__ __forceinline__ void append_codes(const float (&x)[TURNS][W], int8_t* dst, float* scale, int dh, int lanes, int sub, bool mine) {

@@ -4,7 +4,7 @@
 // Bound: the weights are read once, n k / 2 bytes (+ scales); everything else has to hide behind that.
 // An SM's share of the memory bandwidth is about 23 bytes a clock, i.e. 46 weights a clock that must
 // be unpacked and multiplied by every row of x.  FMA units need two to three instructions per weight
-// and row; the tensor path needs 1.4 for the unpacking and next to nothing per row: a word of eight
+// and row; the tensor path needs 1.1 (f16) or 1.4 (bf16) for the unpacking and next to nothing per row: a word of eight
 // weights becomes four registers of exact bf16 (or f16) pairs, which ARE the left operand's fragment
 // of two 16x8x16 products (16 weight rows x 16 k).  x is the right operand, its rows in the eight
 // columns: bf16 and f16 rows as they are, an f32 row as three columns whose bf16 values add up to it
@@ -19,7 +19,7 @@
 // row groups with the ring running ahead over their ends.  Where the rows alone would leave SMs idle,
 // or x is wide, k is also cut over blocks (blockIdx.z); the parts are joined in order by the block
 // that finishes last.
-// Measured: one f16 row through 32768 x 8192, groups of 64 (143 MB): 43 to 47 us, 3.3 TB/s; 360 instructions per
+// Measured: one f16 row through 32768 x 8192, groups of 64 (143 MB): 43 to 47 us, 3.3 TB/s; 374 warp instructions per
 // 2 KB of weights keep 59% of the issue slots busy, and that, not the bytes, is the limit.  16 bf16 rows through
 // 4096 x 4096, groups of 128, GELU: 14.4 to 16.6 us.  768 x 768: 6.1 us, the time to launch it from the host.  Three
 // blocks per SM, stages of 512 k and any fixed wr were no faster.
